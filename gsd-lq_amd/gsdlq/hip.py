@@ -44,6 +44,14 @@ SIGNATURES = {
     "gsdh_gqa_attention_noalloc": [vp] + [vp] * 4 + [i32] * 6 + [f32],
     "gsdh_prefill_attention": [vp] + [vp] * 4 + [i32] * 7 + [f32],
     "gsdh_unpack_codes": [vp, vp, i64, i32, vp, vp],
+    "gsdh_paged_attention": [vp, vp, i32, vp, i64, vp, i32, i32, f32, i32, vp, i64, vp, u64],
+    "gsdh_paged_rope_store": [vp, vp, i32] + [vp, i64] * 4 + [vp, vp, i32, i32, vp, i32, i32],
+    "gsdh_pages_take": [vp, vp, vp, vp, i32],
+    "gsdh_pages_fork": [vp, vp, vp, vp, i32, vp, u64],
+    "gsdh_pages_free": [vp, vp, vp, i32],
+    "gsdh_pages_compact": [vp, vp, vp, vp, u64],
+    "gsdh_pages_copy": [vp, vp, vp, vp, i32, vp, u64],
+    "gsdh_token_logprobs": [vp, vp, i32, i64, i32, i32, vp, i32, vp, vp, vp, vp, vp, u64],
     "gsdh_model_create": [vp, ctypes.POINTER(vp)],
     "gsdh_model_destroy": [vp],
     "gsdh_model_set_embedding": [vp, vp],
@@ -74,6 +82,9 @@ SIGNATURES = {
 RESTYPES = {"gsdh_model_device_bytes": (u64, [vp]), "gsdh_model_stream": (vp, [vp]),
             "gsdh_attention_workspace_bytes": (u64, [i32, i32, i32, i32]),
             "gsdh_model_fused_ffn": (i32, [vp, i32]),
+            "gsdh_paged_attention_workspace_bytes": (u64, [vp, i32, i32]),
+            "gsdh_pages_workspace_bytes": (u64, [vp]),
+            "gsdh_token_logprobs_workspace_bytes": (u64, [i32, i32, i32]),
             "gsdh_last_error": (ctypes.c_char_p, [])}
 
 
@@ -82,6 +93,20 @@ class GsdModelConfig(ctypes.Structure):
                 ("n_kv_heads", i32), ("head_dim", i32), ("vocab", i32), ("max_seq_len", i32),
                 ("rope_interleaved", i32), ("rms_eps", f32), ("rope_theta", f32)]
 
+
+class GsdPagedCache(ctypes.Structure):
+    """The paged KV cache that the gsdh_paged_* and gsdh_pages_* calls work on
+    (struct gsdh_paged_cache); pass ctypes.byref(cache)."""
+    _fields_ = [("k", vp), ("v", vp), ("k_scale", vp), ("v_scale", vp), ("refs", vp), ("tables", vp),
+                ("lens", vp), ("status", vp), ("n_layers", i32), ("n_pages", i32), ("page_size", i32),
+                ("n_kv_heads", i32), ("head_dim", i32), ("dtype", i32), ("head_major", i32),
+                ("n_seqs", i32), ("table_width", i32)]
+
+
+KV_TYPES = {"f16": 0, "bf16": 1, "e4m3": 2}
+LOGIT_TYPES = {"f32": 0, "f16": 1, "bf16": 2}
+# bits of a paged cache's status word
+PAGES_BAD_INDEX, PAGES_EXHAUSTED, PAGES_SHARED, PAGES_TWICE = 1, 2, 4, 8
 
 VECTORS = {"x": 0, "q": 1, "k": 2, "v": 3, "attn": 4, "h": 5, "logits": 6}
 

@@ -198,6 +198,143 @@ int gsdh_greedy_argmax_split(void* stream, const float* logits, int n, int* toke
                              uint64_t* words, uint32_t* counters);
 
 /* ------------------------------------------------------------------------ */
+/* 1b. Many sequences over one paged KV cache                                */
+/* ------------------------------------------------------------------------ */
+/* No counterpart in the reference, whose one sequence has one contiguous
+ * cache (run_gpu_native_chat.py:834-837).  K and V rows lie in pages of
+ * page_size positions; a sequence has a row of page indices, and a page may
+ * belong to several sequences (forks of one prompt).  Everything below is
+ * stream-ordered, allocates nothing, reads no result back to the host and may
+ * be captured into a graph: lengths, tables and lists are read on the device
+ * when the launch runs.  All pointers are device pointers of the current
+ * device.  Calls that write one cache (or share a workspace) must not overlap:
+ * keep them on one stream or order the streams. */
+
+enum { GSDH_KV_F16 = 0, GSDH_KV_BF16 = 1, GSDH_KV_E4M3 = 2 };
+
+/* Bits that launches OR into *status; it is the caller's to read and clear. */
+enum {
+    GSDH_PAGES_BAD_INDEX = 1,  /* a sequence, page or position outside the cache: left out */
+    GSDH_PAGES_EXHAUSTED = 2,  /* too few free pages: the sequence stayed as it was */
+    GSDH_PAGES_SHARED = 4,     /* a row for a page of several sequences (or of none): not written */
+    GSDH_PAGES_TWICE = 8       /* listed twice, or a fork into a sequence that holds tokens: left out */
+};
+
+typedef struct gsdh_paged_cache {
+    /* pools [n_layers][n_pages] of pages [page_size][n_kv_heads][head_dim] (a
+     * contiguous cache [layer][pos][kv head][dim] is one with the pages in
+     * order) or, with head_major, [n_kv_heads][page_size][head_dim]; 16-byte
+     * aligned */
+    void *k, *v;
+    /* e4m3 only (else NULL): float [n_layers][n_kv_heads]; value = e4m3 * scale */
+    const float *k_scale, *v_scale;
+    int *refs;        /* [n_pages] how many sequences hold the page; 0: free.  NULL where no page
+                         operator is used: rows are then stored without looking */
+    int *tables;      /* [n_seqs][table_width] page of positions page_size * j .. */
+    int *lens;        /* [n_seqs] positions held; 0: the sequence is free */
+    uint32_t *status; /* one word, GSDH_PAGES_* */
+    int n_layers, n_pages; /* n_pages up to 2^20 */
+    int page_size;    /* 8, 16, 32, 64, 128 or 256 */
+    int n_kv_heads, head_dim; /* head_dim 64, 128 or 256 */
+    int dtype;        /* GSDH_KV_* */
+    int head_major;
+    int n_seqs;       /* 1 .. 8192 */
+    int table_width;
+} gsdh_paged_cache;
+
+/* Attention of one new token per sequence (gsd_cpu_gqa_attention,
+ * gsd_lq_cpu_engine.c:264-330, for a batch and a paged cache): row i of q,
+ * q[i * q_stride + h * head_dim ..] with RoPE applied, attends over positions
+ * max(0, len - window) .. len - 1 of sequence seqs[i] (seqs NULL: sequence i),
+ * len = lens[seqs[i]]; window 0: all of them.  out[i * out_stride + ...] is
+ * softmax(sm_scale q.K) V in fp32.  A sequence of length 0 gives a row of
+ * zeros; a negative seqs[i] is padding, its row stays as it was; a row whose
+ * sequence, length or pages lie outside the cache becomes NaN (and *status
+ * says so).  n_heads / n_kv_heads 1 .. 16; strides in floats, multiples of 4,
+ * at least n_heads * head_dim for out (q's rows may be one and the same).
+ * workspace: gsdh_paged_attention_workspace_bytes(c, n, n_heads) bytes on this
+ * device (0 for an invalid shape), zero before its first call and 16-byte
+ * aligned; each call leaves it ready for the next, which may have other lengths
+ * and fewer rows but passes the same workspace_bytes.  The result does not depend on how the launch's blocks are ordered. */
+uint64_t gsdh_paged_attention_workspace_bytes(const gsdh_paged_cache* c, int n, int n_heads);
+int gsdh_paged_attention(void* stream, const gsdh_paged_cache* c, int layer, const float* q,
+                         int64_t q_stride, const int* seqs, int n, int n_heads, float sm_scale,
+                         int window, float* out, int64_t out_stride, void* workspace,
+                         uint64_t workspace_bytes);
+
+/* gsd_cpu_rope_and_store_kv (gsd_lq_cpu_engine.c:185-262) for n tokens of any
+ * sequences: token t is position positions[t] of sequence seqs[t]; its rows
+ * q[t * q_stride ..] (n_heads), k[t * k_stride ..] and v[t * v_stride ..]
+ * (n_kv_heads) are fp32.  q_out[t * q_out_stride ..] is the rotated q (q_out
+ * may be q with the same stride); RoPE(k) and v are rounded once to the
+ * cache's type and stored (e4m3: divided by the scale, beyond +-448 clamped).
+ * angles: float [n_angles][head_dim / 2][2], (cos, sin) per position, as the
+ * caller's model defines them; interleaved as in gsdh_rope_and_store_kv, and
+ * equal to it bit for bit on equal angles.  A negative seqs[t] is padding: the
+ * token's outputs stay as they were, and so for a position outside the
+ * sequence's length or the angles (GSDH_PAGES_BAD_INDEX) and a page that is
+ * not this sequence's alone (GSDH_PAGES_SHARED).  Tokens of one call must not
+ * share a position.  Strides in floats, multiples of 4; 16-byte aligned rows. */
+int gsdh_paged_rope_store(void* stream, const gsdh_paged_cache* c, int layer, const float* q,
+                          int64_t q_stride, const float* k, int64_t k_stride, const float* v,
+                          int64_t v_stride, float* q_out, int64_t q_out_stride, const int* seqs,
+                          const int* positions, int n, int n_heads, const float* angles, int n_angles,
+                          int interleaved);
+
+/* Pages.  All need c->refs; lists are device int [n], n <= n_seqs.  Free pages
+ * are taken lowest index first, in the order of the list, so the same calls
+ * give the same tables.  workspace: gsdh_pages_workspace_bytes(c) bytes, 16-byte
+ * aligned; what it holds before a call does not matter.
+ *
+ * take: sequence seqs[i] grows by counts[i] >= 0 positions (pages taken where
+ *   the last one is full, lens raised).  Sequences whose pages, counted in the
+ *   order of the list, do not fit stay as they were (GSDH_PAGES_EXHAUSTED).
+ * fork: the free sequence dst[i] becomes a second src[i]: full pages are
+ *   shared, the rows of a last page that is partly filled are copied (every
+ *   layer) to a page taken for it.  src as it was before the call.
+ * free: seqs[i] gives its pages back and has length 0; a sequence that is free
+ *   already stays so.
+ * compact: pages in use move to the lowest indices (the i-th lowest hole takes
+ *   the i-th lowest page that lies beyond), in every layer and in all tables;
+ *   *n_used (may be NULL) is how many there are.  Rows of a moved page's old
+ *   place keep their old bytes.
+ * copy: page dst[i] becomes a copy of page src[i] in every layer, n <= n_pages;
+ *   a negative index is padding.  refs and tables stay as they are.  A page
+ *   that is a destination twice takes the first source; a source that is also
+ *   a destination is left out (GSDH_PAGES_TWICE). */
+uint64_t gsdh_pages_workspace_bytes(const gsdh_paged_cache* c);
+int gsdh_pages_take(void* stream, const gsdh_paged_cache* c, const int* seqs, const int* counts, int n);
+int gsdh_pages_fork(void* stream, const gsdh_paged_cache* c, const int* src, const int* dst, int n,
+                    void* workspace, uint64_t workspace_bytes);
+int gsdh_pages_free(void* stream, const gsdh_paged_cache* c, const int* seqs, int n);
+int gsdh_pages_compact(void* stream, const gsdh_paged_cache* c, int* n_used, void* workspace,
+                       uint64_t workspace_bytes);
+int gsdh_pages_copy(void* stream, const gsdh_paged_cache* c, const int* src, const int* dst, int n,
+                    void* workspace, uint64_t workspace_bytes);
+
+/* Log probabilities of given tokens (the softmax behind sample_token,
+ * gsd_lq_cpu_runtime.py:422-443, without temperature), for n rows of `vocab`
+ * logits at logits + r * row_stride (elements of `dtype`):
+ *   logprob[r]  = x[tokens[r]] - ln sum exp x  (tokens[r] = -1: no token, 0;
+ *                 any other value outside the vocabulary: NaN)
+ *   entropy[r]  = -sum p ln p, in nats
+ *   top_ids[r][0 .. top_n), top_logprobs: the top_n largest, falling; equal
+ *                 logits by rising index.
+ * A logit of -inf has probability 0.  A row with a NaN, a +inf or nothing but
+ * -inf has no distribution: its logprob, entropy and top_logprobs are NaN (NaN
+ * ranks with -inf among top_ids).  tokens and logprob may both be NULL, as may
+ * entropy; top_ids and top_logprobs with top_n 0.  top_n <= min(32, vocab),
+ * vocab <= 2^20 - 8.  workspace: gsdh_token_logprobs_workspace_bytes bytes (may
+ * be 0), zero before its first call and 16-byte aligned; each call leaves it
+ * ready for the next, which may have fewer rows but passes the same
+ * workspace_bytes. */
+enum { GSDH_LOGITS_F32 = 0, GSDH_LOGITS_F16 = 1, GSDH_LOGITS_BF16 = 2 };
+uint64_t gsdh_token_logprobs_workspace_bytes(int n, int vocab, int top_n);
+int gsdh_token_logprobs(void* stream, const void* logits, int dtype, int64_t row_stride, int n, int vocab,
+                        const int* tokens, int top_n, float* logprob, float* entropy, int* top_ids,
+                        float* top_logprobs, void* workspace, uint64_t workspace_bytes);
+
+/* ------------------------------------------------------------------------ */
 /* 2. Model context (replaces GPUMistralV2Model's device side)              */
 /* ------------------------------------------------------------------------ */
 
