@@ -10,7 +10,7 @@ using namespace gsd;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kGroups = 64;         // of four threads
+constexpr int kGroups = 64;         // of four threads; a row has at most twice as many segments
 constexpr int kMaxTop = 32;
 constexpr int kMaxVocab = (1 << 20) - 8;   // 128 segments of 8192 at most, wherever the row starts
 constexpr int kMaxCand = 4096;      // keys that may reach a threshold (below)
@@ -35,7 +35,7 @@ struct LogprobArgs {
     float *logprob, *entropy, *top_lp;
     int* top_ids;
     unsigned* counters;       // [n], zero between launches
-    float4* part;             // [n][nseg] (m, s, t, -)
+    float* part;              // [n][nseg] (m, s, t, -)
     uint64_t* part_keys;      // [n][nseg][top]
     int64_t stride;
     int vocab, top, nseg;
@@ -229,25 +229,32 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a) 
 
     // this segment's part; the block that arrives last has all of them
     const int64_t slot = (int64_t)row * a.nseg + seg;
-    if (tid == 0) a.part[slot] = make_float4(m, s, t, 0.f);
-    if (tid < a.top) a.part_keys[slot * a.top + tid] = best[tid];
+    if (tid == 0) {
+        put2(a.part + 4 * slot, m, s);
+        put2(a.part + 4 * slot + 2, t, 0.f);
+    }
+    if (tid < a.top) __hip_atomic_store(&a.part_keys[slot * a.top + tid], best[tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    published();
     __syncthreads();
     if (tid == 0) {
-        __threadfence();
-        last = __hip_atomic_fetch_add(&a.counters[row], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)a.nseg - 1u;
-        __threadfence();
-        if (last) __hip_atomic_store(&a.counters[row], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = arrive(&a.counters[row], (unsigned)a.nseg);
         n_cand = 0;
     }
     __syncthreads();
     if (!last) return;
-    const float4* part = a.part + (int64_t)row * a.nseg;
+    const float* part = a.part + (int64_t)row * a.nseg * 4;
+    __shared__ float4 sums[2 * kGroups];
+    for (int i = tid; i < a.nseg; i += kThreads) {
+        const float2 p = get2(part + 4 * i), q = get2(part + 4 * i + 2);
+        sums[i] = make_float4(p.x, p.y, q.x, 0.f);
+    }
+    __syncthreads();
     float top = -INFINITY;
-    for (int i = 0; i < a.nseg; i++) top = fmaxf(top, part[i].x);
+    for (int i = 0; i < a.nseg; i++) top = fmaxf(top, sums[i].x);
     s = t = 0.f;
     const float cm = top == -INFINITY ? 0.f : top;
     for (int i = 0; i < a.nseg; i++) {
-        const float4 p = part[i];
+        const float4 p = sums[i];
         const float d = fmaxf(p.x - cm, -1e30f), f = __builtin_amdgcn_exp2f(d * kLog2e);
         s += f * p.y;
         t += f * (p.z + d * p.y);
@@ -257,11 +264,12 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a) 
         // largest of these are `top` at least
         const uint64_t* keys = a.part_keys + (int64_t)row * a.nseg * a.top;
         const int k = (a.top + a.nseg - 1) / a.nseg;
-        for (int i = tid; i < min(a.nseg, 2 * kGroups); i += kThreads) group[i] = keys[i * a.top + k - 1];
+        const auto get = [&](int i) { return __hip_atomic_load(&keys[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+        for (int i = tid; i < a.nseg; i += kThreads) group[i] = get(i * a.top + k - 1);
         __syncthreads();
-        const uint64_t least = a.nseg <= 2 * kGroups ? nth_largest(group, a.nseg, (a.top + k - 1) / k) : 0;
+        const uint64_t least = nth_largest(group, a.nseg, (a.top + k - 1) / k);
         for (int i = tid; i < a.nseg * a.top; i += kThreads) {
-            const uint64_t y = keys[i];
+            const uint64_t y = get(i);
             if (y != 0 && y >= least) {
                 const int p = atomicAdd(&n_cand, 1);
                 if (p < kMaxCand) cand[p] = y;
@@ -338,8 +346,8 @@ int gsdh_token_logprobs(void* stream, const void* logits, int dtype, int64_t row
     a.logprob = logprob; a.entropy = entropy; a.top_ids = top_ids; a.top_lp = top_logprobs;
     unsigned char* w = static_cast<unsigned char*>(workspace);
     a.counters = reinterpret_cast<unsigned*>(w);
-    a.part = reinterpret_cast<float4*>(w + counter_bytes(workspace_bytes));
-    a.part_keys = reinterpret_cast<uint64_t*>(a.part + (size_t)n * p.nseg);
+    a.part = reinterpret_cast<float*>(w + counter_bytes(workspace_bytes));
+    a.part_keys = reinterpret_cast<uint64_t*>(a.part + 4 * (size_t)n * p.nseg);
     if ((int64_t)n * p.nseg > 0x7FFFFFFF) return fail(-1, "%s: %d rows of %d logits in one call", who, n, vocab);
     hipStream_t st = static_cast<hipStream_t>(stream);
     GSD_PAGED_CHK(dtype == GSDH_LOGITS_F32 ? launch_logprobs<GSDH_LOGITS_F32>(a, n, p.e, st)

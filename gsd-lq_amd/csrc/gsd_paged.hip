@@ -1,5 +1,7 @@
 // gsd_paged.hip -- decode attention over a paged KV cache for a batch of
 // sequences, and RoPE with the append of K/V rows to its pages.
+#include <algorithm>
+
 #include "gsd_device.h"
 #include "gsd_paged.h"
 
@@ -12,9 +14,14 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr int kTile = 32;          // positions of one step of a wave
-constexpr int kWaves = 4;          // waves of a block, each on every fourth tile of its unit
-constexpr int kUnitsPerCu = 4;     // units that a launch is split into, per CU (about)
+constexpr int kWaves = 4;          // waves of a block, each on every fourth tile of its part
+constexpr int kRowCost = 128;      // what a row's start and end weigh beside its positions
+constexpr int kLeastSpan = 16;     // the least a block takes, in tiles
+static_assert(kLeastSpan >= 2 * kWaves, "every span inside a row has tiles of it");
+constexpr int kFan = 16;           // parts that one block joins at a time
+constexpr int kMostFans = 16;      // of a row and KV head
+// positions of a tile, the step of a wave: 8 KB of K and V (4 KB of rows of 64 bytes, 16 KB of rows of 512)
+constexpr int tile_positions(int row_bytes) { return row_bytes <= 128 ? 32 : 16; }
 constexpr int kMaxGroup = 16;      // query heads per KV head: the columns of one matrix product
 
 // ---------------------------------------------------------------------------
@@ -22,16 +29,17 @@ constexpr int kMaxGroup = 16;      // query heads per KV head: the columns of on
 //
 //   x_p = sm_scale q.K_p,  out = sum_p e^(x_p - m) V_p / sum_p e^(x_p - m)
 //
-// in one pass over K and V with a running maximum m and sum l.  A unit is a
-// run of 32-position tiles of one (row, KV head), whose query heads are the
-// columns of the matrix products: S^T = K Q^T and O^T = V^T P^T, 16 x 16 x 32.
-// The keys of a tile are dealt to the products' rows so that the
-// probabilities come out of the first product in the lane that the second
-// one needs them in: lane l (column = head l & 15, group j = l >> 4) gets the
-// scores of positions 4 j + r and 16 + 4 j + r (r < 4) and feeds the same
-// eight positions, for which it also loads V's rows (dims NT (l & 15) ..,
-// NT = head_dim / 16), so nothing goes through LDS or other lanes.  V's
-// eight rows are transposed in registers by byte permutes.
+// in one pass over K and V with a running maximum m and sum l.  A step of a
+// wave is a tile of 16 or 32 positions of one row and KV head, whose query
+// heads are the columns of the matrix products: S^T = K Q^T (16 x 16 x 32) and
+// O^T = V^T P^T (16 x 16 x 16, or x 32 of 32 positions).  The positions are
+// dealt to the products' rows so that the probabilities come out of the first
+// product in the lane that the second one needs them in: lane l (column =
+// head l & 15, group j = l >> 4) gets the scores of positions 4 j + r, and 16
+// + 4 j + r of a tile of 32 (r < 4), and feeds the same positions, for which
+// it also loads V's rows (dims NT (l & 15) .., NT = head_dim / 16), so nothing
+// goes through LDS or other lanes.  V's rows are transposed in registers by
+// byte permutes.
 //
 // fp32 inputs meet the cache's 16-bit rows as sums of 16-bit parts: two fp16
 // parts (22 bits; q scaled by a power of two so that its largest element is
@@ -43,11 +51,14 @@ struct AttendArgs {
     const float* q;
     const int* seqs;
     float* out;
-    unsigned* counters;   // [n][n_kv] arrivals of split rows, zero between launches
-    float* part;          // partial outputs [slot][G][HD], then (m, l) [slot][G][2]
+    unsigned* counters;   // arrivals of split rows [n][n_kv], counter_step words apart; zero between launches
+    // of rows with several parts: outputs [slot][G][HD], (m, l) [slot][G][2], for a span
+    // and KV head the part that continues a row, then the one that starts a row
+    float* part;
     float* part_ml;
     int64_t q_stride, out_stride;
-    int layer, n, group, window, target;   // target: units to split the work into
+    int layer, n, group, window, groups;   // groups: of blocks, one per KV head
+    unsigned counter_step;
     float scale;
 };
 
@@ -74,76 +85,112 @@ __device__ __forceinline__ Row row_of(const AttendArgs& a, int i) {
     r.first = a.window > 0 && len > a.window ? len - a.window : 0;
     return r;
 }
+template <int TP>
 __device__ __forceinline__ int tiles_of(const Row& r) {
-    return r.end > r.first ? (r.end - 1) / kTile - r.first / kTile + 1 : 0;
+    return r.end > r.first ? (r.end - 1) / TP - r.first / TP + 1 : 0;
 }
-// units of a row and KV head (a row without positions has one: it writes the row)
-__device__ __forceinline__ int units_of(const Row& r, int chunk) {
-    if (r.seq < 0) return 0;
-    const int t = tiles_of(r);
-    return t <= chunk ? 1 : (t + chunk - 1) / chunk;
+// what a row weighs in the split of the work: its tiles and, for the start and
+// the end of it, kRowCost more
+template <int TP>
+__device__ __forceinline__ unsigned cost_of(const Row& r) {
+    return r.seq < 0 ? 0u : (unsigned)(tiles_of<TP>(r) + kRowCost / TP);
 }
 
+// A part of a row and KV head: what one block does at a time.
 struct Unit {
     Row row;
-    int i;        // row of the call
-    int head;     // KV head
-    int split, splits;
-    int chunk;    // tiles per unit
-    int slot;     // of split 0's partial (splits > 1)
+    int i;                // row of the call
+    int t0, t1;           // tiles
+    int split, splits;    // which of the row's parts
+    int span;             // of the row's first part
 };
 
-// The unit of this block: every wave scans the rows by itself (lane l takes
-// a run of them), so that no barrier comes before the first loads.  The
-// chunk makes about `target` units of the launch's tiles, whatever the
-// lengths are; rows of a few tiles make one each beyond that.
-__device__ bool find_unit(const AttendArgs& a, unsigned u, Unit& o) {
-    const int lane = threadIdx.x & 63, per = (a.n + 63) / 64, lo = lane * per, hi = min(a.n, lo + per);
-    const int nkv = a.c.n_kv_heads;
-    long long mine = 0;
-    for (int i = lo; i < hi; i++) mine += tiles_of(row_of(a, i));
-    long long total = mine;
-#pragma unroll
-    for (int s = 32; s >= 1; s >>= 1) total += __shfl_xor(total, s, 64);
-    total *= nkv;
-    long long ch = (total + a.target - 1) / a.target;
-    ch = (ch + kWaves - 1) / kWaves * kWaves;
-    // (2^25 tiles hold the longest sequence)
-    const int chunk = (int)(ch < kWaves ? kWaves : ch > (1 << 25) ? 1 << 25 : ch);
-    // units in the low half, slots of split rows in the high half
-    unsigned long long cnt = 0;
-    for (int i = lo; i < hi; i++) {
-        const unsigned k = (unsigned)units_of(row_of(a, i), chunk);
-        cnt += k + ((unsigned long long)(k > 1 ? k : 0) << 32);
+// Sum over the lanes up to this one, in VALU: rows of 16 by shifts, then the
+// last lanes of rows 0 and 2, and of the first half, into what follows them.
+__device__ __forceinline__ unsigned wave_scan(unsigned v) {
+#define GSD_SCAN_STEP(ctrl, rows) v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, false)
+    GSD_SCAN_STEP(0x111, 0xF);   // row_shr 1, 2, 4, 8
+    GSD_SCAN_STEP(0x112, 0xF);
+    GSD_SCAN_STEP(0x114, 0xF);
+    GSD_SCAN_STEP(0x118, 0xF);
+    GSD_SCAN_STEP(0x142, 0xA);   // row_bcast 15, 31
+    GSD_SCAN_STEP(0x143, 0xC);
+#undef GSD_SCAN_STEP
+    return v;
+}
+
+// The parts of the rows that a block does.  The rows' costs lie one after
+// another, and every group of blocks (one block per KV head: what they read
+// together lies together) takes a span of `size` of them, so that all blocks
+// have as much to do whatever the lengths are.  A row is cut at multiples of
+// kWaves tiles.  Every wave goes through the rows by itself, 64 at a time, so
+// that no barrier comes before the first loads.
+struct RowSpan {
+    Row r;                     // the lane's row of the 64 at hand
+    unsigned lo, hi, size;     // the block's span
+    unsigned base, at, tiles;  // cost before the 64, before the lane's row; its tiles
+    int k;                     // which 64
+    unsigned long long mask;   // lanes whose rows have a part in the span, not yet done
+};
+
+// tiles of a row before cost x (the row starts at cost p)
+__device__ __forceinline__ unsigned cut(unsigned p, unsigned tiles, unsigned x) {
+    if (x <= p) return 0;
+    return x - p >= tiles ? tiles : (x - p) / kWaves * kWaves;
+}
+
+template <int TP>
+__device__ __forceinline__ void hold_rows(const AttendArgs& a, RowSpan& o, bool again) {
+    const int i = o.k * 64 + (int)(threadIdx.x & 63);
+    if (again) o.r = i < a.n ? row_of(a, i) : Row{-1, 0, 0, false};
+    const unsigned c = cost_of<TP>(o.r), incl = wave_scan(c);
+    o.at = o.base + incl - c;
+    o.base += (unsigned)__builtin_amdgcn_readlane((int)incl, 63);
+    o.tiles = (unsigned)tiles_of<TP>(o.r);
+    const bool part = o.tiles ? cut(o.at, o.tiles, o.hi) > cut(o.at, o.tiles, o.lo) : c && o.at >= o.lo && o.at < o.hi;
+    o.mask = __ballot(part);
+}
+
+template <int TP>
+__device__ __forceinline__ RowSpan parts_of(const AttendArgs& a, unsigned group) {
+    const int lane = threadIdx.x & 63;
+    RowSpan o{};
+    unsigned mine = 0;
+    for (int i = lane; i < a.n; i += 64) {
+        o.r = row_of(a, i);
+        mine += cost_of<TP>(o.r);
     }
-    unsigned long long incl = cnt;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-        const unsigned long long b = __shfl_up(incl, s, 64);
-        if (lane >= s) incl += b;
+    if (lane >= a.n) o.r = Row{-1, 0, 0, false};
+    const unsigned total = (unsigned)__builtin_amdgcn_readlane((int)wave_scan(mine), 63);
+    o.size = max((total + (unsigned)a.groups - 1) / (unsigned)a.groups, (unsigned)kLeastSpan);
+    o.lo = group * o.size;   // (groups * size is below 2^32: the launch's limit on positions)
+    o.hi = min(o.lo + o.size, total);
+    if (o.lo >= total) o.hi = o.lo;
+    hold_rows<TP>(a, o, a.n > 64);   // (up to 64 rows are at hand)
+    return o;
+}
+
+// The block's next part, or false.
+template <int TP>
+__device__ __forceinline__ bool next_part(const AttendArgs& a, RowSpan& o, Unit& u) {
+    while (!o.mask) {
+        o.k++;
+        if (o.base >= o.hi || o.k * 64 >= a.n) return false;
+        hold_rows<TP>(a, o, true);
     }
-    const unsigned v = u / (unsigned)nkv;
-    unsigned before = (unsigned)(incl - cnt), slots = (unsigned)((incl - cnt) >> 32);
-    const bool here = v >= before && v < (unsigned)incl;
-    const unsigned long long who = __ballot(here);
-    if (!who) return false;
-    int i = lo, k = 0;
-    if (here)
-        for (;; i++) {
-            k = units_of(row_of(a, i), chunk);
-            if (v < before + (unsigned)k) break;
-            before += k;
-            slots += k > 1 ? k : 0;
-        }
-    const int src = __builtin_ctzll(who);
-    o.i = __builtin_amdgcn_readlane(i, src);
-    o.splits = __builtin_amdgcn_readlane(k, src);
-    o.split = (int)v - __builtin_amdgcn_readlane((int)before, src);
-    o.slot = __builtin_amdgcn_readlane((int)slots, src) * nkv;
-    o.head = (int)(u - v * (unsigned)nkv);
-    o.slot += o.head * o.splits;
-    o.chunk = chunk;
-    o.row = row_of(a, o.i);
+    const int src = __builtin_ctzll(o.mask);
+    o.mask &= o.mask - 1;
+    const auto of = [&](int x) { return __builtin_amdgcn_readlane(x, src); };
+    u.i = o.k * 64 + src;
+    u.row = Row{of(o.r.seq), of(o.r.first), of(o.r.end), of((int)o.r.bad) != 0};
+    const unsigned p = (unsigned)of((int)o.at), tiles = (unsigned)of((int)o.tiles), t = (unsigned)(u.row.first / TP);
+    u.t0 = (int)(t + cut(p, tiles, o.lo));
+    u.t1 = (int)(t + cut(p, tiles, o.hi));
+    // the row's first part is in the span whose end cuts off something of it, its last where the row ends
+    const unsigned from = (p + min(tiles, (unsigned)kWaves) - 1) / o.size, to = tiles ? (p + tiles - 1) / o.size : from;
+    u.span = (int)from;
+    u.splits = (int)(to - from) + 1;
+    u.split = (int)(o.lo / o.size - from);
     return true;
 }
 
@@ -155,51 +202,60 @@ __device__ __forceinline__ float max_over_groups(float v) {   // over lanes l, l
 }
 __device__ __forceinline__ float sum_over_groups(float v) { return swap_add32(swap_add16(v, v), swap_add16(v, v), false); }
 
-// Eight fp32 values as parts of 16 bits whose sum they are
-template <int DT>
+// E (4 or 8) fp32 values as parts of 16 bits whose sum they are
+template <int DT, int E>
 struct Parts {
     static constexpr int N = DT == GSDH_KV_BF16 ? 3 : 2;
-    uint4 w[N];
+    typedef uint32_t Words __attribute__((ext_vector_type(E / 2)));
+    Words w[N];
 };
-template <int DT>
-__device__ __forceinline__ Parts<DT> split8(const float (&x)[8]) {
-    Parts<DT> p;
+template <int DT, int E>
+__device__ __forceinline__ Parts<DT, E> split(const float (&x)[E]) {
+    Parts<DT, E> p;
     if constexpr (DT == GSDH_KV_BF16) {
         // truncated parts: 8 + 8 + 8 bits, exact
-        uint32_t h[8], m[8], l[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            h[e] = __float_as_uint(x[e]);
-            const float r = x[e] - __uint_as_float(h[e] & 0xFFFF0000u);
-            m[e] = __float_as_uint(r);
-            l[e] = __float_as_uint(r - __uint_as_float(m[e] & 0xFFFF0000u));
+        for (int i = 0; i < E / 2; i++) {
+            float y[2] = {x[2 * i], x[2 * i + 1]};
+#pragma unroll
+            for (int n = 0; n < 3; n++) {
+                const uint32_t lo = __float_as_uint(y[0]), hi = __float_as_uint(y[1]);
+                p.w[n][i] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+                y[0] -= __uint_as_float(lo & 0xFFFF0000u);
+                y[1] -= __uint_as_float(hi & 0xFFFF0000u);
+            }
         }
-        auto pack = [](const uint32_t (&v)[8]) {
-            return make_uint4(__builtin_amdgcn_perm(v[1], v[0], 0x07060302u), __builtin_amdgcn_perm(v[3], v[2], 0x07060302u),
-                              __builtin_amdgcn_perm(v[5], v[4], 0x07060302u), __builtin_amdgcn_perm(v[7], v[6], 0x07060302u));
-        };
-        p.w[0] = pack(h);
-        p.w[1] = pack(m);
-        p.w[2] = pack(l);
     } else {
-        half8 h, l;
+        typedef _Float16 Halves __attribute__((ext_vector_type(E)));
+        Halves h, l;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
+        for (int e = 0; e < E; e++) {
             h[e] = (_Float16)x[e];
             l[e] = (_Float16)(x[e] - (float)h[e]);
         }
-        p.w[0] = __builtin_bit_cast(uint4, h);
-        p.w[1] = __builtin_bit_cast(uint4, l);
+        p.w[0] = __builtin_bit_cast(typename Parts<DT, E>::Words, h);
+        p.w[1] = __builtin_bit_cast(typename Parts<DT, E>::Words, l);
     }
     return p;
 }
 
 template <int DT>
-__device__ __forceinline__ float4v mma(const uint4 a, const uint4 b, float4v c) {
+__device__ __forceinline__ float4v mma(const u32x4v a, const u32x4v b, float4v c) {   // 16 x 16 x 32
     if constexpr (DT == GSDH_KV_BF16)
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+
+typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
+template <int DT>
+__device__ __forceinline__ float4v mma(const u32x2v a, const u32x2v b, float4v c) {   // 16 x 16 x 16
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+    if constexpr (DT == GSDH_KV_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s4, a), __builtin_bit_cast(s4, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(half4, a), __builtin_bit_cast(half4, b), c, 0, 0, 0);
 }
 
 // two e4m3 values (the low or the high half of w) as fp16: exact
@@ -216,8 +272,10 @@ struct Tile {
     static constexpr int KL = HD * ES / 64;       // 16-byte loads of a lane's part of a K row
     static constexpr int NT = HD / 16;            // dims of a lane's part of a V row
     static constexpr int VW = NT * ES / 4;        // its words
-    uint4 k[2][KL];
-    uint32_t v[8][VW];
+    static constexpr int TP = tile_positions(HD * ES), H = TP / 16;   // positions, halves of 16 of them
+    typedef uint32_t Words __attribute__((ext_vector_type(2 * H)));   // of a lane's 4 H positions, in 16 bits
+    uint4 k[H][KL];
+    uint32_t v[4 * H][VW];
 
     // dim of element 0 of product s's eight, lane group j
     static __device__ __forceinline__ int dim(int s, int j) {
@@ -255,248 +313,392 @@ struct Tile {
             return k[h][s];
         }
     }
-    // V's operands of the four (e4m3) or two dims of word w: positions 0 .. 7 of each dim
-    __device__ __forceinline__ void vfrags(int w, uint4* f) const {
-        uint32_t t[4][4];
+    // V's operands of the four (e4m3) or two dims of word w: the lane's positions of each dim
+    __device__ __forceinline__ void vfrags(int w, Words* f) const {
 #pragma unroll
-        for (int p = 0; p < 4; p++) {
+        for (int p = 0; p < 2 * H; p++) {
             const uint32_t a = v[2 * p][w], b = v[2 * p + 1][w];
             if constexpr (DT == GSDH_KV_E4M3) {
                 const uint32_t x = __builtin_amdgcn_perm(b, a, 0x05010400u), y = __builtin_amdgcn_perm(b, a, 0x07030602u);
-                t[0][p] = e4m3x2<false>(x);
-                t[1][p] = e4m3x2<true>(x);
-                t[2][p] = e4m3x2<false>(y);
-                t[3][p] = e4m3x2<true>(y);
+                f[0][p] = e4m3x2<false>(x);
+                f[1][p] = e4m3x2<true>(x);
+                f[2][p] = e4m3x2<false>(y);
+                f[3][p] = e4m3x2<true>(y);
             } else {
-                t[0][p] = __builtin_amdgcn_perm(b, a, 0x05040100u);
-                t[1][p] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+                f[0][p] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+                f[1][p] = __builtin_amdgcn_perm(b, a, 0x07060302u);
             }
         }
-#pragma unroll
-        for (int d = 0; d < 4 / ES; d++) f[d] = make_uint4(t[d][0], t[d][1], t[d][2], t[d][3]);
     }
 };
 
+// Joins `count` (up to kFan) parts of a row, first, first + step ..: into the
+// row's output, or into the place of the first.  All loads of a word are in
+// flight before the weights are formed (one after another the loads of 64
+// parts took 12 us).
+template <int HD>
+__device__ __forceinline__ void join_parts(const AttendArgs& a, const Unit& u, int head, int first, int step, int count, bool whole,
+                                           float* red, float* out, float vscale) {
+    const int tid = threadIdx.x, G = a.group;
+    constexpr int kThreads = 64 * kWaves;
+    auto slot_of = [&](int k) {
+        const int w = first + k * step;
+        return (unsigned)(((u.span + w) * a.c.n_kv_heads + head) * 2 + (w == 0));
+    };
+    static_assert(kThreads >= kFan * kMaxGroup && kFan == 16, "a thread per part and head, a row of lanes per head");
+    float *weight = red, *inv = red + kFan * kMaxGroup;   // [kFan][G], [G]
+    const int words = G * HD / 2, eg = tid / kFan, ew = tid % kFan;
+    const bool mine = eg < G && ew < count;
+    const float2 e = mine ? get2(a.part_ml + (slot_of(ew) * G + eg) * 2) : make_float2(-INFINITY, 0.f);
+    for (int i = tid; i == tid || i < words; i += kThreads) {   // (all threads meet at the first's barrier)
+        const int word = min(i, words - 1), g = word / (HD / 2);
+        float2 y[kFan];
+#pragma unroll
+        for (int k = 0; k < kFan; k++) y[k] = get2(a.part + slot_of(min(k, count - 1)) * (unsigned)(G * HD) + 2 * word);
+        if (i == tid) {
+            const float top = row16_max(e.x), base = top == -INFINITY ? 0.f : top;
+            const float f = mine ? __builtin_amdgcn_exp2f(e.x - base) : 0.f, sum = row16_sum(f * e.y);
+            if (eg < G) {
+                weight[ew * G + eg] = f;
+                if (ew == 0) {
+                    inv[eg] = sum == 0.f ? 0.f : vscale / sum;
+                    if (!whole) put2(a.part_ml + (slot_of(0) * G + eg) * 2, top, sum);
+                }
+            }
+            __syncthreads();
+        }
+        float2 o = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < kFan; k++) {
+            const float f = weight[k * G + g];
+            if (f != 0.f) {   // (a part behind the last has none, whatever was read in its place)
+                o.x += f * y[k].x;
+                o.y += f * y[k].y;
+            }
+        }
+        if (i >= words) break;
+        if (whole) *reinterpret_cast<float2*>(out + 2 * word) = make_float2(inv[g] * o.x, inv[g] * o.y);
+        else put2(a.part + slot_of(0) * (unsigned)(G * HD) + 2 * word, o.x, o.y);
+    }
+}
+
+// What a wave reads of a unit.
+struct Span {
+    int first, end;        // positions the mask keeps
+    int mine, final_, t1;  // the wave's first and last tile (every kWaves-th); none: mine >= t1
+    const unsigned char *kb, *vb;
+    const int* table;
+};
+
+// One block per KV head and span, as many as fit the chip at once, so that all
+// start together, read at the same rate and end together: units handed out
+// one by one left the last 50 us of a batch of 64 (147 us) to a few of them.
+//
+// While a part streams, the next one's q rows and page indices come in, and
+// its first tile's rows are on their way before this one's waves are joined:
+// with memory saturated each of these waits takes 3 to 5 us.
 template <int HD, int DT>
 __global__ void __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) paged_attn_kernel(const AttendArgs a) {
     typedef Tile<HD, DT> T;
-    constexpr int NP = Parts<DT>::N, NT = T::NT, DPW = 4 / T::ES;   // dims of a V word
-    extern __shared__ float red[];                                  // [kWaves][G][HD], then (m, l) [kWaves][16][2]
-    Unit u;
-    if (!find_unit(a, blockIdx.x, u)) return;
-    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
-    const int G = a.group, nkv = a.c.n_kv_heads, first = u.row.first, end = u.row.end;
-    const float* kscale = a.c.k_scale ? a.c.k_scale + a.layer * nkv + u.head : nullptr;
-    const float vscale = DT == GSDH_KV_E4M3 ? a.c.v_scale[a.layer * nkv + u.head] : 1.0f;
-    float* out = a.out + (int64_t)u.i * a.out_stride + (int64_t)u.head * G * HD;
+    constexpr int TP = T::TP, H = T::H, NP = Parts<DT, 4 * H>::N, NT = T::NT, DPW = 4 / T::ES;   // dims of a V word
+    constexpr int kThreads = 64 * kWaves;
+    constexpr int QN = (kMaxGroup * HD / 4 + kThreads - 1) / kThreads;   // 16-byte words of q a thread brings in
+    extern __shared__ float lds[];
+    __shared__ int last;
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, col = lane & 15, grp = lane >> 4;
+    const int G = a.group, nkv = a.c.n_kv_heads, head = (int)(blockIdx.x % (unsigned)nkv);
+    float *qbuf = lds, *red = lds + G * HD;   // q [G][HD]; outputs [kWaves][G][HD], (m, l) [kWaves][16][2]
 
-    // q's operand: head `col`, zeros beyond the group
-    Parts<DT> q[T::KS];
-    float to_log2;
-    {
-        float x[T::KS][8], most = 0.f;
-        const float* qp = a.q + (int64_t)u.i * a.q_stride + ((int64_t)u.head * G + (col < G ? col : 0)) * HD;
-#pragma unroll
-        for (int s = 0; s < T::KS; s++) {
-            const float4 lo = *reinterpret_cast<const float4*>(qp + T::dim(s, grp));
-            const float4 hi = *reinterpret_cast<const float4*>(qp + T::dim(s, grp) + 4);
-            const float w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                x[s][e] = col < G ? w[e] : 0.f;
-                most = fmaxf(most, fabsf(x[s][e]));
-            }
-        }
-        // 2^(9 - exponent of the largest), kept within the range of normal floats
-        unsigned ex = __float_as_uint(max_over_groups(most)) >> 23;
-        ex = ex < 16u ? 16u : ex > 254u ? 254u : ex;
-        const float up = __uint_as_float((263u - ex) << 23), down = __uint_as_float((ex - 9u) << 23);
-        to_log2 = a.scale * kLog2e * (DT == GSDH_KV_E4M3 ? *kscale : 1.0f) * down;
-#pragma unroll
-        for (int s = 0; s < T::KS; s++) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[s][e] *= up;
-            q[s] = split8<DT>(x[s]);
-        }
-    }
-
-    float4v acc[NT];
-#pragma unroll
-    for (int t = 0; t < NT; t++) acc[t] = float4v{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
-    bool lost = u.row.bad;
-
-    const int t0 = first / kTile + u.split * u.chunk;
-    const int t1 = end > first ? min(t0 + u.chunk, (end - 1) / kTile + 1) : 0;
     const size_t page_b = (size_t)a.c.page_size * nkv * HD * T::ES;
     const unsigned row_b = (a.c.head_major ? 1u : (unsigned)nkv) * HD * T::ES;
-    const size_t head_b = (size_t)u.head * (a.c.head_major ? a.c.page_size : 1) * HD * T::ES;
-    const unsigned char* kb = static_cast<const unsigned char*>(a.c.k) + (size_t)a.layer * a.c.n_pages * page_b + head_b;
-    const unsigned char* vb = static_cast<const unsigned char*>(a.c.v) + (size_t)a.layer * a.c.n_pages * page_b + head_b;
-    const int* table = a.c.tables + (size_t)u.row.seq * a.c.table_width;
+    const size_t layer_b = (size_t)a.layer * a.c.n_pages * page_b;
     const int psl = __builtin_ctz((unsigned)a.c.page_size), psm = a.c.page_size - 1;
-    // positions outside first .. end - 1 (rows of the first and last tile that
-    // the mask drops) read the nearest row inside: what lies beyond, NaN
-    // among it, meets no product
-    auto inside = [&](int p) { return min(max(p, first), end - 1); };
-    auto page_of = [&](int p) {
-        const int pg = table[p >> psl];
-        if ((unsigned)pg < (unsigned)a.c.n_pages) return pg;
-        lost = true;
-        return 0;
+    auto span_of = [&](const Unit& u) {
+        Span s;
+        s.first = u.row.first;
+        s.end = u.row.end;
+        s.t1 = u.t1;
+        s.mine = __builtin_amdgcn_readfirstlane(u.t0 + wid);
+        s.final_ = s.mine < s.t1 ? s.mine + (s.t1 - 1 - s.mine) / kWaves * kWaves : s.mine;
+        const size_t off = layer_b + (size_t)head * (a.c.head_major ? a.c.page_size : 1) * HD * T::ES;
+        s.kb = static_cast<const unsigned char*>(a.c.k) + off;
+        s.vb = static_cast<const unsigned char*>(a.c.v) + off;
+        s.table = a.c.tables + (size_t)(unsigned)max(u.row.seq, 0) * a.c.table_width;
+        return s;
     };
+    // The pages of a tile's runs of eight positions (a page is at least that)
+    // come from a lane each, kAhead of the wave's tiles per load and a load
+    // ahead: a lookup of its own for each tile would come back behind the rows
+    // in flight.
+    constexpr int kRuns = 2 * H, kAhead = 64 / kRuns;
+    auto run_at = [&](int t) { return (t + lane / kRuns * kWaves) * TP + 8 * (lane % kRuns); };   // of tiles t, t + kWaves ..
+    auto pages_from = [&](const Span& s, int t) {
+        return s.table[min(max(run_at(t), s.first), s.end - 1) >> psl];   // (a run without a position: the nearest page)
+    };
+    // byte offsets of the runs' first rows; a page outside the pool is not read
+    auto offsets = [&](int t, int pg, bool& lost) {
+        const bool bad = (unsigned)pg >= (unsigned)a.c.n_pages;
+        lost |= bad;
+        return (size_t)(bad ? 0u : (unsigned)pg) * page_b + (unsigned)(run_at(t) & psm) * row_b;
+    };
+    struct Runs {
+        size_t at[kRuns];
+    };
+    auto runs_of = [&](size_t held, int k) {   // of the k-th tile held
+        Runs p;
+#pragma unroll
+        for (int j = 0; j < kRuns; j++)
+            p.at[j] = (size_t)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)held, kRuns * k + j) |
+                      (size_t)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(held >> 32), kRuns * k + j) << 32;
+        return p;
+    };
+    // Whole runs are loaded, also the rows of the first and last tile that the
+    // mask drops (they lie in pages of the pool; V's are cleared before use).
+    const unsigned k_at = (col & 7) * row_b + 16 * grp, v_at = (4 * grp & 7) * row_b + NT * T::ES * col;
     T tile;
-    auto load_k = [&](int t) {
+    auto load_k = [&](const Span& s, const Runs& runs) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int p = inside(t * kTile + 16 * h + col);
-            tile.load_k(h, kb + (size_t)page_of(p) * page_b + (unsigned)(p & psm) * row_b + 16 * grp);
+        for (int h = 0; h < H; h++) tile.load_k(h, s.kb + ((col < 8 ? runs.at[2 * h] : runs.at[2 * h + 1]) + k_at));
+    };
+    auto load_v = [&](const Span& s, const Runs& runs) {
+#pragma unroll
+        for (int h = 0; h < H; h++) {
+            const unsigned char* p = s.vb + ((grp < 2 ? runs.at[2 * h] : runs.at[2 * h + 1]) + v_at);
+#pragma unroll
+            for (int r = 0; r < 4; r++) tile.load_v(4 * h + r, p + r * row_b);
         }
     };
-    auto load_v = [&](int t) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            // four positions from a multiple of 4 on share a page
-            const int g = t * kTile + 16 * h + 4 * grp;
-            const unsigned char* pb = vb + (size_t)page_of(inside(g)) * page_b + NT * T::ES * col;
-#pragma unroll
-            for (int r = 0; r < 4; r++) tile.load_v(4 * h + r, pb + (unsigned)(inside(g + r) & psm) * row_b);
-        }
-    };
-    if (t0 + wid < t1) {
-        load_k(t0 + wid);
-        load_v(t0 + wid);
-    }
-    for (int t = t0 + wid; t < t1; t += kWaves) {
-        float4v s[2] = {float4v{0.f, 0.f, 0.f, 0.f}, float4v{0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-        for (int i = 0; i < T::KS; i++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const uint4 f = tile.kfrag(h, i);
-#pragma unroll
-                for (int p = NP - 1; p >= 0; p--) s[h] = mma<DT>(f, q[i].w[p], s[h]);
-            }
-        const bool more = t + kWaves < t1;
-        if (more) load_k(t + kWaves);
-        float x[8], top = -INFINITY;
-        const int p0 = t * kTile + 4 * grp;
-        if (p0 - 4 * grp >= first && p0 - 4 * grp + kTile <= end) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = s[e >> 2][e & 3] * to_log2;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int p = p0 + 16 * (e >> 2) + (e & 3);
-                x[e] = p >= first && p < end ? s[e >> 2][e & 3] * to_log2 : -INFINITY;
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 8; e++) top = fmaxf(top, x[e]);
-        top = fmaxf(m, max_over_groups(top));
-        if (__any(top > m)) {
-            const float f = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
-#pragma unroll
-            for (int n = 0; n < NT; n++) acc[n] *= f;
-            l *= f;
-            m = top;
-        }
-        // P as 2^14 times itself: the parts below fp16's normal range stay exact
-        const float base = m == -INFINITY ? 0.f : m - 14.f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            x[e] = __builtin_amdgcn_exp2f(x[e] - base);
-            l += x[e];
-        }
-        const Parts<DT> p = split8<DT>(x);
-#pragma unroll
-        for (int w = 0; w < T::VW; w++) {
-            uint4 f[DPW];
-            tile.vfrags(w, f);
-#pragma unroll
-            for (int d = 0; d < DPW; d++)
-#pragma unroll
-                for (int n = NP - 1; n >= 0; n--) acc[DPW * w + d] = mma<DT>(f[d], p.w[n], acc[DPW * w + d]);
-        }
-        if (more) load_v(t + kWaves);
-    }
-    l = sum_over_groups(l);
-    if (__any(lost)) {
-        l = __builtin_nanf("");
-        if (lane == 0 && u.head == 0) page_status(a.c, GSDH_PAGES_BAD_INDEX);
-    }
 
-    // the four waves' outputs, joined in LDS
-    float* ml = red + kWaves * G * HD;
-    if (col < G) {
-        float* o = red + ((size_t)wid * G + col) * HD + 4 * NT * grp;
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-#pragma unroll
-            for (int t = 0; t < NT; t += 4)
-                *reinterpret_cast<float4*>(o + r * NT + t) = make_float4(acc[t][r], acc[t + 1][r], acc[t + 2][r], acc[t + 3][r]);
-        if (grp == 0) {
-            ml[(wid * kMaxGroup + col) * 2] = m;
-            ml[(wid * kMaxGroup + col) * 2 + 1] = l;
-        }
+    RowSpan parts = parts_of<TP>(a, blockIdx.x / (unsigned)nkv);
+    float kscale = 1.f, vscale = 1.f;
+    if constexpr (DT == GSDH_KV_E4M3) {
+        kscale = a.c.k_scale[a.layer * nkv + head];
+        vscale = a.c.v_scale[a.layer * nkv + head];
     }
-    __syncthreads();
-    const bool whole = u.splits == 1;
-    for (int i = threadIdx.x; i < G * HD / 4; i += 64 * kWaves) {
-        const int g = i / (HD / 4);
-        float top = -INFINITY, sum = 0.f;
+    Unit u{};
+    Span s{};
+    size_t held = 0;
+    bool have = false, lost = false;
+    for (;;) {
+        // the next part: its q and pages
+        Unit un{};
+        Span sn{};
+        float4v qn[QN];
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) top = fmaxf(top, ml[(w * kMaxGroup + g) * 2]);
-        const float base = top == -INFINITY ? 0.f : top;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int j = 0; j < QN; j++) qn[j] = float4v{0.f, 0.f, 0.f, 0.f};
+        size_t heldn = 0;
+        int pagesn = 0;
+        bool lostn = false;
+        const bool more = next_part<TP>(a, parts, un);
+        if (more) {
+            sn = span_of(un);
+            lostn = un.row.bad;
+            if (sn.mine < sn.t1) pagesn = pages_from(sn, sn.mine);
+            const float4v* qp = reinterpret_cast<const float4v*>(a.q + (int64_t)un.i * a.q_stride + (int64_t)head * G * HD);
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-            const float f = __builtin_amdgcn_exp2f(ml[(w * kMaxGroup + g) * 2] - base);
-            const float4 y = *reinterpret_cast<const float4*>(red + ((size_t)w * G * HD + 4 * i));
-            sum += f * ml[(w * kMaxGroup + g) * 2 + 1];
-            o.x += f * y.x; o.y += f * y.y; o.z += f * y.z; o.w += f * y.w;
+            for (int j = 0; j < QN; j++)
+                qn[j] = qp[min(tid + j * kThreads, G * HD / 4 - 1)];
         }
-        if (whole) {
-            const float f = sum == 0.f ? 0.f : vscale / sum;
-            *reinterpret_cast<float4*>(out + 4 * i) = make_float4(f * o.x, f * o.y, f * o.z, f * o.w);
-        } else {
-            const size_t slot = (size_t)u.slot + u.split;
-            *reinterpret_cast<float4*>(a.part + slot * G * HD + 4 * i) = o;
-            if (i % (HD / 4) == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * G + g) * 2) = make_float2(top, sum);
-        }
-    }
-    if (whole) return;
 
-    // the last of the row's units to arrive joins all of them, in their order
-    __shared__ int last;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        unsigned* c = a.counters + (size_t)u.i * nkv + u.head;
-        __threadfence();
-        last = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)u.splits - 1u;
-        __threadfence();
-        if (last) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (!last) return;
-    const float* part = a.part + (size_t)u.slot * G * HD;
-    const float* pml = a.part_ml + (size_t)u.slot * G * 2;
-    for (int i = threadIdx.x; i < G * HD / 4; i += 64 * kWaves) {
-        const int g = i / (HD / 4);
-        float top = -INFINITY, sum = 0.f;
-        for (int w = 0; w < u.splits; w++) top = fmaxf(top, pml[(w * G + g) * 2]);
-        const float base = top == -INFINITY ? 0.f : top;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int w = 0; w < u.splits; w++) {
-            const float2 e = *reinterpret_cast<const float2*>(pml + (w * G + g) * 2);
-            const float4 y = *reinterpret_cast<const float4*>(part + (size_t)w * G * HD + 4 * i);
-            const float f = __builtin_amdgcn_exp2f(e.x - base);
-            sum += f * e.y;
-            o.x += f * y.x; o.y += f * y.y; o.z += f * y.z; o.w += f * y.w;
+        float4v acc[NT];
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int t = 0; t < NT; t++) acc[t] = float4v{0.f, 0.f, 0.f, 0.f};
+        if (have && s.mine < s.t1) {
+            // q's operand: head `col`, zeros beyond the group
+            Parts<DT, 8> q[T::KS];
+            float to_log2;
+            {
+                float x[T::KS][8], most = 0.f;
+                const float* qp = qbuf + (col < G ? col : 0) * HD;
+#pragma unroll
+                for (int i = 0; i < T::KS; i++) {
+                    const float4 lo = *reinterpret_cast<const float4*>(qp + T::dim(i, grp));
+                    const float4 hi = *reinterpret_cast<const float4*>(qp + T::dim(i, grp) + 4);
+                    const float w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        x[i][e] = col < G ? w[e] : 0.f;
+                        most = fmaxf(most, fabsf(x[i][e]));
+                    }
+                }
+                // 2^(9 - exponent of the largest), kept within the range of normal floats
+                unsigned ex = __float_as_uint(max_over_groups(most)) >> 23;
+                ex = ex < 16u ? 16u : ex > 254u ? 254u : ex;
+                const float up = copysignf(__uint_as_float((263u - ex) << 23), a.scale), down = __uint_as_float((ex - 9u) << 23);
+                to_log2 = fabsf(a.scale) * kLog2e * kscale * down;   // (a negative scale: in q's sign)
+#pragma unroll
+                for (int i = 0; i < T::KS; i++) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[i][e] *= up;
+                    q[i] = split<DT, 8>(x[i]);
+                }
+            }
+            // The next tile's K is loaded once this one's scores are formed, its V
+            // once the output is: half a tile or more is always in flight.  The
+            // loads are unconditional (after the wave's last tile that one again,
+            // from the cache), so that a wait never has to drain those behind a
+            // branch.
+            int ahead = pages_from(s, s.mine + kAhead * kWaves), place = 0;   // the next kAhead tiles' pages; the next tile among the held
+            for (int t = s.mine; t < s.t1; t += kWaves) {
+                float4v xs[H];
+#pragma unroll
+                for (int h = 0; h < H; h++) xs[h] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < T::KS; i++)
+#pragma unroll
+                    for (int h = 0; h < H; h++) {
+                        const u32x4v f = __builtin_bit_cast(u32x4v, tile.kfrag(h, i));
+#pragma unroll
+                        for (int p = NP - 1; p >= 0; p--) xs[h] = mma<DT>(f, q[i].w[p], xs[h]);
+                    }
+                const int to = min(t + kWaves, s.final_);
+                place += to != t;
+                if (place == kAhead) {
+                    held = offsets(to, ahead, lost);
+                    ahead = pages_from(s, to + kAhead * kWaves);
+                    place = 0;
+                }
+                const Runs runs = runs_of(held, place);
+                load_k(s, runs);
+                // x stays unscaled until the exponential; rows that the mask drops are -inf
+                float x[4 * H], top = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < 4 * H; e++) x[e] = xs[e / 4][e % 4];
+                const bool edge = t * TP < s.first || (t + 1) * TP > s.end;
+                if (edge) {
+#pragma unroll
+                    for (int e = 0; e < 4 * H; e++) {
+                        const int p = t * TP + 16 * (e / 4) + 4 * grp + e % 4;
+                        if (p < s.first || p >= s.end) x[e] = -INFINITY;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4 * H; e++) top = fmaxf(top, x[e]);
+                top = fmaxf(m, max_over_groups(top) * to_log2);
+                if (__any(top > m)) {
+                    const float f = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) acc[n] *= f;
+                    l *= f;
+                    m = top;
+                }
+                // P as 2^14 times itself: the parts below fp16's normal range stay exact
+                const float base = m == -INFINITY ? 0.f : m - 14.f;
+#pragma unroll
+                for (int e = 0; e < 4 * H; e++) {
+                    x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], to_log2, -base));
+                    l += x[e];
+                }
+                const Parts<DT, 4 * H> p = split<DT, 4 * H>(x);
+                if (edge) {
+                    // what lies outside may be anything, NaN among it: it meets no product
+#pragma unroll
+                    for (int e = 0; e < 4 * H; e++) {
+                        const int q = t * TP + 16 * (e / 4) + 4 * grp + e % 4;
+                        if (q < s.first || q >= s.end)
+#pragma unroll
+                            for (int w = 0; w < T::VW; w++) tile.v[e][w] = 0u;
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < T::VW; w++) {
+                    typename T::Words f[DPW];
+                    tile.vfrags(w, f);
+#pragma unroll
+                    for (int d = 0; d < DPW; d++)
+#pragma unroll
+                        for (int n = NP - 1; n >= 0; n--) acc[DPW * w + d] = mma<DT>(f[d], p.w[n], acc[DPW * w + d]);
+                }
+                load_v(s, runs);
+            }
         }
-        const float f = sum == 0.f ? 0.f : vscale / sum;
-        *reinterpret_cast<float4*>(out + 4 * i) = make_float4(f * o.x, f * o.y, f * o.z, f * o.w);
+        // the next part's first rows
+        if (more && sn.mine < sn.t1) {
+            heldn = offsets(sn.mine, pagesn, lostn);
+            const Runs runs = runs_of(heldn, 0);
+            load_k(sn, runs);
+            load_v(sn, runs);
+        }
+
+        if (have) {
+            l = sum_over_groups(l);
+            if (__any(lost)) {
+                l = __builtin_nanf("");
+                if (lane == 0 && head == 0) page_status(a.c, GSDH_PAGES_BAD_INDEX);
+            }
+            // the waves' outputs, joined in LDS
+            float* ml = red + kWaves * G * HD;
+            if (col < G) {
+                float* o = red + ((size_t)wid * G + col) * HD + 4 * NT * grp;
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int t = 0; t < NT; t += 4)
+                        *reinterpret_cast<float4*>(o + r * NT + t) = make_float4(acc[t][r], acc[t + 1][r], acc[t + 2][r], acc[t + 3][r]);
+                if (grp == 0) *reinterpret_cast<float2*>(ml + (wid * kMaxGroup + col) * 2) = make_float2(m, l);
+            }
+            __syncthreads();
+            const bool whole = u.splits == 1;
+            float* out = a.out + (int64_t)u.i * a.out_stride + (int64_t)head * G * HD;
+            for (int i = tid; i < G * HD / 4; i += kThreads) {
+                const int g = i / (HD / 4);
+                float top = -INFINITY, sum = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWaves; w++) top = fmaxf(top, ml[(w * kMaxGroup + g) * 2]);
+                const float base = top == -INFINITY ? 0.f : top;
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < kWaves; w++) {
+                    const float2 e = *reinterpret_cast<const float2*>(ml + (w * kMaxGroup + g) * 2);
+                    const float f = __builtin_amdgcn_exp2f(e.x - base);
+                    const float4 y = *reinterpret_cast<const float4*>(red + ((size_t)w * G * HD + 4 * i));
+                    sum += f * e.y;
+                    o.x += f * y.x; o.y += f * y.y; o.z += f * y.z; o.w += f * y.w;
+                }
+                if (whole) {
+                    const float f = sum == 0.f ? 0.f : vscale / sum;
+                    *reinterpret_cast<float4*>(out + 4 * i) = make_float4(f * o.x, f * o.y, f * o.z, f * o.w);
+                } else {
+                    const size_t slot = (size_t)((u.span + u.split) * nkv + head) * 2 + (u.split == 0);
+                    float* to = a.part + slot * G * HD + 4 * i;
+                    put2(to, o.x, o.y);
+                    put2(to + 2, o.z, o.w);
+                    if (i % (HD / 4) == 0) put2(a.part_ml + (slot * G + g) * 2, top, sum);
+                }
+            }
+            if (!whole) {
+                // The block that arrives last of kFan neighbouring parts joins them,
+                // the last of these (or the only one) all of the row: which parts
+                // are added to which does not depend on who arrives when.
+                unsigned* counter = a.counters + ((size_t)u.i * nkv + head) * a.counter_step;
+                const int fans = (u.splits + kFan - 1) / kFan, fan = u.split / kFan;
+                int first = fan * kFan, step = 1, count = min(kFan, u.splits - first), index = fans == 1 ? 0 : 1 + fan;
+                for (bool done = fans == 1;; done = true) {
+                    published();
+                    __syncthreads();
+                    if (tid == 0) last = arrive(counter + index, (unsigned)count);
+                    __syncthreads();
+                    if (!last) break;
+                    join_parts<HD>(a, u, head, first, step, count, done, red, out, vscale);
+                    if (done) break;
+                    first = 0;
+                    step = kFan;
+                    count = fans;
+                    index = 0;
+                }
+            }
+        }
+        if (!more) break;
+#pragma unroll
+        for (int j = 0; j < QN; j++)
+            if (tid + j * kThreads < G * HD / 4) reinterpret_cast<float4v*>(qbuf)[tid + j * kThreads] = qn[j];
+        __syncthreads();
+        u = un;
+        s = sn;
+        held = heldn;
+        lost = lostn;
+        have = true;
     }
 }
 
@@ -616,33 +818,43 @@ __global__ void __launch_bounds__(256) paged_store_kernel(const StoreArgs a) {
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
-// partials of split rows: a launch of `target` units' worth of tiles has less
-// than 2 target units in rows of several
+// Waves per SIMD.  With one, a CU has 32 to 64 KB of rows in flight, which is
+// what memory needs; more only wait longer for it (a batch of 64, fp16 rows of
+// 128 dims: 125 us with one, 134 with two).  e4m3 rows cost more instructions
+// a byte, which a second wave hides (48 rows of up to 4096: 50.5 and 54.9 us).
+constexpr int waves_per_simd(int dtype, int hd) { return dtype == GSDH_KV_E4M3 && hd < 256 ? 2 : 1; }
+
+// Blocks that fit the chip, as groups of one per KV head; two partials of each
+// (of a row that it continues and one that it starts).
+constexpr int kCounters = 1 + kMostFans;   // of a row and KV head: the row's, its fans'
 struct AttendSpace {
-    int target;
+    int groups;
     size_t slots;
     uint64_t bytes;
 };
 AttendSpace attend_space(const gsdh_paged_cache& c, int n, int n_heads, int cus) {
     AttendSpace s;
-    s.target = kUnitsPerCu * (cus > 0 ? cus : 1);
-    s.slots = 2 * (size_t)s.target + c.n_kv_heads;
-    s.bytes = counted_workspace((uint64_t)n * c.n_kv_heads, 4 * (uint64_t)s.slots * (n_heads / c.n_kv_heads) * (c.head_dim + 2));
+    const int fit = (cus > 0 ? cus : 1) * waves_per_simd(c.dtype, c.head_dim) * 4 / kWaves;
+    s.groups = std::min(std::max(1, fit / c.n_kv_heads), kFan * kMostFans - 1);
+    s.slots = 2 * (size_t)s.groups * c.n_kv_heads;
+    s.bytes = counted_workspace((uint64_t)n * c.n_kv_heads * kCounters, 4 * (uint64_t)s.slots * (n_heads / c.n_kv_heads) * (c.head_dim + 2));
     return s;
 }
 
 bool attend_shape(const gsdh_paged_cache& c, int n, int n_heads) {
     return n >= 0 && n_heads > 0 && n_heads % c.n_kv_heads == 0 && n_heads / c.n_kv_heads <= kMaxGroup &&
-           (int64_t)n * c.n_kv_heads < (1 << 30);
+           (int64_t)n * c.n_kv_heads < (1 << 30) &&
+           (int64_t)n * ((int64_t)c.table_width * c.page_size / 16 + 2 + kRowCost) < 0x7FFFFFFF;   // costs add up in 32 bits
 }
 
 template <int HD, int DT>
 hipError_t launch_attend(const AttendArgs& a, hipStream_t st) {
     static LdsLimit limit;
-    const size_t lds = 4 * ((size_t)kWaves * a.group * HD + kWaves * kMaxGroup * 2);
+    // q; then the waves' outputs and their (m, l), or (less) the join's weights and 1 / sums
+    const size_t lds = 4 * ((size_t)(1 + kWaves) * a.group * HD + kWaves * kMaxGroup * 2 + (kFan + 1) * kMaxGroup);
     const hipError_t e = raise_lds_limit(limit, reinterpret_cast<const void*>(paged_attn_kernel<HD, DT>), lds);
     if (e != hipSuccess) return e;
-    const unsigned grid = (unsigned)(a.target + (int64_t)a.n * a.c.n_kv_heads);
+    const unsigned grid = (unsigned)(a.groups * a.c.n_kv_heads);
     hipLaunchKernelGGL((paged_attn_kernel<HD, DT>), dim3(grid), dim3(64 * kWaves), lds, st, a);
     return hipGetLastError();
 }
@@ -725,8 +937,10 @@ int gsdh_paged_attention(void* stream, const gsdh_paged_cache* c, int layer, con
     AttendArgs a{};
     a.c = *c;
     a.q = q; a.q_stride = q_stride; a.seqs = seqs; a.out = out; a.out_stride = out_stride;
-    a.layer = layer; a.n = n; a.group = n_heads / c->n_kv_heads; a.window = window; a.target = s.target; a.scale = sm_scale;
+    a.layer = layer; a.n = n; a.group = n_heads / c->n_kv_heads; a.window = window; a.groups = s.groups; a.scale = sm_scale;
     a.counters = static_cast<unsigned*>(workspace);
+    // lines of their own where there is room: arrivals at one line wait for each other
+    a.counter_step = (unsigned)std::min<size_t>(32, counter_bytes(workspace_bytes) / 4 / ((size_t)n * c->n_kv_heads));
     a.part = static_cast<float*>(workspace) + counter_bytes(workspace_bytes) / 4;
     a.part_ml = a.part + s.slots * a.group * c->head_dim;
     hipStream_t st = static_cast<hipStream_t>(stream);

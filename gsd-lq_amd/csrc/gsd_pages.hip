@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(kPlan) pages_compact_kernel(const gsdh_paged_c
 // Whole pages, one after another in each block: page src[i] to page dst[i]
 // in K or V of a layer, 32 to 64 KB (16 slots of 8 heads of 128 dims) with
 // eight 16-byte loads of a thread ahead of its stores.  dst[i] < 0: left out.
-__device__ void move_pages(const gsdh_paged_cache& c, const int* src, const int* dst, int n, size_t page, unsigned block, unsigned blocks) {
+__device__ __forceinline__ void move_pages(const gsdh_paged_cache& c, const int* src, const int* dst, int n, size_t page, unsigned block, unsigned blocks) {
     const unsigned pools = 2u * c.n_layers;
     for (size_t u = block; u < (size_t)n * pools; u += blocks) {
         const unsigned i = (unsigned)(u / pools), pool = (unsigned)(u % pools);

@@ -146,6 +146,7 @@ class _Lib:
                 if rc != 0:
                     raise HipError(f"{name} failed ({rc}): {self.last_error()}")
                 return rc
+            setattr(self, name, call)   # (found without this method from now on)
             return call
         return fn
 
