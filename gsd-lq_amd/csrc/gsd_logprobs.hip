@@ -10,10 +10,14 @@ using namespace gsd;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kGroups = 64;         // of four threads; a row has at most twice as many segments
+constexpr int kGroups = 64;         // of kThreads / 64 threads
+constexpr int kMaxSeg = 128;        // segments of a row
+constexpr int kBlocks = 512;        // that a launch is split into where it has fewer rows: two per CU
+constexpr int kNV = 4;              // 16-byte words of a thread in one chunk
+constexpr int chunk_of(int dtype) { return kThreads * kNV * (dtype == GSDH_LOGITS_F32 ? 4 : 8); }   // logits of a chunk
 constexpr int kMaxTop = 32;
-constexpr int kMaxVocab = (1 << 20) - 8;   // 128 segments of 8192 at most, wherever the row starts
-constexpr int kMaxCand = 4096;      // keys that may reach a threshold (below)
+constexpr int kMaxVocab = (1 << 20) - 8;
+constexpr int kMaxCand = 1024;      // keys that are ranked at once
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
 // A logit and its place as one word that orders them: larger logits first,
@@ -38,7 +42,7 @@ struct LogprobArgs {
     float* part;              // [n][nseg] (m, s, t, -)
     uint64_t* part_keys;      // [n][nseg][top]
     int64_t stride;
-    int vocab, top, nseg;
+    int vocab, top, nseg, chunks;   // chunks of a segment
 };
 
 template <int DT>
@@ -62,6 +66,7 @@ __device__ uint64_t nth_largest(const uint64_t* keys, int count, int want) {
     for (int base = 0; base < count; base += 64) {
         const uint64_t mine = base + lane < count ? keys[base + lane] : 0;
         int above = 0;
+#pragma unroll 8
         for (int i = 0; i < count; i++) above += keys[i] > mine;
         const unsigned long long hit = __ballot(mine != 0 && above == want - 1);
         if (hit) {
@@ -79,23 +84,22 @@ __device__ void select_top(const uint64_t* cand, int count, int top, uint64_t* o
     for (int i = threadIdx.x; i < count; i += kThreads) {
         const uint64_t mine = cand[i];
         int above = 0;
+#pragma unroll 4
         for (int j = 0; j < count; j++) above += cand[j] > mine;
         if (above < top) out[above] = mine;
     }
 }
 
-// The row's results from its sums (m, s, t) and its largest keys (LDS).
-template <int DT>
-__device__ void finish_row(const LogprobArgs& a, int row, float m, float s, float t, const uint64_t* keys) {
+// The row's results from its sums (m, s, t), its token's logit (thread 0) and its largest keys (LDS).
+__device__ __forceinline__ void finish_row(const LogprobArgs& a, int row, int tok, float logit, float m, float s, float t, const uint64_t* keys) {
     const float log_s = __builtin_amdgcn_logf(s) * kLn2;
     // (m is -inf where nothing has probability, and s NaN where a logit was NaN or +inf)
     const bool none = !(s > 0.f) || m == -INFINITY;
     if (threadIdx.x == 0) {
         if (a.logprob) {
-            const int tok = a.tokens[row];
             float v = __builtin_nanf("");
             if (tok == -1) v = 0.f;
-            else if (tok >= 0 && tok < a.vocab && !none) v = (logit_at<DT>(a.logits, row * a.stride + tok) - m) - log_s;
+            else if (tok >= 0 && tok < a.vocab && !none) v = (logit - m) - log_s;
             a.logprob[row] = v;
         }
         if (a.entropy) a.entropy[row] = none ? __builtin_nanf("") : log_s - t / s;
@@ -107,123 +111,209 @@ __device__ void finish_row(const LogprobArgs& a, int row, float m, float s, floa
     }
 }
 
-// One block: a segment of kThreads * E logits of a row, held in registers.
+// One block: a segment of a row, chunk by chunk, the next chunk's loads ahead
+// of this one's arithmetic.  Each thread keeps, of its logits,
 //
 //   m = max x,  s = sum e^(x - m),  t = sum e^(x - m) (x - m)
 //   ln p = x - m - ln s,  entropy = ln s - t / s   (no cancellation: both terms are >= 0)
 //
-// The largest `top`: 64 groups of four threads each take the largest key of
-// theirs; `top` groups reach the top-th largest of these 64, so at most
-// 4 E top logits do (some `top` more of ordinary rows), and these are ranked
-// by counting.  A row of several segments is joined by the block that arrives
-// last.  Logits are read in 16-byte words from the aligned address at or
-// below the row's first, those of a row's edges one by one.
-template <int DT, int E>
+// and the word of four or eight logits that its largest first came in.
+// The largest `top`: 64 groups of four threads each give the largest (value,
+// then lower word) of theirs; `top` groups reach the top-th largest of these,
+// so `top` logits do at least.  The words of the threads that reach it are read
+// again, by all threads, and the logits at or above it (some `top` more of
+// ordinary rows) are ranked by counting.  A row of several segments is joined by the
+// block that arrives last.  Logits are read in 16-byte words from the aligned
+// address at or below the row's first, those of a row's edges one by one.
+//
+// 512 rows of 32768 in fp32 (67 MB) take 14.9 us, 61 rows of 130001 in bf16 (16
+// MB) 14.4: eight instructions a logit, then about 5 us of dependent steps
+// (the groups' keys, the words read again, the ranking, the join).  Segments
+// of 8192 in registers with a selection for each took 27 and 18 us.
+template <int DT>
 __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a) {
-    constexpr int VEC = DT == GSDH_LOGITS_F32 ? 4 : 8, NV = E / VEC, ES = DT == GSDH_LOGITS_F32 ? 4 : 2;
-    __shared__ float red[3 * (kThreads / 64)];
-    __shared__ uint64_t group[2 * kGroups], best[kMaxTop], cand[kMaxCand];
-    __shared__ int n_cand, last;
+    constexpr int VEC = DT == GSDH_LOGITS_F32 ? 4 : 8, ES = DT == GSDH_LOGITS_F32 ? 4 : 2, kChunk = chunk_of(DT), kWavesOf = kThreads / 64;
+    constexpr float kLowest = -3.40282347e38f;
+    __shared__ float red[3 * kWavesOf];
+    __shared__ uint64_t group[kMaxSeg], best[kMaxTop], cand[kMaxCand];
+    __shared__ uint8_t owner[kThreads];
+    __shared__ int n_cand, n_owner, last;
     const int row = blockIdx.x / a.nseg, seg = blockIdx.x % a.nseg, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
     const unsigned char* base = static_cast<const unsigned char*>(a.logits) + row * a.stride * ES;
     const int off = (int)(reinterpret_cast<uintptr_t>(base) % 16) / ES;   // logits between the aligned address and the row
     base -= off * ES;
     const int end = off + a.vocab;   // places off .. end - 1 are the row's
+    const int c0 = seg * a.chunks, c1 = min(c0 + a.chunks, (end + kChunk - 1) / kChunk);
 
-    float x[E];
-#pragma unroll
-    for (int j = 0; j < NV; j++) {
-        const int at = seg * kThreads * E + (j * kThreads + tid) * VEC;
+    // (the token's logit comes with the others, not after them)
+    int tok = -1;
+    float logit = 0.f;
+    if (tid == 0 && a.logprob) {
+        tok = a.tokens[row];
+        if (tok >= 0 && tok < a.vocab) logit = logit_at<DT>(a.logits, row * a.stride + tok);
+    }
+    if (tid == 0) n_cand = n_owner = 0;
+
+    auto place = [&](int c, int j) { return c * kChunk + (j * kThreads + tid) * VEC; };   // of the thread's j-th word in a chunk
+    // the word at place `at`, -inf for what is not the row's
+    auto word = [&](int at) {
+        u32x4v w;
         if (at >= off && at + VEC <= end) {
-            const uint4 w = *reinterpret_cast<const uint4*>(base + (size_t)at * ES);
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+            w = *reinterpret_cast<const u32x4v*>(base + (size_t)at * ES);
+        } else {
+            uint32_t e[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; e++) {
-                if constexpr (DT == GSDH_LOGITS_F32) x[j * VEC + e] = __uint_as_float(u[e]);
-                else if constexpr (DT == GSDH_LOGITS_F16) x[j * VEC + e] = h2f((uint16_t)(u[e >> 1] >> (16 * (e & 1))));
-                else x[j * VEC + e] = __uint_as_float(e & 1 ? u[e >> 1] & 0xFFFF0000u : u[e >> 1] << 16);
+            for (int i = 0; i < VEC; i++) {
+                e[i] = ES == 4 ? 0xFF800000u : DT == GSDH_LOGITS_F16 ? 0xFC00u : 0xFF80u;
+                if (at + i >= off && at + i < end) {
+                    if constexpr (ES == 4) e[i] = reinterpret_cast<const uint32_t*>(base)[at + i];
+                    else e[i] = reinterpret_cast<const uint16_t*>(base)[at + i];
+                }
             }
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = ES == 4 ? e[i] : e[2 * i % VEC] | e[(2 * i + 1) % VEC] << 16;
+        }
+        return w;
+    };
+    auto load = [&](int c, u32x4v (&w)[kNV]) {
+        if (c * kChunk >= off && (c + 1) * kChunk <= end) {
+#pragma unroll
+            for (int j = 0; j < kNV; j++) w[j] = *reinterpret_cast<const u32x4v*>(base + (size_t)place(c, j) * ES);
         } else {
 #pragma unroll
-            for (int e = 0; e < VEC; e++)
-                x[j * VEC + e] = at + e >= off && at + e < end ? logit_at<DT>(base, at + e) : -INFINITY;
+            for (int j = 0; j < kNV; j++) w[j] = word(place(c, j));
+        }
+    };
+    auto values = [](const u32x4v w, float (&x)[VEC]) {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+            if constexpr (DT == GSDH_LOGITS_F32) x[i] = __uint_as_float(w[i]);
+            else if constexpr (DT == GSDH_LOGITS_F16) x[i] = h2f((uint16_t)(w[i >> 1] >> (16 * (i & 1))));
+            else x[i] = __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+        }
+    };
+
+    float mx = -INFINITY, m = kLowest, s = 0.f, t = 0.f;
+    int first = c0 < c1 ? place(c0, 0) : end;   // the word that mx first came in
+    u32x4v next[kNV];
+    if (c0 < c1) load(c0, next);
+    for (int c = c0; c < c1; c++) {
+        u32x4v w[kNV];
+#pragma unroll
+        for (int j = 0; j < kNV; j++) w[j] = next[j];
+        if (c + 1 < c1) load(c + 1, next);
+#pragma unroll
+        for (int j = 0; j < kNV; j++) {
+            float x[VEC];
+            values(w[j], x);
+            float top = x[0];
+#pragma unroll
+            for (int i = 1; i < VEC; i++) top = fmaxf(top, x[i]);
+            first = top > mx ? place(c, j) : first;
+            mx = fmaxf(mx, top);
+        }
+        const float to = fmaxf(mx, kLowest);
+        if (__any(to > m)) {
+            const float d = fmaxf(m - to, -1e30f), f = __builtin_amdgcn_exp2f(d * kLog2e);
+            t = f * fmaf(d, s, t);
+            s *= f;
+            m = to;
+        }
+#pragma unroll
+        for (int j = 0; j < kNV; j++) {
+            float x[VEC];
+            values(w[j], x);
+#pragma unroll
+            for (int i = 0; i < VEC; i++) {
+                const float d = x[i] - m, p = __builtin_amdgcn_exp2f(d * kLog2e);
+                s += p;
+                t = fmaf(p, fmaxf(d, -1e30f), t);
+            }
         }
     }
 
-    float mx = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < E; e++) mx = fmaxf(mx, x[e]);
-    const float wmx = wave_max(mx);
-    if (lane == 0) red[wid] = wmx;
-    if (tid == 0) n_cand = 0;
-
-    // the largest key of the thread, then of its group
+    // the segment's largest, the groups' keys
+    float sm = wave_max(m);
+    if (lane == 0) red[wid] = sm;
+    uint64_t mine = 0;
     if (a.top) {
-        uint64_t mine = 0;
-        auto place = [&](int e) { return seg * kThreads * E + ((e / VEC) * kThreads + tid) * VEC + e % VEC; };
-        if (mx > -INFINITY) {
-            int at = 0;
-#pragma unroll
-            for (int e = E - 1; e >= 0; e--) at = x[e] == mx ? place(e) : at;
-            mine = key_of(mx, at - off);
-        } else {
-            // nothing above -inf: the first place that is the row's
-            for (int e = E - 1; e >= 0; e--)
-                if (place(e) >= off && place(e) < end) mine = key_of(-INFINITY, place(e) - off);
-        }
-        mine = shfl_max(mine, 1);
-        mine = shfl_max(mine, 2);
-        if ((lane & 3) == 0) group[tid >> 2] = mine;
+        // (a thread whose first word lies behind the row has none)
+        if (first + VEC > off && first < end) mine = key_of(mx, first);
+        uint64_t of = shfl_max(mine, 1);
+        of = shfl_max(of, 2);
+        if ((lane & 3) == 0) group[tid >> 2] = of;
     }
     __syncthreads();
-    float m = red[0];
+    sm = red[0];
 #pragma unroll
-    for (int w = 1; w < kThreads / 64; w++) m = fmaxf(m, red[w]);
-    __syncthreads();
-
+    for (int w = 1; w < kWavesOf; w++) sm = fmaxf(sm, red[w]);
+    const float d = fmaxf(m - sm, -1e30f), f = __builtin_amdgcn_exp2f(d * kLog2e);
+    t = wave_sum(f * fmaf(d, s, t));
+    s = wave_sum(s * f);
+    if (lane == 0) {
+        red[kWavesOf + wid] = s;
+        red[2 * kWavesOf + wid] = t;
+    }
     if (a.top) {
         const uint64_t least = nth_largest(group, kGroups, a.top);
         const float lv = value_of(least);
+        const int li = least ? index_of(least) : end;   // (0: fewer groups than that have logits: all of them)
+        if (mine >= least && mine) owner[atomicAdd(&n_owner, 1)] = (uint8_t)tid;
+        __syncthreads();
+        // their words, dealt to all threads
+        const int owners = n_owner, words = owners * (c1 - c0) * kNV;
+        for (int k = tid; k < words; k += kThreads) {
+            const int j = k / owners, at = (c0 + j / kNV) * kChunk + (j % kNV * kThreads + owner[k % owners]) * VEC;
+            float x[VEC];
+            values(word(at), x);
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-            if (least == 0 || fmaxf(x[e], -INFINITY) >= lv) {
-                const int at = seg * kThreads * E + ((e / VEC) * kThreads + tid) * VEC + e % VEC;
-                const uint64_t k = key_of(x[e], at - off);
-                if (k >= least && at >= off && at < end) {
+            for (int i = 0; i < VEC; i++) {
+                const float y = fmaxf(x[i], -INFINITY);
+                if ((!least || y > lv || (y == lv && at <= li)) && at + i >= off && at + i < end) {
                     const int p = atomicAdd(&n_cand, 1);
-                    if (p < kMaxCand) cand[p] = k;
+                    if (p < kMaxCand) cand[p] = key_of(x[i], at + i - off);
                 }
             }
         }
     }
-
-    float s = 0.f, t = 0.f;
-    const float c = m == -INFINITY ? 0.f : m;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        const float d = x[e] - c, p = __builtin_amdgcn_exp2f(d * kLog2e);
-        s += p;
-        t = fmaf(p, fmaxf(d, -1e30f), t);
-    }
-    s = wave_sum(s);
-    t = wave_sum(t);
-    if (lane == 0) {
-        red[(kThreads / 64) + wid] = s;
-        red[2 * (kThreads / 64) + wid] = t;
-    }
     __syncthreads();
+    m = sm;
     s = t = 0.f;
 #pragma unroll
-    for (int w = 0; w < kThreads / 64; w++) {
-        s += red[(kThreads / 64) + w];
-        t += red[2 * (kThreads / 64) + w];
+    for (int w = 0; w < kWavesOf; w++) {
+        s += red[kWavesOf + w];
+        t += red[2 * kWavesOf + w];
     }
     if (a.top) {
-        select_top(cand, min(n_cand, kMaxCand), a.top, best);
+        if (n_cand <= kMaxCand) {
+            select_top(cand, n_cand, a.top, best);
+        } else {
+            // (more than are ranked at once, as where a few threads' logits outweigh
+            // all others': the largest one by one, each below the one before)
+            uint64_t before = ~0ull;
+            for (int r = 0; r < a.top; r++) {
+                uint64_t most = 0;
+                for (int c = c0; c < c1; c++)
+                    for (int j = 0; j < kNV; j++)
+                        for (int i = 0; i < VEC; i++) {
+                            const int at = place(c, j) + i;
+                            const uint64_t k = at >= off && at < end ? key_of(logit_at<DT>(base, at), at - off) : 0;
+                            if (k < before && k > most) most = k;
+                        }
+#pragma unroll
+                for (int d = 32; d >= 1; d >>= 1) most = shfl_max(most, d);
+                if (lane == 0) group[wid] = most;
+                __syncthreads();
+                before = group[0];
+                for (int w = 1; w < kWavesOf; w++) before = group[w] > before ? group[w] : before;
+                if (tid == 0) best[r] = before;
+                __syncthreads();
+            }
+        }
         __syncthreads();
     }
     if (a.nseg == 1) {
-        finish_row<DT>(a, row, m, s, t, best);
+        finish_row(a, row, tok, logit, m, s, t, best);
         return;
     }
 
@@ -242,13 +332,26 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a) 
     }
     __syncthreads();
     if (!last) return;
+    // its segments' sums, and each one's k-th largest key, k = ceil(top / nseg):
+    // ceil(top / k) of these have k keys each that are as large
     const float* part = a.part + (int64_t)row * a.nseg * 4;
-    __shared__ float4 sums[2 * kGroups];
-    for (int i = tid; i < a.nseg; i += kThreads) {
-        const float2 p = get2(part + 4 * i), q = get2(part + 4 * i + 2);
-        sums[i] = make_float4(p.x, p.y, q.x, 0.f);
+    const uint64_t* keys = a.part_keys + (int64_t)row * a.nseg * a.top;
+    const auto get = [&](int i) { return __hip_atomic_load(&keys[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    const int k = (a.top + a.nseg - 1) / a.nseg;
+    __shared__ float4 sums[kMaxSeg];
+    if (tid < a.nseg) {
+        const float2 p = get2(part + 4 * tid), q = get2(part + 4 * tid + 2);
+        if (a.top) group[tid] = get(tid * a.top + k - 1);
+        sums[tid] = make_float4(p.x, p.y, q.x, 0.f);
     }
     __syncthreads();
+    if (a.top) {
+        const uint64_t least = nth_largest(group, a.nseg, (a.top + k - 1) / k);
+        for (int i = tid; i < a.nseg * a.top; i += kThreads) {
+            const uint64_t y = get(i);
+            if (y != 0 && y >= least) cand[atomicAdd(&n_cand, 1)] = y;   // (at most top^2)
+        }
+    }
     float top = -INFINITY;
     for (int i = 0; i < a.nseg; i++) top = fmaxf(top, sums[i].x);
     s = t = 0.f;
@@ -260,48 +363,34 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a) 
         t += f * (p.z + d * p.y);
     }
     if (a.top) {
-        // each segment's k-th largest, k = ceil(top / nseg): k times the ceil(top / k)
-        // largest of these are `top` at least
-        const uint64_t* keys = a.part_keys + (int64_t)row * a.nseg * a.top;
-        const int k = (a.top + a.nseg - 1) / a.nseg;
-        const auto get = [&](int i) { return __hip_atomic_load(&keys[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-        for (int i = tid; i < a.nseg; i += kThreads) group[i] = get(i * a.top + k - 1);
         __syncthreads();
-        const uint64_t least = nth_largest(group, a.nseg, (a.top + k - 1) / k);
-        for (int i = tid; i < a.nseg * a.top; i += kThreads) {
-            const uint64_t y = get(i);
-            if (y != 0 && y >= least) {
-                const int p = atomicAdd(&n_cand, 1);
-                if (p < kMaxCand) cand[p] = y;
-            }
-        }
-        __syncthreads();
-        select_top(cand, min(n_cand, kMaxCand), a.top, best);
+        select_top(cand, n_cand, a.top, best);
         __syncthreads();
     }
-    finish_row<DT>(a, row, top, s, t, best);
+    finish_row(a, row, tok, logit, top, s, t, best);
 }
 
-// Logits of a thread: 32 where the rows fill the chip, else 8, as long as the
-// join of a row's segments stays within its candidates.
+// Segments of a row, and their chunks; `extra`: places ahead of a row that
+// does not start at a 16-byte address.
 struct Plan {
-    int e, nseg;
+    int nseg, chunks;
 };
-Plan plan_of(int n, int vocab, int top) {
-    Plan p{32, (vocab + 7 + kThreads * 32 - 1) / (kThreads * 32)};
-    const int small = (vocab + 7 + kThreads * 8 - 1) / (kThreads * 8);
-    if ((int64_t)n * p.nseg < 512 && small * top <= kMaxCand && small <= 2 * kGroups) p = {8, small};
-    return p;
+Plan plan_of(int n, int vocab, int dtype, int extra) {
+    const int chunks = (vocab + extra + chunk_of(dtype) - 1) / chunk_of(dtype);
+    const int want = std::min(std::min((kBlocks + n - 1) / n, chunks), kMaxSeg), each = (chunks + want - 1) / want;
+    return {(chunks + each - 1) / each, each};
 }
-// bytes of the partial results of n rows, and of a workspace that holds them
-size_t parts_of(int n, const Plan& p, int top) { return p.nseg == 1 ? 0 : (size_t)n * p.nseg * (16 + 8 * (size_t)top); }
-uint64_t space_for(int n, const Plan& p, int top) { return p.nseg == 1 ? 0 : counted_workspace((uint64_t)n, parts_of(n, p, top)); }
+// Partial results: of n rows of (kBlocks + n - 1) / n segments, which is the
+// most that fewer rows have too, in rows of at least two chunks.
+uint64_t logprob_space(int n, int vocab, int top) {
+    if (vocab + 3 <= chunk_of(GSDH_LOGITS_F32)) return 0;
+    const uint64_t rows = (uint64_t)std::min(n, kBlocks - 1);
+    return counted_workspace(rows, (rows + kBlocks) * (16 + 8 * (uint64_t)top));
+}
 
 template <int DT>
-hipError_t launch_logprobs(const LogprobArgs& a, int n, int e, hipStream_t st) {
-    const dim3 grid((unsigned)(n * a.nseg)), block(kThreads);
-    if (e == 32) hipLaunchKernelGGL((logprob_kernel<DT, 32>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((logprob_kernel<DT, 8>), grid, block, 0, st, a);
+hipError_t launch_logprobs(const LogprobArgs& a, int n, hipStream_t st) {
+    hipLaunchKernelGGL(logprob_kernel<DT>, dim3((unsigned)(n * a.nseg)), dim3(kThreads), 0, st, a);
     return hipGetLastError();
 }
 
@@ -314,15 +403,7 @@ bool logprob_shape(int n, int vocab, int top) {
 extern "C" {
 
 uint64_t gsdh_token_logprobs_workspace_bytes(int n, int vocab, int top_n) {
-    if (!logprob_shape(n, vocab, top_n)) return 0;
-    // (fewer rows may take more segments each)
-    uint64_t most = space_for(n, plan_of(n, vocab, top_n), top_n);
-    const Plan few = plan_of(1, vocab, top_n), many = plan_of(1 << 20, vocab, top_n);
-    if (few.nseg != many.nseg) {
-        const int rows = std::min(n, 511 / many.nseg);
-        if (rows > 0) most = std::max(most, space_for(rows, few, top_n));
-    }
-    return most;
+    return logprob_shape(n, vocab, top_n) ? logprob_space(n, vocab, top_n) : 0;
 }
 
 int gsdh_token_logprobs(void* stream, const void* logits, int dtype, int64_t row_stride, int n, int vocab, const int* tokens,
@@ -338,11 +419,13 @@ int gsdh_token_logprobs(void* stream, const void* logits, int dtype, int64_t row
     if (n == 0) return 0;
     if (!logits || reinterpret_cast<uintptr_t>(logits) % (dtype == GSDH_LOGITS_F32 ? 4 : 2))
         return fail(-1, "%s: logits null or not aligned to their type", who);
-    const Plan p = plan_of(n, vocab, top_n);
-    const int rc = check_workspace(workspace, workspace_bytes, space_for(n, p, top_n), who);
+    const int es = dtype == GSDH_LOGITS_F32 ? 4 : 2;
+    const bool aligned = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && (n == 1 || row_stride * es % 16 == 0);
+    const Plan p = plan_of(n, vocab, dtype, aligned ? 0 : 16 / es - 1);
+    const int rc = check_workspace(workspace, workspace_bytes, logprob_space(n, vocab, top_n), who);
     if (rc) return rc;
     LogprobArgs a{};
-    a.logits = logits; a.stride = row_stride; a.tokens = tokens; a.vocab = vocab; a.top = top_n; a.nseg = p.nseg;
+    a.logits = logits; a.stride = row_stride; a.tokens = tokens; a.vocab = vocab; a.top = top_n; a.nseg = p.nseg; a.chunks = p.chunks;
     a.logprob = logprob; a.entropy = entropy; a.top_ids = top_ids; a.top_lp = top_logprobs;
     unsigned char* w = static_cast<unsigned char*>(workspace);
     a.counters = reinterpret_cast<unsigned*>(w);
@@ -350,9 +433,9 @@ int gsdh_token_logprobs(void* stream, const void* logits, int dtype, int64_t row
     a.part_keys = reinterpret_cast<uint64_t*>(a.part + 4 * (size_t)n * p.nseg);
     if ((int64_t)n * p.nseg > 0x7FFFFFFF) return fail(-1, "%s: %d rows of %d logits in one call", who, n, vocab);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    GSD_PAGED_CHK(dtype == GSDH_LOGITS_F32 ? launch_logprobs<GSDH_LOGITS_F32>(a, n, p.e, st)
-                  : dtype == GSDH_LOGITS_F16 ? launch_logprobs<GSDH_LOGITS_F16>(a, n, p.e, st)
-                                             : launch_logprobs<GSDH_LOGITS_BF16>(a, n, p.e, st), who);
+    GSD_PAGED_CHK(dtype == GSDH_LOGITS_F32 ? launch_logprobs<GSDH_LOGITS_F32>(a, n, st)
+                  : dtype == GSDH_LOGITS_F16 ? launch_logprobs<GSDH_LOGITS_F16>(a, n, st)
+                                             : launch_logprobs<GSDH_LOGITS_BF16>(a, n, st), who);
     return 0;
 }
 

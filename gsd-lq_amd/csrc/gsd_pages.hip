@@ -7,6 +7,7 @@
 // runs over the whole chip and is bound by memory.
 #include <algorithm>
 
+#include "gsd_device.h"
 #include "gsd_paged.h"
 
 using namespace gsd;
@@ -18,7 +19,7 @@ constexpr int kRun = 8;             // words of refs a thread looks at per step
 constexpr int kPlanWaves = kPlan / 64;
 
 // workspace words: header, then lists
-constexpr int kMoves = 0, kUsed = 1, kHead = 4;
+constexpr int kMoves = 0, kUsed = 1, kFirst = 2, kHead = 4;   // moves, pages in use, the first source in its list
 
 struct Space {
     size_t src, dst, map, plan, words;   // offsets in ints
@@ -80,15 +81,22 @@ __device__ int scan_pages(const int* refs, int n, int stop, int* lds, Pred pred,
             if (lane == 0) lds[j * kPlanWaves + wid] = __popcll(mask[j]);
         }
         __syncthreads();
-        int before[kRun], sum = 0;
+        // the counts' sums up to each, two to a lane, by every wave for itself
+        static_assert(kRun * kPlanWaves == 128, "two counts a lane");
+        const int2 two = reinterpret_cast<const int2*>(lds)[lane];
+        int incl = two.x + two.y;
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) {
+            const int b = __shfl_up(incl, s, 64);
+            if (lane >= s) incl += b;
+        }
+        const int sum = __builtin_amdgcn_readlane(incl, 63);
+        int before[kRun];
 #pragma unroll
         for (int j = 0; j < kRun; j++) {
-            before[j] = sum;
-            for (int w = 0; w < kPlanWaves; w++) {
-                const int k = lds[j * kPlanWaves + w];
-                if (w < wid) before[j] += k;
-                sum += k;
-            }
+            const int at = j * kPlanWaves + wid;   // (the pair of counts that this one is in)
+            const int upto = __shfl(incl, at >> 1, 64), lo = __shfl(two.x, at >> 1, 64), hi = __shfl(two.y, at >> 1, 64);
+            before[j] = at & 1 ? upto - hi : upto - hi - lo;
         }
         __syncthreads();   // (the counts are read)
         const unsigned long long below = (1ull << lane) - 1ull;
@@ -128,12 +136,12 @@ __device__ void first_of(const gsdh_paged_cache& c, const int* list, int n, int*
     __syncthreads();
 }
 
-// dynamic LDS of a planning block: first[n_seqs], off[n], then the scans' words
+// dynamic LDS of a planning block: the scans' words, first[n_seqs], off[n]
 size_t plan_lds(const gsdh_paged_cache& c, int n) { return 4 * ((size_t)c.n_seqs + n + kRun * kPlanWaves + kPlanWaves); }
 
 __global__ void __launch_bounds__(kPlan) pages_take_kernel(const gsdh_paged_cache c, const int* seqs, const int* counts, int n) {
-    extern __shared__ int lds[];
-    int *first = lds, *off = first + c.n_seqs, *words = off + n, *scan = words + kRun * kPlanWaves;
+    extern __shared__ __align__(16) int lds[];
+    int *words = lds, *scan = words + kRun * kPlanWaves, *first = scan + kPlanWaves, *off = first + c.n_seqs;
     first_of(c, seqs, n, first);
     // how many pages each wants: -1 in the list's place of one that is left out
     auto want = [&](int i, uint32_t* bad) {
@@ -186,8 +194,8 @@ __global__ void __launch_bounds__(kPlan) pages_take_kernel(const gsdh_paged_cach
 // A fork's plan per list entry, in the workspace: source, destination (-1:
 // left out), positions, the page taken for the last partly filled one (-1: none)
 __global__ void __launch_bounds__(kPlan) pages_fork_kernel(const gsdh_paged_cache c, const int* src, const int* dst, int n, int4* plan) {
-    extern __shared__ int lds[];
-    int *first = lds, *off = first + c.n_seqs, *words = off + n, *scan = words + kRun * kPlanWaves;
+    extern __shared__ __align__(16) int lds[];
+    int *words = lds, *scan = words + kRun * kPlanWaves, *first = scan + kPlanWaves, *off = first + c.n_seqs;
     first_of(c, dst, n, first);
     uint32_t bad = 0;
     int total = 0;
@@ -293,55 +301,64 @@ __global__ void __launch_bounds__(256) pages_free_kernel(const gsdh_paged_cache 
     }
 }
 
-// Which page moves where: src[i] -> dst[i]; map[p] is the new place of a page
+// Which page moves where: src[first + i] -> dst[i]; map[p] is the new place of a page
 // p that moves, -1 for the free ones among those behind the last used place.
 __global__ void __launch_bounds__(kPlan) pages_compact_kernel(const gsdh_paged_cache c, int* n_used, int* ws, Space s) {
-    __shared__ int words[kRun * kPlanWaves];
+    __shared__ __align__(8) int words[kRun * kPlanWaves];
     int *src = ws + s.src, *dst = ws + s.dst, *map = ws + s.map;
     const auto used = [](int r, int) { return r > 0; };
     const int n = scan_pages(c.refs, c.n_pages, c.n_pages + 1, words, used, [](int, bool, int) {});
-    const int stay = scan_pages(c.refs, n, n + 1, words, used, [&](int page, bool in_use, int rank) {
-        if (!in_use) dst[page - rank] = page;
-    });
-    scan_pages(c.refs + n, c.n_pages - n, c.n_pages + 1, words, used, [&](int i, bool in_use, int rank) {
-        if (in_use) src[rank] = n + i;
-        else map[n + i] = -1;
+    // holes below n in their order; behind them the used pages by their rank among all
+    __shared__ int stay;   // used pages below n
+    if (threadIdx.x == 0) stay = 0;
+    scan_pages(c.refs, c.n_pages, c.n_pages + 1, words, used, [&](int page, bool in_use, int rank) {
+        if (page < n) {
+            if (!in_use) dst[page - rank] = page;
+            if (page == n - 1) stay = rank + in_use;
+        } else if (in_use) {
+            src[rank] = page;
+        } else {
+            map[page] = -1;
+        }
     });
     const int moves = n - stay;
     __threadfence_block();
     __syncthreads();
     for (int i = threadIdx.x; i < moves; i += kPlan) {
-        const int a = src[i], b = dst[i];
+        const int a = src[stay + i], b = dst[i];
         map[a] = b;
         c.refs[b] = c.refs[a];
         c.refs[a] = 0;
     }
     if (threadIdx.x == 0) {
         ws[kMoves] = moves;
+        ws[kFirst] = stay;
         ws[kUsed] = n;
         if (n_used) *n_used = n;
     }
 }
 
 // Whole pages, one after another in each block: page src[i] to page dst[i]
-// in K or V of a layer, 32 to 64 KB (16 slots of 8 heads of 128 dims) with
-// eight 16-byte loads of a thread ahead of its stores.  dst[i] < 0: left out.
-__device__ __forceinline__ void move_pages(const gsdh_paged_cache& c, const int* src, const int* dst, int n, size_t page, unsigned block, unsigned blocks) {
-    const unsigned pools = 2u * c.n_layers;
+// in K or V of a layer (32 KB for 16 slots of 8 heads of 128 dims), eight
+// 16-byte loads of a thread ahead of its stores.  The stores pass the caches
+// by: a server's moves exceed them, and what they would push out is still to
+// be read (294 MB moved: 74 us with ordinary stores, 59 so).  dst[i] < 0: left out.
+__device__ __forceinline__ void move_pages(u32x4v* k_pool, u32x4v* v_pool, size_t n_pages, unsigned pools, const int* src, const int* dst,
+                                           int n, size_t page, unsigned block, unsigned blocks) {
     for (size_t u = block; u < (size_t)n * pools; u += blocks) {
         const unsigned i = (unsigned)(u / pools), pool = (unsigned)(u % pools);
         const int a = src[i], b = dst[i];
         if (b < 0) continue;
-        uint4* base = static_cast<uint4*>(pool & 1 ? c.v : c.k) + (size_t)(pool >> 1) * c.n_pages * page;
-        const uint4* s = base + (size_t)a * page;
-        uint4* d = base + (size_t)b * page;
+        u32x4v* base = (pool & 1 ? v_pool : k_pool) + (pool >> 1) * n_pages * page;
+        const u32x4v* s = base + (size_t)a * page;
+        u32x4v* d = base + (size_t)b * page;
         size_t k = threadIdx.x;
         for (; k + 7 * 256 < page; k += 8 * 256) {
-            uint4 w[8];
+            u32x4v w[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) w[j] = s[k + 256 * j];
 #pragma unroll
-            for (int j = 0; j < 8; j++) d[k + 256 * j] = w[j];
+            for (int j = 0; j < 8; j++) __builtin_nontemporal_store(w[j], d + k + 256 * j);
         }
         for (; k < page; k += 256) d[k] = s[k];
     }
@@ -349,10 +366,11 @@ __device__ __forceinline__ void move_pages(const gsdh_paged_cache& c, const int*
 
 // The moves of a compaction, and the tables' entries after them.
 __global__ void __launch_bounds__(256) pages_compact_rows_kernel(const gsdh_paged_cache c, const int* ws, Space s, size_t page, unsigned table_blocks) {
-    const int moves = ws[kMoves], used = ws[kUsed];
+    const int moves = ws[kMoves], used = ws[kUsed], first = ws[kFirst];
     if (moves == 0) return;
     if (blockIdx.x >= table_blocks) {
-        move_pages(c, ws + s.src, ws + s.dst, moves, page, blockIdx.x - table_blocks, gridDim.x - table_blocks);
+        move_pages(static_cast<u32x4v*>(c.k), static_cast<u32x4v*>(c.v), (size_t)c.n_pages, 2u * c.n_layers, ws + s.src + first, ws + s.dst, moves, page,
+                   blockIdx.x - table_blocks, gridDim.x - table_blocks);
         return;
     }
     for (int q = blockIdx.x; q < c.n_seqs; q += table_blocks) {
@@ -400,10 +418,11 @@ __global__ void __launch_bounds__(kPlan) pages_copy_kernel(const gsdh_paged_cach
 }
 
 __global__ void __launch_bounds__(256) pages_copy_rows_kernel(const gsdh_paged_cache c, const int* ws, Space s, int n, size_t page) {
-    move_pages(c, ws + s.src, ws + s.dst, n, page, blockIdx.x, gridDim.x);
+    move_pages(static_cast<u32x4v*>(c.k), static_cast<u32x4v*>(c.v), (size_t)c.n_pages, 2u * c.n_layers, ws + s.src, ws + s.dst, n, page, blockIdx.x,
+               gridDim.x);
 }
 
-unsigned move_blocks() { return 8u * (unsigned)std::max(1, device_cu_count()); }
+unsigned move_blocks() { return 4u * (unsigned)std::max(1, device_cu_count()); }
 
 int check_list(const gsdh_paged_cache* c, const int* a, const int* b, int n, int most, const char* who) {
     if (n < 0 || n > most) return fail(-1, "%s: a list of %d (at most %d)", who, n, most);
