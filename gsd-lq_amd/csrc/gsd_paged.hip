@@ -10,7 +10,6 @@ using namespace gsd;
 namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -18,8 +17,8 @@ constexpr int kWaves = 4;          // waves of a block, each on every fourth til
 constexpr int kRowCost = 128;      // what a row's start and end weigh beside its positions
 constexpr int kLeastSpan = 16;     // the least a block takes, in tiles
 static_assert(kLeastSpan >= 2 * kWaves, "every span inside a row has tiles of it");
-constexpr int kFan = 16;           // parts that one block joins at a time
-constexpr int kMostFans = 16;      // of a row and KV head
+constexpr int kFan = 16;           // parts whose words a thread loads at once when it joins them
+constexpr int kMostFans = 16;      // sets of parts of a row and KV head that are joined on their own
 // positions of a tile, the step of a wave: 8 KB of K and V (4 KB of rows of 64 bytes, 16 KB of rows of 512)
 constexpr int tile_positions(int row_bytes) { return row_bytes <= 128 ? 32 : 16; }
 constexpr int kMaxGroup = 16;      // query heads per KV head: the columns of one matrix product
@@ -57,7 +56,8 @@ struct AttendArgs {
     float* part;
     float* part_ml;
     int64_t q_stride, out_stride;
-    int layer, n, group, window, groups;   // groups: of blocks, one per KV head
+    int layer, n, group, window;
+    int groups, few;      // of blocks, one per KV head: in the launch, and used for long rows
     unsigned counter_step;
     float scale;
 };
@@ -162,10 +162,20 @@ __device__ __forceinline__ RowSpan parts_of(const AttendArgs& a, unsigned group)
     }
     if (lane >= a.n) o.r = Row{-1, 0, 0, false};
     const unsigned total = (unsigned)__builtin_amdgcn_readlane((int)wave_scan(mine), 63);
-    o.size = max((total + (unsigned)a.groups - 1) / (unsigned)a.groups, (unsigned)kLeastSpan);
-    o.lo = group * o.size;   // (groups * size is below 2^32: the launch's limit on positions)
+    // Long rows keep memory busy with a wave per SIMD, and more only wait longer
+    // for it; many short rows are a chain of waits each, which a second one fills
+    // (fp16 rows of 128 dims: 64 rows of up to 8191 positions 127 us with one, 134
+    // with two; 128 rows of 100 23 and 19 us, 512 of 200 133 and 115).
+    // e4m3 rows cost more instructions a byte, which a second wave hides, too, where
+    // its span is no shorter than the chain of waits around it (48 rows of up to 4096:
+    // 50 and 55 us; 16 rows of 1000: 14 us with one, 19 with two).
+    const bool all = (a.n >= a.groups && total < (unsigned)a.n * ((1024 + kRowCost) / TP)) ||
+                     (a.c.dtype == GSDH_KV_E4M3 && total >= 24u * (unsigned)a.groups);
+    const unsigned groups = (unsigned)(all ? a.groups : a.few);
+    o.size = max((total + groups - 1) / groups, (unsigned)kLeastSpan);
+    // (groups * size is below 2^32: the launch's limit on positions)
+    o.lo = group < groups ? min(group * o.size, total) : total;
     o.hi = min(o.lo + o.size, total);
-    if (o.lo >= total) o.hi = o.lo;
     hold_rows<TP>(a, o, a.n > 64);   // (up to 64 rows are at hand)
     return o;
 }
@@ -332,48 +342,67 @@ struct Tile {
     }
 };
 
-// Joins `count` (up to kFan) parts of a row, first, first + step ..: into the
-// row's output, or into the place of the first.  All loads of a word are in
-// flight before the weights are formed (one after another the loads of 64
-// parts took 12 us).
+// Parts that one block joins at a time: two rounds of loads where the outputs
+// are a word per thread, one where they are several (a second level of joins
+// costs 2.5 us, a round 0.7).
+__device__ __forceinline__ int fan_of(int outputs) { return outputs <= 512 ? 2 * kFan : kFan; }
+
+// Joins `count` (up to 2 kFan) parts of a row, first, first + step ..: into
+// the row's output, or into the place of the first.  The loads of kFan words
+// are in flight before the weights are formed (one after another the loads of
+// 64 parts took 12 us).
 template <int HD>
 __device__ __forceinline__ void join_parts(const AttendArgs& a, const Unit& u, int head, int first, int step, int count, bool whole,
                                            float* red, float* out, float vscale) {
     const int tid = threadIdx.x, G = a.group;
     constexpr int kThreads = 64 * kWaves;
+    static_assert(kThreads >= kFan * kMaxGroup && kFan == 16, "a thread per two parts and head, a row of lanes per head");
     auto slot_of = [&](int k) {
-        const int w = first + k * step;
+        const int w = first + min(k, count - 1) * step;
         return (unsigned)(((u.span + w) * a.c.n_kv_heads + head) * 2 + (w == 0));
     };
-    static_assert(kThreads >= kFan * kMaxGroup && kFan == 16, "a thread per part and head, a row of lanes per head");
-    float *weight = red, *inv = red + kFan * kMaxGroup;   // [kFan][G], [G]
+    float *weight = red, *inv = red + 2 * kFan * kMaxGroup;   // [2 kFan][G], 0 behind the last part; [G]
     const int words = G * HD / 2, eg = tid / kFan, ew = tid % kFan;
-    const bool mine = eg < G && ew < count;
-    const float2 e = mine ? get2(a.part_ml + (slot_of(ew) * G + eg) * 2) : make_float2(-INFINITY, 0.f);
+    float2 e[2];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const int k = ew + j * kFan;
+        e[j] = eg < G && k < count ? get2(a.part_ml + (slot_of(k) * G + eg) * 2) : make_float2(-INFINITY, 0.f);
+    }
     for (int i = tid; i == tid || i < words; i += kThreads) {   // (all threads meet at the first's barrier)
         const int word = min(i, words - 1), g = word / (HD / 2);
-        float2 y[kFan];
-#pragma unroll
-        for (int k = 0; k < kFan; k++) y[k] = get2(a.part + slot_of(min(k, count - 1)) * (unsigned)(G * HD) + 2 * word);
-        if (i == tid) {
-            const float top = row16_max(e.x), base = top == -INFINITY ? 0.f : top;
-            const float f = mine ? __builtin_amdgcn_exp2f(e.x - base) : 0.f, sum = row16_sum(f * e.y);
-            if (eg < G) {
-                weight[ew * G + eg] = f;
-                if (ew == 0) {
-                    inv[eg] = sum == 0.f ? 0.f : vscale / sum;
-                    if (!whole) put2(a.part_ml + (slot_of(0) * G + eg) * 2, top, sum);
-                }
-            }
-            __syncthreads();
-        }
         float2 o = make_float2(0.f, 0.f);
+#pragma unroll 1
+        for (int k0 = 0; k0 < count; k0 += kFan) {
+            float2 y[kFan];
 #pragma unroll
-        for (int k = 0; k < kFan; k++) {
-            const float f = weight[k * G + g];
-            if (f != 0.f) {   // (a part behind the last has none, whatever was read in its place)
-                o.x += f * y[k].x;
-                o.y += f * y[k].y;
+            for (int k = 0; k < kFan; k++) y[k] = get2(a.part + slot_of(k0 + k) * (unsigned)(G * HD) + 2 * word);
+            if (i == tid && k0 == 0) {
+                const float top = row16_max(fmaxf(e[0].x, e[1].x)), base = top == -INFINITY ? 0.f : top;
+                float f[2], part = 0.f;
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    f[j] = ew + j * kFan < count ? __builtin_amdgcn_exp2f(e[j].x - base) : 0.f;
+                    part += f[j] * e[j].y;
+                }
+                const float sum = row16_sum(part);
+                if (eg < G) {
+                    weight[ew * G + eg] = f[0];
+                    weight[(ew + kFan) * G + eg] = f[1];
+                    if (ew == 0) {
+                        inv[eg] = sum == 0.f ? 0.f : vscale / sum;
+                        if (!whole) put2(a.part_ml + (slot_of(0) * G + eg) * 2, top, sum);
+                    }
+                }
+                __syncthreads();
+            }
+#pragma unroll
+            for (int k = 0; k < kFan; k++) {
+                const float f = weight[(k0 + k) * G + g];
+                if (f != 0.f) {   // (a part behind the last has none, whatever was read in its place)
+                    o.x += f * y[k].x;
+                    o.y += f * y[k].y;
+                }
             }
         }
         if (i >= words) break;
@@ -525,8 +554,12 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) paged_attn_ker
                 // 2^(9 - exponent of the largest), kept within the range of normal floats
                 unsigned ex = __float_as_uint(max_over_groups(most)) >> 23;
                 ex = ex < 16u ? 16u : ex > 254u ? 254u : ex;
-                const float up = copysignf(__uint_as_float((263u - ex) << 23), a.scale), down = __uint_as_float((ex - 9u) << 23);
-                to_log2 = fabsf(a.scale) * kLog2e * kscale * down;   // (a negative scale: in q's sign)
+                // (a negative scale is in q's sign; one of 0 stays above it, so that a
+                // masked -inf times it stays -inf)
+                const float scale = a.scale * kLog2e * kscale;
+                const float up = copysignf(__uint_as_float((263u - ex) << 23), scale), down = __uint_as_float((ex - 9u) << 23);
+                to_log2 = fabsf(scale) * down;
+                if (to_log2 < 1.17549435e-38f) to_log2 = 1.17549435e-38f;
 #pragma unroll
                 for (int i = 0; i < T::KS; i++) {
 #pragma unroll
@@ -668,12 +701,12 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) paged_attn_ker
                 }
             }
             if (!whole) {
-                // The block that arrives last of kFan neighbouring parts joins them,
+                // The block that arrives last of `many` neighbouring parts joins them,
                 // the last of these (or the only one) all of the row: which parts
                 // are added to which does not depend on who arrives when.
                 unsigned* counter = a.counters + ((size_t)u.i * nkv + head) * a.counter_step;
-                const int fans = (u.splits + kFan - 1) / kFan, fan = u.split / kFan;
-                int first = fan * kFan, step = 1, count = min(kFan, u.splits - first), index = fans == 1 ? 0 : 1 + fan;
+                const int many = fan_of(G * HD), fans = (u.splits + many - 1) / many, fan = u.split / many;
+                int first = fan * many, step = 1, count = min(many, u.splits - first), index = fans == 1 ? 0 : 1 + fan;
                 for (bool done = fans == 1;; done = true) {
                     published();
                     __syncthreads();
@@ -683,7 +716,7 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) paged_attn_ker
                     join_parts<HD>(a, u, head, first, step, count, done, red, out, vscale);
                     if (done) break;
                     first = 0;
-                    step = kFan;
+                    step = many;
                     count = fans;
                     index = 0;
                 }
@@ -818,40 +851,44 @@ __global__ void __launch_bounds__(256) paged_store_kernel(const StoreArgs a) {
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
-// Waves per SIMD.  With one, a CU has 32 to 64 KB of rows in flight, which is
-// what memory needs; more only wait longer for it (a batch of 64, fp16 rows of
-// 128 dims: 125 us with one, 134 with two).  e4m3 rows cost more instructions
-// a byte, which a second wave hides (48 rows of up to 4096: 50.5 and 54.9 us).
-constexpr int waves_per_simd(int dtype, int hd) { return dtype == GSDH_KV_E4M3 && hd < 256 ? 2 : 1; }
+// waves per SIMD that a launch has (it uses one of them for long rows)
+constexpr int waves_per_simd(int hd) { return hd < 256 ? 2 : 1; }
 
 // Blocks that fit the chip, as groups of one per KV head; two partials of each
 // (of a row that it continues and one that it starts).
 constexpr int kCounters = 1 + kMostFans;   // of a row and KV head: the row's, its fans'
 struct AttendSpace {
-    int groups;
+    int groups, few;
     size_t slots;
     uint64_t bytes;
 };
 AttendSpace attend_space(const gsdh_paged_cache& c, int n, int n_heads, int cus) {
     AttendSpace s;
-    const int fit = (cus > 0 ? cus : 1) * waves_per_simd(c.dtype, c.head_dim) * 4 / kWaves;
-    s.groups = std::min(std::max(1, fit / c.n_kv_heads), kFan * kMostFans - 1);
+    auto fit = [&](int waves) {
+        return std::min(std::max(1, (cus > 0 ? cus : 1) * waves * 4 / kWaves / c.n_kv_heads), kFan * kMostFans - 1);
+    };
+    s.groups = fit(waves_per_simd(c.head_dim));
+    s.few = fit(1);
     s.slots = 2 * (size_t)s.groups * c.n_kv_heads;
     s.bytes = counted_workspace((uint64_t)n * c.n_kv_heads * kCounters, 4 * (uint64_t)s.slots * (n_heads / c.n_kv_heads) * (c.head_dim + 2));
     return s;
 }
 
+// the rows' costs add up in 32 bits
+bool positions_fit(const gsdh_paged_cache& c, int n) {
+    return n < 0 || (int64_t)n * ((int64_t)c.table_width * c.page_size / 16 + 2 + kRowCost) < 0x7FFFFFFF;
+}
+
 bool attend_shape(const gsdh_paged_cache& c, int n, int n_heads) {
     return n >= 0 && n_heads > 0 && n_heads % c.n_kv_heads == 0 && n_heads / c.n_kv_heads <= kMaxGroup &&
-           (int64_t)n * c.n_kv_heads < (1 << 30) &&
-           (int64_t)n * ((int64_t)c.table_width * c.page_size / 16 + 2 + kRowCost) < 0x7FFFFFFF;   // costs add up in 32 bits
+           (int64_t)n * c.n_kv_heads < (1 << 30);
 }
 
 template <int HD, int DT>
 hipError_t launch_attend(const AttendArgs& a, hipStream_t st) {
     static LdsLimit limit;
     // q; then the waves' outputs and their (m, l), or (less) the join's weights and 1 / sums
-    const size_t lds = 4 * ((size_t)(1 + kWaves) * a.group * HD + kWaves * kMaxGroup * 2 + (kFan + 1) * kMaxGroup);
+    const size_t lds = 4 * ((size_t)(1 + kWaves) * a.group * HD + kWaves * kMaxGroup * 2 + (2 * kFan + 1) * kMaxGroup);
     const hipError_t e = raise_lds_limit(limit, reinterpret_cast<const void*>(paged_attn_kernel<HD, DT>), lds);
     if (e != hipSuccess) return e;
     const unsigned grid = (unsigned)(a.groups * a.c.n_kv_heads);
@@ -910,7 +947,9 @@ int check_workspace(const void* ws, uint64_t have, uint64_t need, const char* wh
 extern "C" {
 
 uint64_t gsdh_paged_attention_workspace_bytes(const gsdh_paged_cache* c, int n, int n_heads) {
-    if (check_paged_cache(c, "paged_attention_workspace_bytes", false) || !attend_shape(*c, n, n_heads)) return 0;
+    if (check_paged_cache(c, "paged_attention_workspace_bytes", false) || !positions_fit(*c, n) ||
+        !attend_shape(*c, n, n_heads))
+        return 0;
     return attend_space(*c, n, n_heads, device_cu_count()).bytes;
 }
 
@@ -921,6 +960,8 @@ int gsdh_paged_attention(void* stream, const gsdh_paged_cache* c, int layer, con
     int rc = check_paged_cache(c, who, false);
     if (rc) return rc;
     if (layer < 0 || layer >= c->n_layers) return fail(-1, "%s: layer %d outside 0..%d", who, layer, c->n_layers - 1);
+    if (!positions_fit(*c, n))
+        return fail(-1, "%s: %d rows of up to %lld positions in one call", who, n, (long long)c->table_width * c->page_size);
     if (!attend_shape(*c, n, n_heads))
         return fail(-1, "%s: %d rows of %d heads over %d KV heads (1..16 query heads per KV head)", who, n, n_heads,
                     c->n_kv_heads);
@@ -937,7 +978,7 @@ int gsdh_paged_attention(void* stream, const gsdh_paged_cache* c, int layer, con
     AttendArgs a{};
     a.c = *c;
     a.q = q; a.q_stride = q_stride; a.seqs = seqs; a.out = out; a.out_stride = out_stride;
-    a.layer = layer; a.n = n; a.group = n_heads / c->n_kv_heads; a.window = window; a.groups = s.groups; a.scale = sm_scale;
+    a.layer = layer; a.n = n; a.group = n_heads / c->n_kv_heads; a.window = window; a.groups = s.groups; a.few = s.few; a.scale = sm_scale;
     a.counters = static_cast<unsigned*>(workspace);
     // lines of their own where there is room: arrivals at one line wait for each other
     a.counter_step = (unsigned)std::min<size_t>(32, counter_bytes(workspace_bytes) / 4 / ((size_t)n * c->n_kv_heads));

@@ -250,7 +250,8 @@ typedef struct gsdh_paged_cache {
  * softmax(sm_scale q.K) V in fp32.  A sequence of length 0 gives a row of
  * zeros; a negative seqs[i] is padding, its row stays as it was; a row whose
  * sequence, length or pages lie outside the cache becomes NaN (and *status
- * says so).  n_heads / n_kv_heads 1 .. 16; strides in floats, multiples of 4,
+ * says so); a row that holds NaN or an infinity gives NaN or an infinity.
+ * n * table_width * page_size < 2^34.  n_heads / n_kv_heads 1 .. 16; strides in floats, multiples of 4,
  * at least n_heads * head_dim for out (q's rows may be one and the same).
  * workspace: gsdh_paged_attention_workspace_bytes(c, n, n_heads) bytes on this
  * device (0 for an invalid shape), zero before its first call and 16-byte

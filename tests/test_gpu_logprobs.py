@@ -154,6 +154,26 @@ def test_rows_without_a_distribution(lib, kind, vocab):
     check(values, tokens, call(lib, bits.reshape(-1), kind, 7, vocab, vocab, tokens, 4), 4)
 
 
+@pytest.mark.parametrize("kind,lowest", [("f32", -3.4028234663852886e38), ("bf16", -3.3895313892515355e38), ("f16", -65504.0)])
+@pytest.mark.parametrize("vocab", [100, 9001, 40000])
+def test_lowest_values_as_masks(lib, kind, lowest, vocab):
+    """Masks of the type's lowest value: all of a row, all but some, mixed with -inf; few allowed tokens."""
+    banner(f"logprobs {kind} {vocab}: masks of {lowest:.3g}")
+    rng = np.random.default_rng(vocab)
+    x = rng.standard_normal((6, vocab))
+    x[0] = lowest
+    x[1, 3:] = lowest
+    x[2, ::2] = lowest
+    x[3, 7:] = -np.inf
+    x[4] = np.where(rng.random(vocab) < 0.5, lowest, -np.inf)
+    x[5, : vocab - 2] = lowest
+    bits = bits_of(x, kind)
+    values = bits.astype(np.float64) if kind == "f32" else decode(bits, kind)
+    tokens = [0, 1, 1, 2, -1, vocab - 1]
+    tokens[4] = int(np.flatnonzero(np.isfinite(values[4]))[0])
+    check(values, tokens, call(lib, bits.reshape(-1), kind, 6, vocab, vocab, tokens, 20), 20)
+
+
 def test_optional_outputs(lib):
     banner("logprobs: without tokens, entropy or alternatives")
     x = np.random.default_rng(1).standard_normal((3, 9000)).astype(np.float32)

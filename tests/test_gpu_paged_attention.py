@@ -148,6 +148,20 @@ def test_sizes_of_q(lib, scale_q):
     check(got, *c.attend(0, q, [0], np.float32(1.0 / scale_q if scale_q < 1 else 0.05 / scale_q)), [300])
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1e-42])
+def test_scales(lib, scale):
+    """No scale, a negative one, one below the normal range; negative and zero scales of an 8-bit cache."""
+    rng = np.random.default_rng(15)
+    for scales in (None, np.array([[[-0.5, 0.0]], [[-2.0, 0.25]]], np.float32)):
+        c = Cache("e4m3", 1, 60, 8, 2, 64, False, 4, scales=np.ones((2, 1, 2), np.float32)).fill([0, 1, 50, 333], rng, grid)
+        if scales is not None:
+            c.scales = scales
+            c.upload()
+        q = grid(rng, (4, 8, 64))
+        got = c.run_attend(0, q, range(4), scale)
+        check(got, *c.attend(0, q, range(4), np.float32(scale)), [0, 1, 50, 333])
+
+
 def test_infinities_and_nan(lib):
     """A NaN or an infinity among a sequence's own rows shows in its row alone
     (as an infinity or a NaN: the parts of P may differ in sign)."""

@@ -60,6 +60,14 @@ def test_caches(lib, other, text):
     assert lib.gsdh_paged_attention_workspace_bytes(at, 1, 4) == 0
 
 
+def test_positions_of_one_call(lib):
+    c = cache(table_width=1 << 22, page_size=256, n_seqs=100)
+    with pytest.raises(hip.HipError, match="100 rows of up to 1073741824 positions"):
+        attend(lib, c, n=100)
+    assert lib.gsdh_paged_attention_workspace_bytes(ctypes.byref(c), 100, 4) == 0
+    assert lib.gsdh_paged_attention_workspace_bytes(ctypes.byref(c), 10, 4) > 0
+
+
 def test_null_cache(lib):
     with pytest.raises(hip.HipError, match="null cache"):
         lib.gsdh_pages_free(None, None, BUF, 1)
