@@ -125,12 +125,12 @@ __device__ __forceinline__ int owner_of(const int* off, int n, int k) {
     return lo;
 }
 
-// first[s] = the first place in the list that names sequence s
-__device__ void first_of(const gsdh_paged_cache& c, const int* list, int n, int* first) {
+// first[s] = the first place in the list that names sequence s; `own`: list[threadIdx.x]
+__device__ __forceinline__ void first_of(const gsdh_paged_cache& c, const int* list, int own, int n, int* first) {
     for (int s = threadIdx.x; s < c.n_seqs; s += kPlan) first[s] = 0x7FFFFFFF;
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += kPlan) {
-        const int s = list[i];
+        const int s = i < kPlan ? own : list[i];
         if (s >= 0 && s < c.n_seqs) atomicMin(&first[s], i);
     }
     __syncthreads();
@@ -142,13 +142,17 @@ size_t plan_lds(const gsdh_paged_cache& c, int n) { return 4 * ((size_t)c.n_seqs
 __global__ void __launch_bounds__(kPlan) pages_take_kernel(const gsdh_paged_cache c, const int* seqs, const int* counts, int n) {
     extern __shared__ __align__(16) int lds[];
     int *words = lds, *scan = words + kRun * kPlanWaves, *first = scan + kPlanWaves, *off = first + c.n_seqs;
-    first_of(c, seqs, n, first);
+    // (the thread's own entry, all there is of lists up to kPlan, is read ahead:
+    // the launch is a chain of dependent loads)
+    const int tid = threadIdx.x, s0 = tid < n ? seqs[tid] : -1, k0 = tid < n ? counts[tid] : 0;
+    const int len0 = s0 >= 0 && s0 < c.n_seqs ? c.lens[s0] : 0;
+    first_of(c, seqs, s0, n, first);
     // how many pages each wants: -1 in the list's place of one that is left out
     auto want = [&](int i, uint32_t* bad) {
-        const int s = seqs[i], k = counts[i];
+        const int s = i < kPlan ? s0 : seqs[i], k = i < kPlan ? k0 : counts[i];
         if (s < 0 || s >= c.n_seqs || k < 0) { *bad |= GSDH_PAGES_BAD_INDEX; return -1; }
         if (first[s] != i) { *bad |= GSDH_PAGES_TWICE; return -1; }
-        const int len = c.lens[s];
+        const int len = i < kPlan ? len0 : c.lens[s];
         if (!len_ok(c, len) || k > c.table_width * c.page_size - len) { *bad |= GSDH_PAGES_BAD_INDEX; return -1; }
         return pages_for(c, len + k) - pages_for(c, len);   // (beyond the pool: cannot be met)
     };
@@ -175,17 +179,17 @@ __global__ void __launch_bounds__(kPlan) pages_take_kernel(const gsdh_paged_cach
         uint32_t none = 0;
         const int k = want(i, &none);
         if (k < 0) continue;
-        int* len = c.lens + seqs[i];
+        const int s = i < kPlan ? s0 : seqs[i], len = i < kPlan ? len0 : c.lens[s];
         if (k > 0 && off[i] + k > found) {
             bad |= GSDH_PAGES_EXHAUSTED;
             // the pages there were for the first one that does not fit
-            int* t = c.tables + (size_t)seqs[i] * c.table_width + pages_for(c, *len);
+            int* t = c.tables + (size_t)s * c.table_width + pages_for(c, len);
             for (int j = 0; j < min(found - off[i], k); j++) {
                 c.refs[t[j]] = 0;
                 t[j] = -1;
             }
         } else {
-            *len += counts[i];
+            c.lens[s] = len + (i < kPlan ? k0 : counts[i]);
         }
     }
     if (bad) page_status(c, bad);
@@ -196,19 +200,29 @@ __global__ void __launch_bounds__(kPlan) pages_take_kernel(const gsdh_paged_cach
 __global__ void __launch_bounds__(kPlan) pages_fork_kernel(const gsdh_paged_cache c, const int* src, const int* dst, int n, int4* plan) {
     extern __shared__ __align__(16) int lds[];
     int *words = lds, *scan = words + kRun * kPlanWaves, *first = scan + kPlanWaves, *off = first + c.n_seqs;
-    first_of(c, dst, n, first);
+    const int tid = threadIdx.x, a0 = tid < n ? src[tid] : -1, b0 = tid < n ? dst[tid] : -1;   // (as in pages_take_kernel)
+    const int alen0 = a0 >= 0 && a0 < c.n_seqs ? c.lens[a0] : 0, blen0 = b0 >= 0 && b0 < c.n_seqs ? c.lens[b0] : 0;
+    const int last0 = len_ok(c, alen0) && alen0 % c.page_size ? c.tables[(size_t)a0 * c.table_width + alen0 / c.page_size] : 0;
+    first_of(c, dst, b0, n, first);
     uint32_t bad = 0;
     int total = 0;
     for (int base = 0; base < n; base += kPlan) {
         const int i = base + (int)threadIdx.x;
         int k = 0;
         if (i < n) {
-            const int a = src[i], b = dst[i];
+            const bool own = i < kPlan;
+            const int a = own ? a0 : src[i], b = own ? b0 : dst[i];
             int4 e = make_int4(a, -1, 0, -1);
-            if (a < 0 || a >= c.n_seqs || b < 0 || b >= c.n_seqs || !len_ok(c, c.lens[a])) bad |= GSDH_PAGES_BAD_INDEX;
-            else if (first[b] != i || c.lens[b] != 0) bad |= GSDH_PAGES_TWICE;
-            else e = make_int4(a, b, c.lens[a], -1);
-            const int part = e.z % c.page_size, page = part ? c.tables[(size_t)a * c.table_width + e.z / c.page_size] : 0;
+            if (a < 0 || a >= c.n_seqs || b < 0 || b >= c.n_seqs) {
+                bad |= GSDH_PAGES_BAD_INDEX;
+            } else {
+                const int len = own ? alen0 : c.lens[a];
+                if (!len_ok(c, len)) bad |= GSDH_PAGES_BAD_INDEX;
+                else if (first[b] != i || (own ? blen0 : c.lens[b]) != 0) bad |= GSDH_PAGES_TWICE;
+                else e = make_int4(a, b, len, -1);
+            }
+            const int part = e.z % c.page_size;
+            const int page = !part ? 0 : own ? last0 : c.tables[(size_t)a * c.table_width + e.z / c.page_size];
             if ((unsigned)page >= (unsigned)c.n_pages) {
                 bad |= GSDH_PAGES_BAD_INDEX;
                 e = make_int4(a, -1, 0, -1);
@@ -263,20 +277,27 @@ __global__ void __launch_bounds__(256) pages_fork_rows_kernel(const gsdh_paged_c
     }
     if (!part) return;
     const int pool = blockIdx.y - 1;
-    // 16-byte words: of a slot's heads, or of one head's slots
-    const unsigned row = (unsigned)c.n_kv_heads * c.head_dim * es / 16, slot_row = (unsigned)c.head_dim * es / 16;
-    const size_t page = (size_t)row * c.page_size;
-    uint4* base = static_cast<uint4*>(pool & 1 ? c.v : c.k) + (size_t)(pool >> 1) * c.n_pages * page;
-    const uint4* s = base + (size_t)from[full] * page;
-    uint4* d = base + (size_t)e.w * page;
-    if (!c.head_major) {
-        for (unsigned i = threadIdx.x; i < row * part; i += 256) d[i] = s[i];
-    } else {
-        const unsigned run = slot_row * part;
-        for (unsigned i = threadIdx.x; i < run * c.n_kv_heads; i += 256) {
-            const unsigned at = i / run * slot_row * c.page_size + i % run;
-            d[at] = s[at];
+    void *const k_pool = c.k, *const v_pool = c.v;
+    // 16-byte words: the filled slots of all heads lie together, or each head's do
+    const unsigned slot = (unsigned)c.head_dim * es / 16, runs = c.head_major ? c.n_kv_heads : 1;
+    const unsigned run = slot * part * (c.head_major ? 1 : c.n_kv_heads), gap = c.head_major ? slot * c.page_size - run : 0;
+    const size_t page = (size_t)slot * c.n_kv_heads * c.page_size;
+    u32x4v* base = static_cast<u32x4v*>(pool & 1 ? v_pool : k_pool) + (size_t)(pool >> 1) * c.n_pages * page;
+    const u32x4v* s = base + (size_t)from[full] * page;
+    u32x4v* d = base + (size_t)e.w * page;
+    const unsigned all = run * runs;
+    for (unsigned k = threadIdx.x; k < all; k += 8 * 256) {
+        u32x4v w[8];
+        unsigned at[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const unsigned i = min(k + 256 * j, all - 1);
+            at[j] = gap ? i + i / run * gap : i;
+            w[j] = s[at[j]];
         }
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (k + 256 * j < all) d[at[j]] = w[j];
     }
 }
 

@@ -40,6 +40,7 @@ class Paged(Cache):
         for s, k in zip(seqs, counts):
             if not 0 <= s < self.seqs or k < 0:
                 bits |= 1
+                seen.add(s)   # (the first place that names a sequence counts, whatever it asks)
                 continue
             if s in seen:
                 bits |= 8
