@@ -18,6 +18,7 @@ constexpr int chunk_of(int dtype) { return kThreads * kNV * (dtype == GSDH_LOGIT
 constexpr int kMaxTop = 32;
 constexpr int kMaxVocab = (1 << 20) - 8;
 constexpr int kMaxCand = 1024;      // keys that are ranked at once
+constexpr int kHeld = 2;            // keys of other segments that a thread holds
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
 // A logit and its place as one word that orders them: larger logits first,
@@ -56,18 +57,54 @@ __device__ __forceinline__ uint64_t shfl_max(uint64_t k, int mask) {
     const uint64_t o = __shfl_xor((unsigned long long)k, mask, 64);
     return o > k ? o : k;
 }
+// over lanes l, l ^ 1, l ^ 2, l ^ 3, in VALU
+__device__ __forceinline__ uint64_t quad_max(uint64_t k) {
+#define GSD_QUAD_STEP(ctrl)                                                                                              \
+    {                                                                                                                    \
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)k, ctrl, 0xF, 0xF, true);                  \
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(k >> 32), ctrl, 0xF, 0xF, true);          \
+        const uint64_t o = (uint64_t)hi << 32 | lo;                                                                      \
+        k = o > k ? o : k;                                                                                               \
+    }
+    GSD_QUAD_STEP(0xB1);   // quad_perm 1 0 3 2
+    GSD_QUAD_STEP(0x4E);   // quad_perm 2 3 0 1
+#undef GSD_QUAD_STEP
+    return k;
+}
+
+// How many of the first `count` (<= 64) keys are above each: every wave counts
+// a quarter of them for key `lane`, all waves have the sums.  All threads take
+// part; keys and `partial` were last used before a barrier.  (One wave's loop
+// over 64 keys took 1 us.)
+typedef int Partial[kThreads / 64][64];
+__device__ __forceinline__ int count_above(const uint64_t* keys, int count, uint64_t mine, Partial& partial) {
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, per = (count + kThreads / 64 - 1) / (kThreads / 64);
+    int above = 0;
+#pragma unroll 8
+    for (int i = wid * per; i < min(wid * per + per, count); i++) above += keys[i] > mine;
+    partial[wid][lane] = above;
+    __syncthreads();
+    above = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; w++) above += partial[w][lane];
+    return above;
+}
 
 // The `want`-th largest of the first `count` (<= 128) keys of lds (0: fewer
-// nonzero ones than that), by counting for each how many are larger.  Each
-// wave computes it for itself; nonzero keys differ.
-__device__ uint64_t nth_largest(const uint64_t* keys, int count, int want) {
+// nonzero ones than that), by counting for each how many are larger.  Every
+// wave has it; nonzero keys differ.
+__device__ uint64_t nth_largest(const uint64_t* keys, int count, int want, Partial& partial) {
     const int lane = threadIdx.x & 63;
     uint64_t found = 0;
     for (int base = 0; base < count; base += 64) {
         const uint64_t mine = base + lane < count ? keys[base + lane] : 0;
         int above = 0;
+        if (count <= 64) {
+            above = count_above(keys, count, mine, partial);
+        } else {
 #pragma unroll 8
-        for (int i = 0; i < count; i++) above += keys[i] > mine;
+            for (int i = 0; i < count; i++) above += keys[i] > mine;
+        }
         const unsigned long long hit = __ballot(mine != 0 && above == want - 1);
         if (hit) {
             const int src = __builtin_ctzll(hit);
@@ -79,8 +116,15 @@ __device__ uint64_t nth_largest(const uint64_t* keys, int count, int want) {
 }
 
 // out[r] = the r-th largest of cand[0 .. count), r < top; 0 behind the last
-__device__ void select_top(const uint64_t* cand, int count, int top, uint64_t* out) {
+__device__ void select_top(const uint64_t* cand, int count, int top, uint64_t* out, Partial& partial) {
     for (int i = count + (int)threadIdx.x; i < top; i += kThreads) out[i] = 0;
+    if (count <= 64) {
+        const int lane = threadIdx.x & 63;
+        const uint64_t mine = lane < count ? cand[lane] : 0;
+        const int above = count_above(cand, count, mine, partial);
+        if ((int)threadIdx.x < count && above < top) out[above] = mine;
+        return;
+    }
     for (int i = threadIdx.x; i < count; i += kThreads) {
         const uint64_t mine = cand[i];
         int above = 0;
@@ -137,6 +181,7 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a) 
     __shared__ float red[3 * kWavesOf];
     __shared__ uint64_t group[kMaxSeg], best[kMaxTop], cand[kMaxCand];
     __shared__ uint8_t owner[kThreads];
+    __shared__ Partial partial;
     __shared__ int n_cand, n_owner, last;
     const int row = blockIdx.x / a.nseg, seg = blockIdx.x % a.nseg, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
     const unsigned char* base = static_cast<const unsigned char*>(a.logits) + row * a.stride * ES;
@@ -239,8 +284,7 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a) 
     if (a.top) {
         // (a thread whose first word lies behind the row has none)
         if (first + VEC > off && first < end) mine = key_of(mx, first);
-        uint64_t of = shfl_max(mine, 1);
-        of = shfl_max(of, 2);
+        const uint64_t of = quad_max(mine);
         if ((lane & 3) == 0) group[tid >> 2] = of;
     }
     __syncthreads();
@@ -255,7 +299,7 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a) 
         red[2 * kWavesOf + wid] = t;
     }
     if (a.top) {
-        const uint64_t least = nth_largest(group, kGroups, a.top);
+        const uint64_t least = nth_largest(group, kGroups, a.top, partial);
         const float lv = value_of(least);
         const int li = least ? index_of(least) : end;   // (0: fewer groups than that have logits: all of them)
         if (mine >= least && mine) owner[atomicAdd(&n_owner, 1)] = (uint8_t)tid;
@@ -286,7 +330,7 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a) 
     }
     if (a.top) {
         if (n_cand <= kMaxCand) {
-            select_top(cand, n_cand, a.top, best);
+            select_top(cand, n_cand, a.top, best, partial);
         } else {
             // (more than are ranked at once, as where a few threads' logits outweigh
             // all others': the largest one by one, each below the one before)
@@ -339,18 +383,29 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a) 
     const auto get = [&](int i) { return __hip_atomic_load(&keys[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
     const int k = (a.top + a.nseg - 1) / a.nseg;
     __shared__ float4 sums[kMaxSeg];
+    // (all that is read here in one go: each of these loads takes a microsecond)
+    const int own = min(tid, a.nseg - 1), all = a.nseg * a.top;
+    uint64_t y[kHeld], kth = 0;
+    const float2 p = get2(part + 4 * own), q = get2(part + 4 * own + 2);
+    if (a.top) {
+        kth = get(own * a.top + k - 1);
+#pragma unroll
+        for (int j = 0; j < kHeld; j++) y[j] = get(min(tid + j * kThreads, all - 1));
+    }
     if (tid < a.nseg) {
-        const float2 p = get2(part + 4 * tid), q = get2(part + 4 * tid + 2);
-        if (a.top) group[tid] = get(tid * a.top + k - 1);
+        group[tid] = kth;
         sums[tid] = make_float4(p.x, p.y, q.x, 0.f);
     }
     __syncthreads();
     if (a.top) {
-        const uint64_t least = nth_largest(group, a.nseg, (a.top + k - 1) / k);
-        for (int i = tid; i < a.nseg * a.top; i += kThreads) {
-            const uint64_t y = get(i);
-            if (y != 0 && y >= least) cand[atomicAdd(&n_cand, 1)] = y;   // (at most top^2)
-        }
+        const uint64_t least = nth_largest(group, a.nseg, (a.top + k - 1) / k, partial);
+        const auto keep = [&](uint64_t x) {
+            if (x != 0 && x >= least) cand[atomicAdd(&n_cand, 1)] = x;   // (at most top^2)
+        };
+#pragma unroll
+        for (int j = 0; j < kHeld; j++)
+            if (tid + j * kThreads < all) keep(y[j]);
+        for (int i = tid + kHeld * kThreads; i < all; i += kThreads) keep(get(i));
     }
     float top = -INFINITY;
     for (int i = 0; i < a.nseg; i++) top = fmaxf(top, sums[i].x);
@@ -364,7 +419,7 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a) 
     }
     if (a.top) {
         __syncthreads();
-        select_top(cand, n_cand, a.top, best);
+        select_top(cand, n_cand, a.top, best, partial);
         __syncthreads();
     }
     finish_row(a, row, tok, logit, top, s, t, best);
