@@ -170,8 +170,8 @@ __device__ __forceinline__ void finish_row(const LogprobArgs& a, int row, int to
 // block that arrives last.  Logits are read in 16-byte words from the aligned
 // address at or below the row's first, those of a row's edges one by one.
 //
-// 512 rows of 32768 in fp32 (67 MB) take 14.8 us, 61 rows of 130001 in bf16 (16
-// MB) 14.3: eight instructions a logit, then about 5 us of dependent steps
+// 512 rows of 32768 in fp32 (67 MB) take 14.4 us, 61 rows of 130001 in bf16 (16
+// MB) 13.4: eight instructions a logit, then about 5 us of dependent steps
 // (the groups' keys, the words read again, the ranking, the join).  Segments
 // of 8192 in registers with a selection for each took 27 and 18 us.
 template <int DT>
