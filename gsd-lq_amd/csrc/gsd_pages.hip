@@ -164,9 +164,10 @@ __global__ void __launch_bounds__(kPlan) pages_take_kernel(const gsdh_paged_cach
         const int k = i < n ? min(max(want(i, &bad), 0), c.n_pages + 1) : 0;
         int sum;
         const int at = block_scan(k, scan, &sum);
-        if (i < n) off[i] = total + at;
-        // (a sum beyond the pool's pages cannot be met: no need to let it overflow)
-        total = min(total + sum, 0x3FFFFFFF);
+        // (a sum beyond the pool's pages cannot be met, and stays there: what
+        // kPlan entries add, at most 2^20 + 1 each, would pass 32 bits in the end)
+        if (i < n) off[i] = (int)min((unsigned)total + (unsigned)at, 0x3FFFFFFFu);
+        total = (int)min((unsigned)total + (unsigned)sum, 0x3FFFFFFFu);
     }
     __syncthreads();
     const int found = scan_pages(c.refs, c.n_pages, total, words, [](int r, int) { return r == 0; },

@@ -298,6 +298,47 @@ def test_largest_lists(lib):
     c.same()
 
 
+def test_long_lists_with_faults(lib):
+    """Lists longer than a planning block's threads: repeats, counts below
+    zero and indices outside in every part of them, forks of partly filled pages."""
+    banner("pages: lists of thousands with faults in them")
+    c = Paged("e4m3", 1, 9000, 8, 1, 64, False, 4000, 4)
+    c.k[:], c.v[:] = 1, 2
+    c.upload()
+    rng = np.random.default_rng(5)
+    seqs, counts = rng.integers(-2, 2002, 3500), rng.integers(-1, 12, 3500)
+    c.same(c.take([int(x) for x in seqs], [int(x) for x in counts]))
+    c.same(c.take([2, 2], [-1, 3]))   # the first place counts, whatever it asks
+    held = np.flatnonzero(c.lens)
+    assert len(held) > 1100 and (c.lens[held] % 8 != 0).sum() > 1000
+    src, dst = rng.choice(held, 3000), rng.integers(1990, 4002, 3000)
+    c.same(c.fork([int(x) for x in src], [int(x) for x in dst]))
+    c.same(c.free([int(x) for x in rng.integers(0, 4001, 2500)]))
+    c.compact()
+    c.same()
+
+
+def test_wants_beyond_32_bits(lib):
+    """Sequences that together want more pages than 32 bits count: the first
+    takes the whole pool of 2^20, the others stay as they were."""
+    banner("pages: 2100 sequences that want 2^20 pages each")
+    n, pages = 2100, 1 << 20
+    small = Paged("f16", 1, 8, 8, 1, 64, False, 1, 1)   # (its rows are not touched)
+    tables = ctypes.c_void_p()
+    lib.gsdh_malloc(ctypes.byref(tables), 4 * n * pages)
+    refs, lens = ints(np.zeros(pages, np.int32)), ints(np.zeros(n, np.int32))
+    c = small.struct(refs=refs.ptr, lens=lens.ptr, tables=tables.value, n_pages=pages, n_seqs=n, table_width=pages)
+    seqs, counts = ints(np.arange(n)), ints(np.full(n, 8 * pages))
+    lib.gsdh_pages_take(None, ctypes.byref(c), p(seqs), p(counts), n)
+    assert H(lens, np.int32, n).tolist() == [8 * pages] + [0] * (n - 1)
+    assert (H(refs, np.int32, pages) == 1).all() and small.status() == 2
+    row = np.empty(pages, np.int32)
+    lib.gsdh_memcpy_d2h(row.ctypes.data_as(ctypes.c_void_p), tables, row.nbytes, None)
+    lib.gsdh_stream_sync(None)
+    assert np.array_equal(row, np.arange(pages))
+    lib.gsdh_free(tables)
+
+
 def test_serving(lib):
     """The operators as a server runs them: prompts stored, decode steps of a
     changing batch (take, store, attend), forks, ends, compactions; every
