@@ -398,11 +398,11 @@ __device__ __forceinline__ void join_parts(const AttendArgs& a, const Unit& u, i
             }
 #pragma unroll
             for (int k = 0; k < kFan; k++) {
+                // (behind the last part: 0 times its words again.  A part whose weight is 0
+                // is added too, a NaN or an infinity among its V shows wherever it lies.)
                 const float f = weight[(k0 + k) * G + g];
-                if (f != 0.f) {   // (a part behind the last has none, whatever was read in its place)
-                    o.x += f * y[k].x;
-                    o.y += f * y[k].y;
-                }
+                o.x += f * y[k].x;
+                o.y += f * y[k].y;
             }
         }
         if (i >= words) break;
