@@ -1,6 +1,7 @@
 // gsd_paged.hip -- decode attention over a paged KV cache for a batch of
 // sequences, and RoPE with the append of K/V rows to its pages.
 #include <algorithm>
+#include <cfloat>
 
 #include "gsd_device.h"
 #include "gsd_paged.h"
@@ -536,13 +537,12 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) paged_attn_ker
         }
 
         float4v acc[NT];
-        float m = -INFINITY, l = 0.f;
+        float m = -INFINITY, l = 0.f, to_log2 = 1.f;   // m: the largest unscaled score; times to_log2: as an exponent of 2
 #pragma unroll
         for (int t = 0; t < NT; t++) acc[t] = float4v{0.f, 0.f, 0.f, 0.f};
         if (have && s.mine < s.t1) {
             // q's operand: head `col`, zeros beyond the group
             Parts<DT, 8> q[T::KS];
-            float to_log2;
             {
                 float x[T::KS][8], most = 0.f;
                 const float* qp = qbuf + (col < G ? col : 0) * HD;
@@ -600,7 +600,9 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) paged_attn_ker
                 }
                 const Runs runs = runs_of(held, place);
                 load_k(s, runs);
-                // x stays unscaled until the exponential; rows that the mask drops are -inf
+                // Scores and their maximum stay unscaled: what the exponential gets is the
+                // difference, so the largest has weight 1 whatever fp32 rounds off the
+                // scaled scores.  Rows that the mask drops are -inf.
                 float x[4 * H], top = -INFINITY;
 #pragma unroll
                 for (int e = 0; e < 4 * H; e++) x[e] = xs[e / 4][e % 4];
@@ -614,19 +616,19 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) paged_attn_ker
                 }
 #pragma unroll
                 for (int e = 0; e < 4 * H; e++) top = fmaxf(top, x[e]);
-                top = fmaxf(m, max_over_groups(top) * to_log2);
+                top = fmaxf(m, max_over_groups(top));
                 if (__any(top > m)) {
-                    const float f = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
+                    const float f = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - top) * to_log2);
 #pragma unroll
                     for (int n = 0; n < NT; n++) acc[n] *= f;
                     l *= f;
                     m = top;
                 }
                 // P as 2^14 times itself: the parts below fp16's normal range stay exact
-                const float base = m == -INFINITY ? 0.f : m - 14.f;
+                const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
                 for (int e = 0; e < 4 * H; e++) {
-                    x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], to_log2, -base));
+                    x[e] = __builtin_amdgcn_exp2f(fmaf(x[e] - base, to_log2, 14.f));
                     l += x[e];
                 }
                 const Parts<DT, 4 * H> p = split<DT, 4 * H>(x);
@@ -661,6 +663,8 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) paged_attn_ker
         }
 
         if (have) {
+            // (scores beyond fp32's range stay finite: a difference of two is a number)
+            if (m != -INFINITY) m = fminf(fmaxf(m * to_log2, -FLT_MAX), FLT_MAX);
             l = sum_over_groups(l);
             if (__any(lost)) {
                 l = __builtin_nanf("");

@@ -1,5 +1,6 @@
 """gsdh_paged_attention where single numbers are extreme: NaN and infinities
-that only a weight of zero meets."""
+that only a weight of zero meets, scores far beyond what fp32 tells apart by
+one."""
 import numpy as np
 import pytest
 
@@ -7,6 +8,7 @@ from gpu_util import banner
 from paged_util import Cache, grid, nan_bits
 
 pytestmark = pytest.mark.gpu
+STEP = 2.0 ** -24
 INF = {"f16": np.uint16(0x7C00), "bf16": np.uint16(0x7F80)}
 
 
@@ -55,3 +57,32 @@ def test_bad_v_under_a_weight_of_zero(lib, kind, what, at, places):
         # (the one weight: its parts carry 22 bits, its sum and quotient a step each)
         assert (np.abs(got[:, rest] - v[rest]) <= 2.0 ** -21 * np.abs(v[rest])).all(), place
         assert c.status() == 0
+
+
+def bound(mag, lens):
+    """Of outputs whose scores are exact: n / 128 + 96 steps of the sums (as in the attention's own tests)."""
+    return STEP * (np.asarray(lens)[:, None, None] / 128 + 96) * mag + 1e-30
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16", "e4m3"])
+@pytest.mark.parametrize("exponent", [13, 20, 23, 26, 30, 40])
+@pytest.mark.parametrize("scale", [1.0, 0.11])
+def test_large_scores(lib, kind, exponent, scale):
+    """Scores of 1e4 to 1e13: one position has all the weight, or several with
+    the very same score share it (different scores are 2^exponent / 16 * scale
+    apart at least, 56 in the smallest case; their products are exact)."""
+    banner(f"paged attention {kind}: q around 2^{exponent}, scale {scale}")
+    rng = np.random.default_rng(exponent)
+    lens = [1, 1, 2, 33, 300, 5000, 1]
+    c = Cache(kind, 1, sum(-(-n // 16) for n in lens), 16, 2, 64, False, len(lens), 320,
+              scales=np.ones((2, 1, 2), np.float32) if kind == "e4m3" else None).fill(lens, rng, grid)
+    q = grid(rng, (len(lens), 16, 64)) * np.float32(2.0 ** exponent)
+    got = c.run_attend(0, q, range(len(lens)), scale)
+    want, mag, top, _ = c.attend(0, q, range(len(lens)), np.float32(scale))
+    assert top.max() > 2.0 ** exponent * scale
+    assert np.isfinite(got).all()
+    assert (np.abs(got - want) <= bound(mag, lens)).all()
+    for i, n in enumerate(lens):
+        if n == 1:   # the only position's V row
+            v = c.values(1, 0, i, [0])[0]
+            assert (np.abs(got[i].reshape(2, 8, 64) - v[:, None]) <= 2.0 ** -21 * np.abs(v[:, None])).all()
