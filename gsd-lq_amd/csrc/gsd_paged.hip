@@ -44,7 +44,11 @@ constexpr int kMaxGroup = 16;      // query heads per KV head: the columns of on
 // fp32 inputs meet the cache's 16-bit rows as sums of 16-bit parts: two fp16
 // parts (22 bits; q scaled by a power of two so that its largest element is
 // below 1024, P by 2^14, so that small parts keep their bits) or three bf16
-// parts (24 bits).  e4m3 rows are exact in fp16.
+// parts (24 bits).  e4m3 rows are exact in fp16.  bf16 rows have fp32's range,
+// and the powers of two keep all sums within it: q's largest element is below
+// 2^-9 (256 products of such with finite K stay below 2^127), and a row's P add up
+// to less than 1.  What falls below fp32's least normal number for it, 2^-126, is
+// lost: parts of weights under 2^-80 of the largest, and bits of V under 2^-70.
 // ---------------------------------------------------------------------------
 struct AttendArgs {
     gsdh_paged_cache c;
@@ -557,13 +561,14 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) paged_attn_ker
                         most = fmaxf(most, fabsf(x[i][e]));
                     }
                 }
-                // 2^(9 - exponent of the largest), kept within the range of normal floats
+                // 2^(kTop - exponent of the largest), kept within the range of normal floats
+                constexpr int kTop = DT == GSDH_KV_BF16 ? -10 : 9;
                 unsigned ex = __float_as_uint(max_over_groups(most)) >> 23;
-                ex = ex < 16u ? 16u : ex > 254u ? 254u : ex;
+                ex = min(max(ex, 16u), 253u + (unsigned)min(kTop, 1));
                 // (a negative scale is in q's sign; one of 0 stays above it, so that a
                 // masked -inf times it stays -inf)
                 const float scale = a.scale * kLog2e * kscale;
-                const float up = copysignf(__uint_as_float((263u - ex) << 23), scale), down = __uint_as_float((ex - 9u) << 23);
+                const float up = copysignf(__uint_as_float((254u + kTop - ex) << 23), scale), down = __uint_as_float((ex - kTop) << 23);
                 to_log2 = fabsf(scale) * down;
                 if (to_log2 < 1.17549435e-38f) to_log2 = 1.17549435e-38f;
 #pragma unroll
@@ -578,6 +583,9 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) paged_attn_ker
             // loads are unconditional (after the wave's last tile that one again,
             // from the cache), so that a wait never has to drain those behind a
             // branch.
+            // P as 2^14 times itself: the parts below fp16's normal range stay exact; bf16:
+            // as P over a power of two that is above the row's number of positions
+            const float weight_of_top = DT == GSDH_KV_BF16 ? (float)(__builtin_clz((unsigned)(s.end - s.first)) - 32) : 14.f;
             int ahead = pages_from(s, s.mine + kAhead * kWaves), place = 0;   // the next kAhead tiles' pages; the next tile among the held
             for (int t = s.mine; t < s.t1; t += kWaves) {
                 float4v xs[H];
@@ -624,11 +632,10 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) paged_attn_ker
                     l *= f;
                     m = top;
                 }
-                // P as 2^14 times itself: the parts below fp16's normal range stay exact
                 const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
                 for (int e = 0; e < 4 * H; e++) {
-                    x[e] = __builtin_amdgcn_exp2f(fmaf(x[e] - base, to_log2, 14.f));
+                    x[e] = __builtin_amdgcn_exp2f(fmaf(x[e] - base, to_log2, weight_of_top));
                     l += x[e];
                 }
                 const Parts<DT, 4 * H> p = split<DT, 4 * H>(x);

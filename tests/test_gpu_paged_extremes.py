@@ -1,6 +1,6 @@
 """gsdh_paged_attention where single numbers are extreme: NaN and infinities
 that only a weight of zero meets, scores far beyond what fp32 tells apart by
-one."""
+one, rows near the ends of the cache type's range."""
 import numpy as np
 import pytest
 
@@ -86,3 +86,30 @@ def test_large_scores(lib, kind, exponent, scale):
         if n == 1:   # the only position's V row
             v = c.values(1, 0, i, [0])[0]
             assert (np.abs(got[i].reshape(2, 8, 64) - v[:, None]) <= 2.0 ** -21 * np.abs(v[:, None])).all()
+
+
+@pytest.mark.parametrize("k,q,v,scale", [
+    (0, 0, 110, 0.11), (0, 0, 126, 0.11), (0, 0, -60, 0.11),       # V near both ends of the type
+    (120, -120, 0, 0.11), (124, -124, 124, 0.11),                   # K as large, with a q as small
+    (120, 0, 0, 0.11 * 2.0 ** -120), (126, -6, 126, 0.11 * 2.0 ** -120),   # or a scale as small
+    (-100, 100, 0, 0.11), (-60, 60, 60, 0.11), (100, 10, 100, 1.0)])
+def test_bf16_rows_over_their_range(lib, k, q, v, scale):
+    """bf16 rows have fp32's range: whatever is finite gives the finite average
+    that the definition gives (K, q and V are small whole numbers times the powers
+    of two given, so that the scores' sums are exact)."""
+    banner(f"paged attention bf16: K 2^{k}, q 2^{q}, V 2^{v}, scale {scale:.3g}")
+    rng = np.random.default_rng(k + 1000)
+    lens = [1, 33, 300, 6000]
+    c = Cache("bf16", 1, sum(-(-n // 16) for n in lens), 16, 1, 64, False, len(lens), 400).fill(lens, rng, grid)
+    for s, n in enumerate(lens):
+        at = np.arange(n)
+        c.set_values(0, 0, s, at, grid(rng, (n, 1, 64)) * np.float32(2.0 ** k))
+        c.set_values(1, 0, s, at, grid(rng, (n, 1, 64)) * np.float32(2.0 ** v))
+    c.upload()
+    qs = grid(rng, (len(lens), 4, 64)) * np.float32(2.0 ** q)
+    got = c.run_attend(0, qs, range(len(lens)), scale)
+    want, mag, top, _ = c.attend(0, qs, range(len(lens)), np.float32(scale))
+    assert np.isfinite(got).all()
+    # the scores' scaling and their exponential: 8 steps each, twice (in weight and sum), where they do not pick one position
+    steps = np.asarray(lens)[:, None] / 128 + 96 + np.where(top < 1e4, 16 * top, 0)
+    assert (np.abs(got - want) <= STEP * steps[..., None] * mag + 1e-30).all()
