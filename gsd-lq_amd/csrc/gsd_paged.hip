@@ -395,7 +395,7 @@ __device__ __forceinline__ void join_parts(const AttendArgs& a, const Unit& u, i
                     weight[ew * G + eg] = f[0];
                     weight[(ew + kFan) * G + eg] = f[1];
                     if (ew == 0) {
-                        inv[eg] = sum == 0.f ? 0.f : vscale / sum;
+                        inv[eg] = vscale / sum;   // (sum 0: every score was -inf; NaN)
                         if (!whole) put2(a.part_ml + (slot_of(0) * G + eg) * 2, top, sum);
                     }
                 }
@@ -707,7 +707,8 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) paged_attn_ker
                     o.x += f * y.x; o.y += f * y.y; o.z += f * y.z; o.w += f * y.w;
                 }
                 if (whole) {
-                    const float f = sum == 0.f ? 0.f : vscale / sum;
+                    // (nothing to attend to: zeros; scores that are all -inf: NaN)
+                    const float f = u.row.end == u.row.first && sum == 0.f ? 0.f : vscale / sum;
                     *reinterpret_cast<float4*>(out + 4 * i) = make_float4(f * o.x, f * o.y, f * o.z, f * o.w);
                 } else {
                     const size_t slot = (size_t)((u.span + u.split) * nkv + head) * 2 + (u.split == 0);

@@ -250,7 +250,11 @@ typedef struct gsdh_paged_cache {
  * softmax(sm_scale q.K) V in fp32.  A sequence of length 0 gives a row of
  * zeros; a negative seqs[i] is padding, its row stays as it was; a row whose
  * sequence, length or pages lie outside the cache becomes NaN (and *status
- * says so); a row that holds NaN or an infinity gives NaN or an infinity.
+ * says so).  A NaN in what the row reads makes it NaN (in V: that dimension of
+ * it), an infinity in V makes that dimension infinite or NaN.  An infinity in K
+ * whose product with q is negative is a weight of 0, or, where the 16-bit parts
+ * that q is multiplied in differ in sign or are 0, makes the row NaN, as any other
+ * does; so does a row that has no weight but such.
  * n * table_width * page_size < 2^34.  n_heads / n_kv_heads 1 .. 16; strides in floats, multiples of 4,
  * at least n_heads * head_dim for out (q's rows may be one and the same).
  * workspace: gsdh_paged_attention_workspace_bytes(c, n, n_heads) bytes on this

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 from gpu_util import banner
-from paged_util import Cache, grid, nan_bits
+from paged_util import Cache, grid, nan_bits, normal
 
 pytestmark = pytest.mark.gpu
 STEP = 2.0 ** -24
@@ -113,3 +113,44 @@ def test_bf16_rows_over_their_range(lib, k, q, v, scale):
     # the scores' scaling and their exponential: 8 steps each, twice (in weight and sum), where they do not pick one position
     steps = np.asarray(lens)[:, None] / 128 + 96 + np.where(top < 1e4, 16 * top, 0)
     assert (np.abs(got - want) <= STEP * steps[..., None] * mag + 1e-30).all()
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_infinite_k(lib, kind):
+    """An infinity in K: a score of +inf or NaN leaves no distribution (NaN); one
+    of -inf is a weight of 0 (or NaN, where the parts of q differ in sign), and
+    a row of nothing else is NaN, not the zeros of an empty sequence."""
+    banner(f"paged attention {kind}: infinities in K")
+    rng = np.random.default_rng(21)
+    lens, at, dim = [300, 300, 5000, 1, 1, 40, 0], [7, 299, 4000, 0, 0, None, None], 11
+    c = Cache(kind, 1, sum(-(-n // 16) for n in lens), 16, 1, 64, False, len(lens), 320).fill(lens, rng, grid)
+    for s, p in enumerate(at):
+        if lens[s]:
+            i = c.rows(None, 0, np.arange(lens[s]) if p is None else [p], c.tables[s])
+            row = c.k[i]
+            row[..., dim] = INF[kind] | (0x8000 if s % 2 else 0)
+            c.k[i] = row
+    c.upload()
+    q = normal(rng, (len(lens), 16, 64))
+    got = c.run_attend(0, q, range(len(lens)), 0.1)
+    assert (got[6] == 0).all()
+    seen = set()
+    for s in range(6):
+        down = q[s, :, dim] * (-1 if s % 2 else 1) < 0   # heads whose score is -inf
+        assert not np.isfinite(got[s][~down]).any(), s
+        if at[s] is None or lens[s] == 1:
+            assert np.isnan(got[s]).all(), s
+            continue
+        keep = np.delete(np.arange(lens[s]), at[s])
+        k, v = (c.values(w, 0, s, keep)[:, 0] for w in (0, 1))
+        for h in np.flatnonzero(down):
+            if np.isnan(got[s, h]).all():
+                continue
+            x = k @ q[s, h].astype(np.float64) * np.float32(0.1)
+            e = np.exp(x - x.max())
+            e /= e.sum()
+            dot = (np.abs(k) @ np.abs(q[s, h])).max() * 0.1
+            steps = 2 * ((64 + 16) * dot + 8 * np.abs(x).max()) + lens[s] / 128 + 96
+            assert (np.abs(got[s, h] - e @ v) <= STEP * steps * (e @ np.abs(v)) + 1e-30).all(), (s, h)
+            seen.add((s, h))
+    assert len(seen) > 0
