@@ -306,10 +306,16 @@ __global__ void __launch_bounds__(256) pages_fork_rows_kernel(const gsdh_paged_c
 __global__ void __launch_bounds__(256) pages_free_kernel(const gsdh_paged_cache c, const int* seqs) {
     const int s = seqs[blockIdx.x];
     __shared__ int len;
-    if (threadIdx.x == 0) len = s >= 0 && s < c.n_seqs ? atomicExch(&c.lens[s], 0) : -1;   // (one of two that name it gets the length)
+    const bool in = s >= 0 && s < c.n_seqs;
+    if (threadIdx.x == 0) len = in ? atomicExch(&c.lens[s], 0) : -1;   // (one of two that name it gets the length)
     __syncthreads();
     if (!len_ok(c, len)) {
-        if (threadIdx.x == 0) page_status(c, GSDH_PAGES_BAD_INDEX);
+        if (threadIdx.x == 0) {
+            // (back again; one that names it, too, and came in between found a free
+            // sequence.  A load ahead of the exchange would be one more wait, 0.5 us.)
+            if (in) atomicExch(&c.lens[s], len);
+            page_status(c, GSDH_PAGES_BAD_INDEX);
+        }
         return;
     }
     int* t = c.tables + (size_t)s * c.table_width;

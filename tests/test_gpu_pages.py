@@ -444,3 +444,23 @@ def test_captured(lib):
             setattr(c, n, getattr(twin, n))
     lib.gsdh_graph_destroy(graph)
     lib.gsdh_stream_destroy(stream)
+
+
+def test_free_of_a_bad_length(lib):
+    """A sequence whose length no table can hold stays as it was, pages and all, however often it is listed."""
+    banner("pages: free of lengths outside the tables")
+    c = _cache(pages=40, lens=[16, 9, 20, 12], seqs=6, layers=1)
+    good = c.lens.copy()
+    c.lens[1], c.lens[2] = 8 * 10 + 1, -3
+    c.upload()
+    a = ints([1, 2, 0, 1, 2])
+    c.lib.gsdh_pages_free(None, c.at, p(a), 5)
+    c.refs[c.tables[0, :2]] = 0
+    c.tables[0, :2], c.lens[0], good[0] = -1, 0, 0
+    for name in ("refs", "lens", "tables"):
+        assert np.array_equal(c.download(name), getattr(c, name)), name
+    assert c.status() == 1
+    # with its length put right it gives its pages back
+    c.lens[:] = good
+    c.upload()
+    c.same(c.free([1, 2]))
