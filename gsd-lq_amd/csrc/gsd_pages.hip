@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(kPlan) pages_fork_kernel(const gsdh_paged_cach
         if (i < n) off[i] = total + at;
         total += sum;
     }
-    __syncthreads();   // (every length is read)
+    __syncthreads();
     const int found = scan_pages(c.refs, c.n_pages, total, words, [](int r, int) { return r == 0; },
         [&](int page, bool free_, int rank) {
             if (!free_ || rank >= total) return;
@@ -252,15 +252,15 @@ __global__ void __launch_bounds__(kPlan) pages_fork_kernel(const gsdh_paged_cach
         if (e.z % c.page_size && off[i] >= found) {
             plan[i].y = -1;
             bad |= GSDH_PAGES_EXHAUSTED;
-        } else {
-            c.lens[e.y] = e.z;
         }
     }
     if (bad) page_status(c, bad);
 }
 
-// One block of a fork's rows: blockIdx.y = 0: the entry's table row and the
-// shared pages' counts; else the filled rows of the last page in K or V of a layer.
+// One block of a fork's rows: blockIdx.y = 0: the entry's table row, the shared
+// pages' counts and the length, if all shared pages are the pool's (else the page
+// taken goes back; a look at them in the plan would be 1 us more of its chain);
+// else the filled rows of the last page in K or V of a layer.
 __global__ void __launch_bounds__(256) pages_fork_rows_kernel(const gsdh_paged_cache c, const int4* plan, int es) {
     const int4 e = plan[blockIdx.x];
     if (e.y < 0) return;
@@ -268,13 +268,25 @@ __global__ void __launch_bounds__(256) pages_fork_rows_kernel(const gsdh_paged_c
     const int* from = c.tables + (size_t)e.x * c.table_width;
     if (blockIdx.y == 0) {
         int* to = c.tables + (size_t)e.y * c.table_width;
+        bool out = false;
+        for (int j = threadIdx.x; j < full; j += 256) out |= (unsigned)from[j] >= (unsigned)c.n_pages;
+        out = __syncthreads_or(out);
+        if (out) {
+            if (threadIdx.x == 0) {
+                if (part) c.refs[e.w] = 0;
+                page_status(c, GSDH_PAGES_BAD_INDEX);
+            }
+            return;
+        }
         for (int j = threadIdx.x; j < full; j += 256) {
             const int p = from[j];
             to[j] = p;
-            if ((unsigned)p < (unsigned)c.n_pages) atomicAdd(&c.refs[p], 1);
-            else page_status(c, GSDH_PAGES_BAD_INDEX);
+            atomicAdd(&c.refs[p], 1);
         }
-        if (part && threadIdx.x == 0) to[full] = e.w;
+        if (threadIdx.x == 0) {
+            if (part) to[full] = e.w;
+            c.lens[e.y] = e.z;
+        }
         return;
     }
     if (!part) return;

@@ -298,7 +298,9 @@ int gsdh_paged_rope_store(void* stream, const gsdh_paged_cache* c, int layer, co
  *   order of the list, do not fit stay as they were (GSDH_PAGES_EXHAUSTED).
  * fork: the free sequence dst[i] becomes a second src[i]: full pages are
  *   shared, the rows of a last page that is partly filled are copied (every
- *   layer) to a page taken for it.  src as it was before the call.
+ *   layer) to a page taken for it.  src as it was before the call.  A source whose
+ *   table names a page outside the cache is left out (GSDH_PAGES_BAD_INDEX; among
+ *   its full pages: once the free pages are dealt out, the one it got is free again).
  * free: seqs[i] gives its pages back and has length 0; a sequence that is free
  *   already stays so.
  * compact: pages in use move to the lowest indices (the i-th lowest hole takes

@@ -446,6 +446,73 @@ def test_captured(lib):
     lib.gsdh_stream_destroy(stream)
 
 
+def test_forks_of_bad_tables_are_left_out(lib):
+    """A source whose table names a page outside the pool, wherever in it: the
+    entry leaves everything as it was, and keeps no page; the others are done."""
+    banner("pages: forks of tables with bad pages")
+    lens = [20, 9, 1200, 1200, 24, 700, 16]
+    c = _cache(pages=500, lens=lens, seqs=20, width=160, layers=1)
+    bad = {0: (0, 500), 2: (149, -1), 3: (70, 1 << 30), 4: (2, -9), 6: (1, 500)}
+    for s, (j, page) in bad.items():
+        c.tables[s, j] = page
+    c.upload()
+    src, dst = [0, 1, 2, 3, 5, 4, 6, 1, 0, 5, 2], [8, 9, 10, 11, 12, 13, 14, 15, 16, 17, 18]
+    a, b = ints(src), ints(dst)
+    c.lib.gsdh_pages_fork(None, c.at, p(a), p(b), len(src), p(c.work()), c.work().nbytes)
+    free, back = iter(c.free_pages()), []
+    for s, d in zip(src, dst):
+        if s in bad:
+            if lens[s] % c.page:
+                back.append(next(free))   # (dealt out and given back: its rows may be any)
+            continue
+        full, part = divmod(lens[s], c.page)
+        c.tables[d, :full] = c.tables[s, :full]
+        np.add.at(c.refs, c.tables[s, :full], 1)
+        c.lens[d] = lens[s]
+        if part:
+            new, old = next(free), c.tables[s, full]
+            c.tables[d, full], c.refs[new] = new, 1
+            for pool in (c.k, c.v):
+                pool[:, new, :part] = pool[:, old, :part]
+    for name in ("refs", "lens", "tables"):
+        assert np.array_equal(c.download(name), getattr(c, name)), name
+    for name in ("k", "v"):
+        assert np.array_equal(np.delete(c.download(name), back, 1), np.delete(getattr(c, name), back, 1)), name
+    assert len(back) == 2 and c.status() == 1
+
+
+def test_long_lists_of_forks_of_bad_tables(lib):
+    """The same beyond a planning block's threads: a bad source in every part of the list, often."""
+    banner("pages: 3000 forks, some of tables with bad pages")
+    c = Paged("e4m3", 1, 5000, 8, 1, 64, False, 4000, 4)
+    c.k[:], c.v[:] = 1, 2
+    rng = np.random.default_rng(8)
+    c.tables[:1000] = rng.permutation(5000)[:4000].reshape(1000, 4)
+    c.refs[c.tables[:1000].reshape(-1)] = 1
+    c.lens[:1000] = rng.integers(25, 33, 1000)
+    bad = rng.choice(1000, 200, replace=False)
+    c.tables[bad, rng.integers(0, 3, 200)] = 5000
+    c.upload()
+    src, dst = rng.integers(0, 1000, 3000), 1000 + np.arange(3000)
+    a, b = ints(src), ints(dst)
+    c.lib.gsdh_pages_fork(None, c.at, p(a), p(b), 3000, p(c.work()), c.work().nbytes)
+    good = ~np.isin(src, bad)
+    out = np.flatnonzero(c.lens[src] < 32)[1000:]   # (a page of its own for each: the first thousand have one)
+    done = good.copy()
+    done[out] = False
+    refs, tables, got = c.download("refs"), c.download("tables"), c.download("lens")
+    assert np.array_equal(got[1000:], np.where(done, c.lens[src], 0))
+    assert (tables[1000:][~done] == -1).all() and np.array_equal(tables[:1000], c.tables[:1000])
+    assert np.array_equal(tables[1000:][done][:, :3], c.tables[src[done], :3])
+    count = np.zeros(5000, np.int32)
+    held = np.concatenate([c.tables[:1000].reshape(-1), tables[1000:][done].reshape(-1)])
+    np.add.at(count, held[(held >= 0) & (held < 5000)], 1)
+    names = np.zeros(5000, bool)   # (the pages that the bad entries' places held stay held)
+    names[np.flatnonzero((c.refs == 1) & (count == 0))] = True
+    assert np.array_equal(refs, count + names)
+    assert len(out) and c.status() == 3
+
+
 def test_free_of_a_bad_length(lib):
     """A sequence whose length no table can hold stays as it was, pages and all, however often it is listed."""
     banner("pages: free of lengths outside the tables")
