@@ -290,7 +290,9 @@ int gsdh_paged_rope_store(void* stream, const gsdh_paged_cache* c, int layer, co
  * are taken lowest index first, in the order of the list, so the same calls
  * give the same tables.  An entry outside the cache is left out
  * (GSDH_PAGES_BAD_INDEX), and so is every place but the first that names a
- * sequence to be grown or forked into (GSDH_PAGES_TWICE).  workspace: gsdh_pages_workspace_bytes(c) bytes, 16-byte
+ * sequence to be grown or forked into (GSDH_PAGES_TWICE).  Sequences below 0 are
+ * outside the cache here: to pad a list, take 0 positions for a sequence, free one
+ * that is free, fork a free one into itself.  workspace: gsdh_pages_workspace_bytes(c) bytes, 16-byte
  * aligned; what it holds before a call does not matter.
  *
  * take: sequence seqs[i] grows by counts[i] >= 0 positions (pages taken where

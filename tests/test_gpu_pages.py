@@ -531,3 +531,71 @@ def test_free_of_a_bad_length(lib):
     c.lens[:] = good
     c.upload()
     c.same(c.free([1, 2]))
+
+
+def test_a_padded_step(lib):
+    """One captured step of up to five rows, replayed for fewer: the list of take
+    names every sequence, with a count of 0 where none is wanted, the rows of
+    store and attention are padded with -1, a list of sequences that ended with
+    one that is free.  No bit of the status word is raised."""
+    banner("pages: a padded step, captured")
+    rng = np.random.default_rng(17)
+    heads, kv, hd, rows, scale = 8, 2, 64, 5, 0.125
+    c = _cache("f16", 1, 40, 8, kv, hd, False, 7, 8, [7, 8, 30, 0, 0, 1, 0])
+    table = angles(64, hd)
+    da, w = D(table), (heads + 2 * kv) * hd
+    every, counts, ended = ints(range(7)), ints([0] * 7), ints([6] * 2)
+    seqs, pos = ints([-1] * rows), ints([0] * rows)
+    dx, q, out = D(np.zeros((rows, w), np.float32)), D(np.zeros((rows, heads, hd), np.float32)), D(np.zeros((rows, heads, hd), np.float32))
+    at = lambda h: ctypes.c_void_p(dx.ptr.value + 4 * h * hd)  # noqa: E731
+    ws, stream, graph = c.space(rows, heads), ctypes.c_void_p(), ctypes.c_void_p()
+    lib.gsdh_stream_create(ctypes.byref(stream))
+
+    def put(buf, a, dtype=np.int32):
+        a = np.ascontiguousarray(a, dtype)
+        lib.gsdh_memcpy_h2d(buf.ptr, a.ctypes.data_as(ctypes.c_void_p), a.nbytes, None)
+        lib.gsdh_stream_sync(None)
+
+    lib.gsdh_stream_begin_capture(stream)
+    lib.gsdh_pages_free(stream, c.at, p(ended), 2)
+    lib.gsdh_pages_take(stream, c.at, p(every), p(counts), 7)
+    lib.gsdh_paged_rope_store(stream, c.at, 0, at(0), w, at(heads), w, at(heads + kv), w, p(q), heads * hd, p(seqs), p(pos), rows, heads,
+                              p(da), 64, 1)
+    lib.gsdh_paged_attention(stream, c.at, 0, p(q), heads * hd, p(seqs), rows, heads, scale, 0, p(out), heads * hd, p(ws), ws.nbytes)
+    lib.gsdh_stream_end_capture(stream, ctypes.byref(graph))
+    for active, gone in (([0, 2, 5], [6, 6]), ([1, 0, 2, 5, 3], [6, 6]), ([3], [2, 6]), ([3, 0], [0, 1]), ([], [6, 4])):
+        x = grid(rng, (rows, heads + 2 * kv, hd))
+        put(ended, gone)
+        put(counts, [int(s in active) for s in range(7)])
+        # (the sequence that ends and is active starts again)
+        where = [0 if s in gone else int(c.lens[s]) for s in active]
+        put(seqs, active + [-1] * (rows - len(active)))
+        put(pos, where + [0] * (rows - len(active)))
+        put(dx, x.reshape(rows, w), np.float32)
+        lib.gsdh_memcpy_h2d(out.ptr, np.full(rows * heads * hd, 7, np.float32).ctypes.data_as(ctypes.c_void_p), 4 * rows * heads * hd, None)
+        lib.gsdh_graph_replay(graph, stream)
+        lib.gsdh_stream_sync(stream)
+        # the same on the model
+        for s in set(gone):
+            k = c.need(int(c.lens[s]))
+            np.add.at(c.refs, c.tables[s, :k], -1)
+            c.tables[s, :k], c.lens[s] = -1, 0
+        for s in sorted(active):
+            if c.lens[s] % c.page == 0:
+                new = c.free_pages()[0]
+                c.tables[s, c.lens[s] // c.page], c.refs[new] = new, 1
+            c.lens[s] += 1
+        rot = rotate(x[:len(active), heads:heads + kv], table[where], 1)
+        for t, (s, n) in enumerate(zip(active, where)):
+            c.set_values(0, 0, s, [n], rot[t:t + 1])
+            c.set_values(1, 0, s, [n], x[t:t + 1, heads + kv:])
+        c.same(0)
+        got = H(out, np.float32, rows * heads * hd).reshape(rows, heads, hd)
+        assert (got[len(active):] == 7).all()
+        if active:
+            qs = rotate(x[:len(active), :heads], table[where], 1)
+            want, mag, top, dot = c.attend(0, qs, active, np.float32(scale))
+            eps = 2 * ((hd + 16) * dot + 8 * top) + 64 / 128 + 96   # (the bound of the attention's own tests)
+            assert (np.abs(got[:len(active)] - want) <= 2.0 ** -24 * eps[..., None] * mag).all()
+    lib.gsdh_graph_destroy(graph)
+    lib.gsdh_stream_destroy(stream)
