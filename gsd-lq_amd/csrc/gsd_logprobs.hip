@@ -333,7 +333,8 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(const LogprobArgs a) 
             select_top(cand, n_cand, a.top, best, partial);
         } else {
             // (more than are ranked at once, as where a few threads' logits outweigh
-            // all others': the largest one by one, each below the one before)
+            // all others': the largest one by one, each below the one before.  61 rows of
+            // 130001 in fp32, the largest at 8 threads of the 256, top 20: 71 us, not 14)
             uint64_t before = ~0ull;
             for (int r = 0; r < a.top; r++) {
                 uint64_t most = 0;

@@ -4,8 +4,11 @@
 // The bookkeeping (refs, tables, lens: a few hundred KB at most) is one
 // block's work: its order decides which page a sequence gets, and a block
 // can keep that order with barriers instead of launches: a chain of loads of
-// 3 us (take) to 6 (fork, compact) on a pool of a few thousand pages.  What
-// moves rows runs over the whole chip and is bound by memory (5 TB/s read and written).
+// 3 us (take) to 6 (fork, compact) on pools of 216 and 372 pages.  Counts are
+// looked at 8192 pages a step, about 1 us, one step after another: take on 131072
+// pages of which the lowest nine tenths are in use 18 us, compact's two passes with
+// 11700 pages freed 110 us.  What moves rows runs over the whole chip and is bound by
+// memory (5 TB/s read and written; 200 pages of 2 MB copied, 839 MB moved: 149 us).
 #include <algorithm>
 
 #include "gsd_device.h"

@@ -255,12 +255,15 @@ typedef struct gsdh_paged_cache {
  * whose product with q is negative is a weight of 0, or, where the 16-bit parts
  * that q is multiplied in differ in sign or are 0, makes the row NaN, as any other
  * does; so does a row that has no weight but such.
- * n * table_width * page_size < 2^34.  n_heads / n_kv_heads 1 .. 16; strides in floats, multiples of 4,
- * at least n_heads * head_dim for out (q's rows may be one and the same).
+ * n * (table_width * page_size / 16 + 130) < 2^31 - 1 (the quotient rounded
+ * down), n * n_kv_heads < 2^30.  n_heads / n_kv_heads 1 .. 16; strides in floats,
+ * multiples of 4, at least n_heads * head_dim for out (q's rows may be one and the
+ * same).
  * workspace: gsdh_paged_attention_workspace_bytes(c, n, n_heads) bytes on this
  * device (0 for an invalid shape), zero before its first call and 16-byte
  * aligned; each call leaves it ready for the next, which may have other lengths
- * and fewer rows but passes the same workspace_bytes.  The result does not depend on how the launch's blocks are ordered. */
+ * and fewer rows but passes the same workspace_bytes.  The result does not depend
+ * on how the launch's blocks are ordered. */
 uint64_t gsdh_paged_attention_workspace_bytes(const gsdh_paged_cache* c, int n, int n_heads);
 int gsdh_paged_attention(void* stream, const gsdh_paged_cache* c, int layer, const float* q,
                          int64_t q_stride, const int* seqs, int n, int n_heads, float sm_scale,
