@@ -569,11 +569,12 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) paged_attn_ker
                 unsigned ex = __float_as_uint(max_over_groups(most)) >> 23;
                 ex = min(max(ex, 16u), 253u + (unsigned)min(kTop, 1));
                 // (a negative scale is in q's sign; one of 0 stays above it, so that a
-                // masked -inf times it stays -inf)
+                // masked -inf times it stays -inf, and no farther than 2^-149: a bf16
+                // row's unscaled scores reach 2^127)
                 const float scale = a.scale * kLog2e * kscale;
                 const float up = copysignf(__uint_as_float((254u + kTop - ex) << 23), scale), down = __uint_as_float((ex - kTop) << 23);
                 to_log2 = fabsf(scale) * down;
-                if (to_log2 < 1.17549435e-38f) to_log2 = 1.17549435e-38f;
+                if (to_log2 < FLT_TRUE_MIN) to_log2 = FLT_TRUE_MIN;
 #pragma unroll
                 for (int i = 0; i < T::KS; i++) {
 #pragma unroll

@@ -250,11 +250,11 @@ typedef struct gsdh_paged_cache {
  * softmax(sm_scale q.K) V in fp32.  A sequence of length 0 gives a row of
  * zeros; a negative seqs[i] is padding, its row stays as it was; a row whose
  * sequence, length or pages lie outside the cache becomes NaN (and *status
- * says so).  A NaN in what the row reads makes it NaN (in V: that dimension of
- * it), an infinity in V makes that dimension infinite or NaN.  An infinity in K
- * whose product with q is negative is a weight of 0, or, where the 16-bit parts
- * that q is multiplied in differ in sign or are 0, makes the row NaN, as any other
- * does; so does a row that has no weight but such.
+ * says so).  A NaN makes NaN of all that is formed from it: of a head (in q), of
+ * the heads of a KV head (in K), of one dimension of these (in V); an infinity in V
+ * makes that dimension infinite or NaN.  An infinity in K makes NaN, too, but where
+ * its product with q is -inf, also in the 16-bit parts that q is split in: that is a
+ * weight of 0, and NaN if no position has more.
  * n * (table_width * page_size / 16 + 130) < 2^31 - 1 (the quotient rounded
  * down), n * n_kv_heads < 2^30.  n_heads / n_kv_heads 1 .. 16; strides in floats,
  * multiples of 4, at least n_heads * head_dim for out (q's rows may be one and the

@@ -115,6 +115,25 @@ def test_bf16_rows_over_their_range(lib, k, q, v, scale):
     assert (np.abs(got - want) <= STEP * steps[..., None] * mag + 1e-30).all()
 
 
+@pytest.mark.parametrize("k", [0, 100, 126])
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-42])
+def test_bf16_scale_of_zero(lib, k, scale):
+    """A scale of 0 (or next to it) weighs all positions alike (nearly), however large K is."""
+    banner(f"paged attention bf16: K 2^{k}, scale {scale:.3g}")
+    rng = np.random.default_rng(k)
+    lens = [1, 40, 3000]
+    c = Cache("bf16", 1, sum(-(-n // 16) for n in lens), 16, 1, 64, False, len(lens), 200).fill(lens, rng, grid)
+    for s, n in enumerate(lens):
+        c.set_values(0, 0, s, np.arange(n), grid(rng, (n, 1, 64)) * np.float32(2.0 ** k))
+    c.upload()
+    q = grid(rng, (len(lens), 4, 64))
+    got = c.run_attend(0, q, range(len(lens)), scale)
+    want, mag, top, _ = c.attend(0, q, range(len(lens)), float(np.float32(scale)))
+    # (1e-42 times log2 e is rounded to a multiple of 2^-149: half of that to 1.4e-42, of the score, twice)
+    steps = np.asarray(lens)[:, None] / 128 + 96 + 16 * top + 2 * top * 2.0 ** -150 / 1.4e-42 / STEP
+    assert (np.abs(got - want) <= STEP * steps[..., None] * mag + 1e-30).all()
+
+
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
 def test_infinite_k(lib, kind):
     """An infinity in K: a score of +inf or NaN leaves no distribution (NaN); one
