@@ -220,43 +220,6 @@ __device__ __forceinline__ float max_over_groups(float v) {   // over lanes l, l
 }
 __device__ __forceinline__ float sum_over_groups(float v) { return swap_add32(swap_add16(v, v), swap_add16(v, v), false); }
 
-// E (4 or 8) fp32 values as parts of 16 bits whose sum they are
-template <int DT, int E>
-struct Parts {
-    static constexpr int N = DT == GSDH_KV_BF16 ? 3 : 2;
-    typedef uint32_t Words __attribute__((ext_vector_type(E / 2)));
-    Words w[N];
-};
-template <int DT, int E>
-__device__ __forceinline__ Parts<DT, E> split(const float (&x)[E]) {
-    Parts<DT, E> p;
-    if constexpr (DT == GSDH_KV_BF16) {
-        // truncated parts: 8 + 8 + 8 bits, exact
-#pragma unroll
-        for (int i = 0; i < E / 2; i++) {
-            float y[2] = {x[2 * i], x[2 * i + 1]};
-#pragma unroll
-            for (int n = 0; n < 3; n++) {
-                const uint32_t lo = __float_as_uint(y[0]), hi = __float_as_uint(y[1]);
-                p.w[n][i] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
-                y[0] -= __uint_as_float(lo & 0xFFFF0000u);
-                y[1] -= __uint_as_float(hi & 0xFFFF0000u);
-            }
-        }
-    } else {
-        typedef _Float16 Halves __attribute__((ext_vector_type(E)));
-        Halves h, l;
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            h[e] = (_Float16)x[e];
-            l[e] = (_Float16)(x[e] - (float)h[e]);
-        }
-        p.w[0] = __builtin_bit_cast(typename Parts<DT, E>::Words, h);
-        p.w[1] = __builtin_bit_cast(typename Parts<DT, E>::Words, l);
-    }
-    return p;
-}
-
 template <int DT>
 __device__ __forceinline__ float4v mma(const u32x4v a, const u32x4v b, float4v c) {   // 16 x 16 x 32
     if constexpr (DT == GSDH_KV_BF16)
@@ -274,12 +237,6 @@ __device__ __forceinline__ float4v mma(const u32x2v a, const u32x2v b, float4v c
         return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s4, a), __builtin_bit_cast(s4, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(half4, a), __builtin_bit_cast(half4, b), c, 0, 0, 0);
-}
-
-// two e4m3 values (the low or the high half of w) as fp16: exact
-template <bool HI>
-__device__ __forceinline__ uint32_t e4m3x2(uint32_t w) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
 }
 
 // The rows of one tile as a lane holds them, and where they come from.

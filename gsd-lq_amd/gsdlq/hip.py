@@ -45,6 +45,7 @@ SIGNATURES = {
     "gsdh_prefill_attention": [vp] + [vp] * 4 + [i32] * 7 + [f32],
     "gsdh_unpack_codes": [vp, vp, i64, i32, vp, vp],
     "gsdh_paged_attention": [vp, vp, i32, vp, i64, vp, i32, i32, f32, i32, vp, i64, vp, u64],
+    "gsdh_paged_chunk_attention": [vp, vp, i32, vp, i32, i64, vp, vp, i32, i32, i32, f32, i32, vp, i64, vp, u64],
     "gsdh_paged_rope_store": [vp, vp, i32] + [vp, i64] * 4 + [vp, vp, i32, i32, vp, i32, i32],
     "gsdh_pages_take": [vp, vp, vp, vp, i32],
     "gsdh_pages_fork": [vp, vp, vp, vp, i32, vp, u64],
@@ -83,6 +84,7 @@ RESTYPES = {"gsdh_model_device_bytes": (u64, [vp]), "gsdh_model_stream": (vp, [v
             "gsdh_attention_workspace_bytes": (u64, [i32, i32, i32, i32]),
             "gsdh_model_fused_ffn": (i32, [vp, i32]),
             "gsdh_paged_attention_workspace_bytes": (u64, [vp, i32, i32]),
+            "gsdh_paged_chunk_attention_workspace_bytes": (u64, [vp, i32, i32, i32]),
             "gsdh_pages_workspace_bytes": (u64, [vp]),
             "gsdh_token_logprobs_workspace_bytes": (u64, [i32, i32, i32]),
             "gsdh_last_error": (ctypes.c_char_p, [])}
@@ -105,6 +107,7 @@ class GsdPagedCache(ctypes.Structure):
 
 KV_TYPES = {"f16": 0, "bf16": 1, "e4m3": 2}
 LOGIT_TYPES = {"f32": 0, "f16": 1, "bf16": 2}
+ROW_TYPES = {"f32": 0, "f16": 1, "bf16": 2}
 # bits of a paged cache's status word
 PAGES_BAD_INDEX, PAGES_EXHAUSTED, PAGES_SHARED, PAGES_TWICE = 1, 2, 4, 8
 

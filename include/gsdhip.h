@@ -270,6 +270,39 @@ int gsdh_paged_attention(void* stream, const gsdh_paged_cache* c, int layer, con
                          int window, float* out, int64_t out_stride, void* workspace,
                          uint64_t workspace_bytes);
 
+/* Types of the rows that the operators below take and give. */
+enum { GSDH_ROWS_F32 = 0, GSDH_ROWS_F16 = 1, GSDH_ROWS_BF16 = 2 };
+
+/* Causal attention of a chunk of new tokens per sequence (gsd_cpu_gqa_attention,
+ * gsd_lq_cpu_engine.c:264-330, for prompts, drafts and single tokens side by
+ * side): rows starts[i] .. starts[i + 1] - 1 of q are the last tokens of sequence
+ * seqs[i] (seqs NULL: sequence i), in order, their K/V rows already stored; of m
+ * rows, row j is at position p = lens[seqs[i]] - m + j and attends over positions
+ * max(0, p + 1 - window) .. p (window 0: all of them).  starts: int [n + 1],
+ * rising, within 0 .. n_tokens.  Rows of q and out are of `dtype`, RoPE applied:
+ * fp32 over any cache, the cache's own 16-bit type, or either over an e4m3 cache;
+ * row t at q + t * q_stride, n_heads x head_dim.  With fp32 rows the result is
+ * exact to fp32's rounding; with 16-bit rows the weights are rounded once to the
+ * type, sums and statistics stay fp32.
+ * A negative seqs[i] is padding, and rows that no chunk names stay as they were, as
+ * do those of a chunk whose starts fall or lie outside 0 .. n_tokens
+ * (GSDH_PAGES_BAD_INDEX).  A chunk of 0 rows is one without work.  A chunk of a
+ * sequence outside the cache, or that is longer than its sequence, becomes NaN, and
+ * so does a row that sees a position whose page lies outside the pool; *status says
+ * so.  What a row does not see never reaches it, NaN and infinities included; what it
+ * sees acts as in gsdh_paged_attention, an infinity in V as a NaN where a tile has a
+ * mask.  Rows that two chunks name hold either's.
+ * n_heads / n_kv_heads 1 .. 16; rows 16-byte aligned, strides in elements, of whole
+ * 16 bytes, at least n_heads * head_dim for out.  workspace:
+ * gsdh_paged_chunk_attention_workspace_bytes(c, n, n_tokens, n_heads) bytes (0 for an
+ * invalid shape), 16-byte aligned; what it holds before a call does not matter, and
+ * more n_tokens never need less.  Equal calls give equal bits. */
+uint64_t gsdh_paged_chunk_attention_workspace_bytes(const gsdh_paged_cache* c, int n, int n_tokens, int n_heads);
+int gsdh_paged_chunk_attention(void* stream, const gsdh_paged_cache* c, int layer, const void* q, int dtype,
+                               int64_t q_stride, const int* seqs, const int* starts, int n, int n_tokens,
+                               int n_heads, float sm_scale, int window, void* out, int64_t out_stride,
+                               void* workspace, uint64_t workspace_bytes);
+
 /* gsd_cpu_rope_and_store_kv (gsd_lq_cpu_engine.c:185-262) for n tokens of any
  * sequences: token t is position positions[t] of sequence seqs[t]; its rows
  * q[t * q_stride ..] (n_heads), k[t * k_stride ..] and v[t * v_stride ..]
