@@ -1,0 +1,333 @@
+// gsd_rope.hip -- rotary positions: rows of q and K turned by angles that are
+// formed from the positions, to rows or into the paged cache.
+#include <cmath>
+
+#include "gsd_device.h"
+#include "gsd_paged.h"
+
+using namespace gsd;
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMostPairs = 1024;   // of a block's tokens
+
+struct TurnArgs {
+    const void *x, *k, *v;   // rows to rows: x alone
+    void* out;
+    const double* freqs;
+    const int *seqs, *positions;
+    gsdh_paged_cache c;
+    int64_t x_stride, k_stride, v_stride, out_stride;
+    int n, heads, nkv, hd;        // heads: of x
+    int pairs, interleaved;
+    int turned_runs, head_runs;   // threads' runs of a head that is turned: of four pairs; with those that follow
+    int tokens, parts;            // of a block; blocks of a token
+    int layer, in_place;
+    float scale;
+};
+
+template <typename T>
+struct Vec {
+    typedef T four __attribute__((ext_vector_type(4)));
+};
+
+template <typename RT, bool VEC>
+__device__ __forceinline__ void load_run(const RT* p, int count, float* x) {   // up to four values
+    if constexpr (VEC) {
+        const auto w = *reinterpret_cast<const typename Vec<RT>::four*>(p);
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = (float)w[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = e < count ? (float)p[e] : 0.f;
+    }
+}
+template <typename RT, bool VEC>
+__device__ __forceinline__ void store_run(RT* p, int count, const float* x) {
+    if constexpr (VEC) {
+        typename Vec<RT>::four w;
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = (RT)x[e];
+        *reinterpret_cast<typename Vec<RT>::four*>(p) = w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (e < count) p[e] = (RT)x[e];
+    }
+}
+// the same into a cache of type DT (bytes at p); e4m3: divided by the scale, beyond +-448 clamped, NaN kept
+template <int DT, bool VEC>
+__device__ __forceinline__ void cache_run(unsigned char* p, int count, const float* x, float scale) {
+    if constexpr (DT == GSDH_KV_F16) {
+        store_run<_Float16, VEC>(reinterpret_cast<_Float16*>(p), count, x);
+    } else if constexpr (DT == GSDH_KV_BF16) {
+        store_run<__bf16, VEC>(reinterpret_cast<__bf16*>(p), count, x);
+    } else {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            y[e] = x[e] / scale;
+            y[e] = y[e] > 448.f ? 448.f : y[e] < -448.f ? -448.f : y[e];
+        }
+        const uint32_t w =
+            (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false), true);
+        if constexpr (VEC) {
+            *reinterpret_cast<uint32_t*>(p) = w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (e < count) p[e] = (unsigned char)(w >> 8 * e);
+        }
+    }
+}
+
+// y_i = c x_i - s x_j, y_j = s x_i + c x_j, (c, s) = scale (cos, sin)(position *
+// frequency): turns t = position * (frequency / 2 pi) in fp64, so that far
+// positions keep their angles (an fp32 product is off by 2^-24 of it: half a
+// degree at position 131072 and frequency 1), t's fraction rounded once to fp32.
+//
+// A thread: four pairs of a head, or up to eight values that are not turned
+// (the rest of a head, V).  A block's angles are formed once, in LDS, while its
+// rows are on their way.  DT < 0: rows to rows; else K and V go to the cache.
+// VEC: runs of four values are aligned (else element by element).
+//
+// Bound by memory for a prompt's rows and by the launch for a step's.
+template <typename RT, int DT, bool VEC>
+__global__ void __launch_bounds__(kThreads) turn_kernel(const TurnArgs a) {
+    __shared__ float2 cs[kMostPairs];
+    const int per_token = (a.heads + (DT < 0 ? 0 : a.nkv)) * a.head_runs + (DT < 0 ? 0 : a.nkv * (a.hd / 8));
+    const int first = a.tokens > 1 ? (int)blockIdx.x * a.tokens : (int)blockIdx.x / a.parts;
+    const int item = a.tokens > 1 ? (int)threadIdx.x : (int)(blockIdx.x % (unsigned)a.parts) * kThreads + (int)threadIdx.x;
+    const int tok = first + item / per_token, in_token = item % per_token;   // (one token: item < per_token, or nothing to do)
+    const bool mine = item < a.tokens * per_token && tok < a.n;
+
+    // what, and from where
+    int seq = 0, pos = 0, page = 0;
+    uint32_t bad = 0;
+    bool live = mine;
+    if constexpr (DT >= 0) {
+        if (mine) {
+            seq = a.seqs[tok];
+            pos = a.positions[tok];
+            live = seq >= 0;
+            if (live) {
+                if (seq >= a.c.n_seqs || pos < 0 || pos >= a.c.table_width * a.c.page_size || pos >= a.c.lens[seq]) {
+                    bad = GSDH_PAGES_BAD_INDEX;
+                } else {
+                    page = a.c.tables[(size_t)seq * a.c.table_width + pos / a.c.page_size];
+                    if ((unsigned)page >= (unsigned)a.c.n_pages) bad = GSDH_PAGES_BAD_INDEX;
+                    else if (a.c.refs && a.c.refs[page] != 1) bad = GSDH_PAGES_SHARED;
+                }
+                if (bad && in_token == 0) page_status(a.c, bad);
+                live = !bad;
+            }
+        }
+    }
+    const int turned_heads = a.heads + (DT < 0 ? 0 : a.nkv), turned_items = turned_heads * a.head_runs;
+    const bool is_v = DT >= 0 && in_token >= turned_items;
+    const int head = is_v ? (in_token - turned_items) / (a.hd / 8) : in_token / a.head_runs;
+    const int run = is_v ? (in_token - turned_items) % (a.hd / 8) : in_token % a.head_runs;
+    const bool is_k = DT >= 0 && !is_v && head >= a.heads;
+    const bool turns = !is_v && run < a.turned_runs;
+    int i0, i1, n0, n1;   // the two runs of up to four values
+    if (turns) {
+        const int left = a.pairs - 4 * run;
+        if (a.interleaved) {
+            i0 = 8 * run;
+            i1 = i0 + 4;
+            n0 = min(4, 2 * left);
+            n1 = max(0, min(4, 2 * left - 4));
+        } else {
+            i0 = 4 * run;
+            i1 = i0 + a.pairs;
+            n0 = n1 = min(4, left);
+        }
+    } else {
+        i0 = is_v ? 8 * run : 2 * a.pairs + 8 * (run - a.turned_runs);
+        i1 = i0 + 4;
+        n0 = min(4, a.hd - i0);
+        n1 = max(0, min(4, a.hd - i1));
+    }
+    if (!turns && !is_k && !is_v && a.in_place) live = false;
+    const RT* src = static_cast<const RT*>(is_v ? a.v : is_k ? a.k : a.x) +
+                    (int64_t)tok * (is_v ? a.v_stride : is_k ? a.k_stride : a.x_stride) + (int64_t)(is_k ? head - a.heads : head) * a.hd;
+    float x[8];
+    if (live) {
+        load_run<RT, VEC>(src + i0, n0, x);
+        load_run<RT, VEC>(src + i1, n1, x + 4);
+    }
+    for (int p = threadIdx.x; p < a.tokens * a.pairs; p += kThreads) {
+        const int t = first + p / a.pairs;
+        if (t >= a.n) break;
+        const double turn = (double)a.positions[t] * (a.freqs[p % a.pairs] * 0.15915494309189533577);   // 1 / 2 pi
+        float s, c;
+        sincospif((float)(2.0 * (turn - rint(turn))), &s, &c);
+        cs[p] = make_float2(c * a.scale, s * a.scale);
+    }
+    __syncthreads();
+    if (!live) return;
+    if (turns) {
+        const float2* const w = cs + (tok - first) * a.pairs + 4 * run;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (!VEC && 4 * run + e >= a.pairs) break;
+            const float2 r = w[e];
+            const float u = a.interleaved ? x[2 * e] : x[e], v = a.interleaved ? x[2 * e + 1] : x[e + 4];
+            const float y = u * r.x - v * r.y, z = u * r.y + v * r.x;
+            if (a.interleaved) {
+                x[2 * e] = y;
+                x[2 * e + 1] = z;
+            } else {
+                x[e] = y;
+                x[e + 4] = z;
+            }
+        }
+    }
+    if constexpr (DT >= 0) {
+        if (is_k || is_v) {
+            constexpr int ES = DT == GSDH_KV_E4M3 ? 1 : 2;
+            const int h = is_k ? head - a.heads : head, ps = a.c.page_size, slot = pos % ps;
+            const float scale = DT == GSDH_KV_E4M3 ? (is_v ? a.c.v_scale : a.c.k_scale)[a.layer * a.nkv + h] : 1.f;
+            const size_t at = ((size_t)a.layer * a.c.n_pages + page) * ps * a.nkv * a.hd +
+                              (a.c.head_major ? (size_t)h * ps + slot : (size_t)slot * a.nkv + h) * a.hd;
+            unsigned char* dst = static_cast<unsigned char*>(is_v ? a.c.v : a.c.k) + at * ES;
+            cache_run<DT, VEC>(dst + (size_t)i0 * ES, n0, x, scale);
+            cache_run<DT, VEC>(dst + (size_t)i1 * ES, n1, x + 4, scale);
+            return;
+        }
+    }
+    RT* dst = static_cast<RT*>(a.out) + (int64_t)tok * a.out_stride + (int64_t)head * a.hd;
+    store_run<RT, VEC>(dst + i0, n0, x);
+    store_run<RT, VEC>(dst + i1, n1, x + 4);
+}
+
+int check_rope(const gsdh_rope* r, int head_dim, int dtype, const char* who) {
+    if (!r) return fail(-1, "%s: null rope", who);
+    if (r->rotary_dim < 2 || r->rotary_dim % 2 || r->rotary_dim > head_dim)
+        return fail(-1, "%s: rotary_dim %d is not even or outside 2..%d", who, r->rotary_dim, head_dim);
+    if (dtype < GSDH_ROWS_F32 || dtype > GSDH_ROWS_BF16) return fail(-1, "%s: type %d", who, dtype);
+    if (!r->freqs || reinterpret_cast<uintptr_t>(r->freqs) % 8) return fail(-1, "%s: frequencies null or not aligned", who);
+    return 0;
+}
+
+bool rows_fit(const void* p, int64_t stride, int64_t width, int dtype) {
+    const int unit = dtype == GSDH_ROWS_F32 ? 4 : 8;
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % unit == 0 && stride >= width;
+}
+
+// the blocks' shape; false: too many
+bool plan_turn(TurnArgs& a, const gsdh_rope& r, bool paged) {
+    a.freqs = r.freqs;
+    a.pairs = r.rotary_dim / 2;
+    a.interleaved = r.interleaved != 0;
+    a.scale = r.scale;
+    a.turned_runs = (a.pairs + 3) / 4;
+    a.head_runs = a.turned_runs + (a.hd - r.rotary_dim + 7) / 8;
+    const int64_t items = (int64_t)(a.heads + (paged ? a.nkv : 0)) * a.head_runs + (paged ? (int64_t)a.nkv * (a.hd / 8) : 0);
+    // short tokens share a block
+    a.tokens = (int)(items <= kThreads / 2 ? kThreads / items : 1);
+    if (a.tokens * a.pairs > kMostPairs) a.tokens = kMostPairs / a.pairs;
+    a.parts = (int)((items + kThreads - 1) / kThreads);
+    return (a.tokens > 1 ? (int64_t)a.n : (int64_t)a.n * a.parts) <= 0x7FFFFFFF;
+}
+
+template <typename RT, int DT>
+void launch_turn(const TurnArgs& a, bool vec, hipStream_t st) {
+    const dim3 grid((unsigned)(a.tokens > 1 ? (a.n + a.tokens - 1) / a.tokens : a.n * a.parts)), block(kThreads);
+    if (vec) hipLaunchKernelGGL((turn_kernel<RT, DT, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((turn_kernel<RT, DT, false>), grid, block, 0, st, a);
+}
+template <int DT>
+void launch_turn_rows(const TurnArgs& a, int dtype, bool vec, hipStream_t st) {
+    if (dtype == GSDH_ROWS_F32) launch_turn<float, DT>(a, vec, st);
+    else if (dtype == GSDH_ROWS_F16) launch_turn<_Float16, DT>(a, vec, st);
+    else launch_turn<__bf16, DT>(a, vec, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+int gsdh_rope_frequencies(int kind, double theta, int rotary_dim, double factor, double context, double low, double high, double* freqs) {
+    const char* who = "rope_frequencies";
+    if (kind < GSDH_ROPE_PLAIN || kind > GSDH_ROPE_BY_PARTS) return fail(-1, "%s: kind %d", who, kind);
+    if (rotary_dim < 2 || rotary_dim % 2) return fail(-1, "%s: rotary_dim %d", who, rotary_dim);
+    if (!(theta > 0) || std::isinf(theta)) return fail(-1, "%s: theta %g", who, theta);
+    if (kind != GSDH_ROPE_PLAIN && (!(factor > 0) || std::isinf(factor))) return fail(-1, "%s: factor %g", who, factor);
+    if (kind == GSDH_ROPE_NTK && rotary_dim == 2) return fail(-1, "%s: one pair has no base to change", who);
+    if (kind == GSDH_ROPE_BY_PARTS && (!(context > 0) || !(high > low)))
+        return fail(-1, "%s: a context of %g positions, turns from %g to %g", who, context, low, high);
+    if (!freqs) return fail(-1, "%s: null buffer", who);
+    if (kind == GSDH_ROPE_NTK) theta *= std::pow(factor, (double)rotary_dim / (rotary_dim - 2));
+    for (int i = 0; i < rotary_dim / 2; i++) {
+        double f = std::pow(theta, -2.0 * i / rotary_dim);
+        if (kind == GSDH_ROPE_LINEAR) f /= factor;
+        if (kind == GSDH_ROPE_BY_PARTS) {
+            const double turns = context * f * 0.15915494309189533577;   // 1 / 2 pi
+            double keep = (turns - low) / (high - low);
+            keep = keep < 0 ? 0 : keep > 1 ? 1 : keep;
+            f = keep * f + (1 - keep) * (f / factor);
+        }
+        freqs[i] = f;
+    }
+    return 0;
+}
+
+int gsdh_rope_rows(void* stream, const gsdh_rope* r, const void* x, int dtype, int64_t x_stride, void* out, int64_t out_stride,
+                   const int* positions, int n, int n_heads, int head_dim) {
+    const char* who = "rope_rows";
+    if (head_dim < 8 || head_dim > 1024 || head_dim % 8) return fail(-1, "%s: head_dim %d is not a multiple of 8 in 8..1024", who, head_dim);
+    const int rc = check_rope(r, head_dim, dtype, who);
+    if (rc) return rc;
+    if (n < 0 || n_heads <= 0 || n_heads > 16384) return fail(-1, "%s: %d tokens of %d heads", who, n, n_heads);
+    if (n == 0) return 0;
+    if (!x || !out || !positions) return fail(-1, "%s: null buffer", who);
+    const int64_t width = (int64_t)n_heads * head_dim;
+    if (!rows_fit(x, x_stride, x == out ? width : 0, dtype) || !rows_fit(out, out_stride, width, dtype))
+        return fail(-1, "%s: rows need 16-byte alignment, strides of whole 16 bytes and at least %lld for out", who, (long long)width);
+    if (x == out && x_stride != out_stride) return fail(-1, "%s: rows turned in place need one stride", who);
+    TurnArgs a{};
+    a.x = x; a.x_stride = x_stride; a.out = out; a.out_stride = out_stride; a.positions = positions;
+    a.n = n; a.heads = n_heads; a.hd = head_dim; a.in_place = x == out;
+    if (!plan_turn(a, *r, false)) return fail(-1, "%s: %d tokens of %d heads in one call", who, n, n_heads);
+    launch_turn_rows<-1>(a, dtype, r->rotary_dim % 8 == 0, static_cast<hipStream_t>(stream));
+    GSD_PAGED_CHK(hipGetLastError(), who);
+    return 0;
+}
+
+int gsdh_paged_rope_append(void* stream, const gsdh_paged_cache* c, int layer, const gsdh_rope* r, int dtype, const void* q, int64_t q_stride,
+                           const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* q_out, int64_t q_out_stride,
+                           const int* seqs, const int* positions, int n, int n_heads) {
+    const char* who = "paged_rope_append";
+    int rc = check_paged_cache(c, who, false);
+    if (rc) return rc;
+    rc = check_rope(r, c->head_dim, dtype, who);
+    if (rc) return rc;
+    if (layer < 0 || layer >= c->n_layers) return fail(-1, "%s: layer %d outside 0..%d", who, layer, c->n_layers - 1);
+    if (n < 0 || n_heads <= 0 || n_heads > 16384) return fail(-1, "%s: %d tokens of %d heads", who, n, n_heads);
+    if (n == 0) return 0;
+    if (!q || !k || !v || !q_out || !seqs || !positions) return fail(-1, "%s: null buffer", who);
+    const int64_t width = (int64_t)n_heads * c->head_dim;
+    if (!rows_fit(q, q_stride, q == q_out ? width : 0, dtype) || !rows_fit(k, k_stride, 0, dtype) || !rows_fit(v, v_stride, 0, dtype) ||
+        !rows_fit(q_out, q_out_stride, width, dtype))
+        return fail(-1, "%s: rows need 16-byte alignment, strides of whole 16 bytes and at least %lld for q_out", who, (long long)width);
+    if (q_out == q && q_out_stride != q_stride) return fail(-1, "%s: q turned in place needs one stride", who);
+    TurnArgs a{};
+    a.c = *c;
+    a.x = q; a.x_stride = q_stride; a.k = k; a.k_stride = k_stride; a.v = v; a.v_stride = v_stride; a.out = q_out; a.out_stride = q_out_stride;
+    a.seqs = seqs; a.positions = positions; a.n = n; a.heads = n_heads; a.nkv = c->n_kv_heads; a.hd = c->head_dim; a.layer = layer;
+    a.in_place = q == q_out;
+    if (!plan_turn(a, *r, true)) return fail(-1, "%s: %d tokens of %d heads in one call", who, n, n_heads);
+    const bool vec = r->rotary_dim % 8 == 0;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    switch (c->dtype) {
+        case GSDH_KV_F16: launch_turn_rows<GSDH_KV_F16>(a, dtype, vec, st); break;
+        case GSDH_KV_BF16: launch_turn_rows<GSDH_KV_BF16>(a, dtype, vec, st); break;
+        default: launch_turn_rows<GSDH_KV_E4M3>(a, dtype, vec, st); break;
+    }
+    GSD_PAGED_CHK(hipGetLastError(), who);
+    return 0;
+}
+
+}  // extern "C"

@@ -16,6 +16,7 @@ _PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.environ.get("GSD_HIP_LIB") or os.path.join(_PKG_DIR, "libgsdhip.so")
 
 vp, i32, i64, u64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_uint64, ctypes.c_float
+f64 = ctypes.c_double
 
 # name -> argtypes (restype int unless noted)
 SIGNATURES = {
@@ -47,12 +48,16 @@ SIGNATURES = {
     "gsdh_paged_attention": [vp, vp, i32, vp, i64, vp, i32, i32, f32, i32, vp, i64, vp, u64],
     "gsdh_paged_chunk_attention": [vp, vp, i32, vp, i32, i64, vp, vp, i32, i32, i32, f32, i32, vp, i64, vp, u64],
     "gsdh_paged_rope_store": [vp, vp, i32] + [vp, i64] * 4 + [vp, vp, i32, i32, vp, i32, i32],
+    "gsdh_rope_frequencies": [i32, f64, i32, f64, f64, f64, f64, vp],
+    "gsdh_rope_rows": [vp, vp, vp, i32, i64, vp, i64, vp, i32, i32, i32],
+    "gsdh_paged_rope_append": [vp, vp, i32, vp, i32] + [vp, i64] * 4 + [vp, vp, i32, i32],
     "gsdh_pages_take": [vp, vp, vp, vp, i32],
     "gsdh_pages_fork": [vp, vp, vp, vp, i32, vp, u64],
     "gsdh_pages_free": [vp, vp, vp, i32],
     "gsdh_pages_compact": [vp, vp, vp, vp, u64],
     "gsdh_pages_copy": [vp, vp, vp, vp, i32, vp, u64],
     "gsdh_token_logprobs": [vp, vp, i32, i64, i32, i32, vp, i32, vp, vp, vp, vp, vp, u64],
+    "gsdh_logits_adjust": [vp, vp, vp, i32, i64, i32, i32, vp, i64],
     "gsdh_model_create": [vp, ctypes.POINTER(vp)],
     "gsdh_model_destroy": [vp],
     "gsdh_model_set_embedding": [vp, vp],
@@ -105,9 +110,24 @@ class GsdPagedCache(ctypes.Structure):
                 ("n_seqs", i32), ("table_width", i32)]
 
 
+class GsdRope(ctypes.Structure):
+    """A rotation (struct gsdh_rope): freqs is a device float64 [rotary_dim / 2],
+    made on the host by gsdh_rope_frequencies or by the caller's model."""
+    _fields_ = [("freqs", vp), ("rotary_dim", i32), ("interleaved", i32), ("scale", f32)]
+
+
+class GsdLogitRules(ctypes.Structure):
+    """What gsdh_logits_adjust does to rows of logits (struct gsdh_logit_rules);
+    what is left at its default is left out."""
+    _fields_ = [("history", vp), ("history_lens", vp), ("prompt_lens", vp), ("repetition", vp), ("frequency", vp),
+                ("presence", vp), ("bias_starts", vp), ("bias_ids", vp), ("bias", vp), ("masks", vp), ("mask_rows", vp),
+                ("history_width", i32), ("n_bias", i32), ("mask_words", i32), ("n_masks", i32)]
+
+
 KV_TYPES = {"f16": 0, "bf16": 1, "e4m3": 2}
 LOGIT_TYPES = {"f32": 0, "f16": 1, "bf16": 2}
 ROW_TYPES = {"f32": 0, "f16": 1, "bf16": 2}
+ROPE_KINDS = {"plain": 0, "linear": 1, "ntk": 2, "by_parts": 3}
 # bits of a paged cache's status word
 PAGES_BAD_INDEX, PAGES_EXHAUSTED, PAGES_SHARED, PAGES_TWICE = 1, 2, 4, 8
 

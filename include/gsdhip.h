@@ -322,6 +322,49 @@ int gsdh_paged_rope_store(void* stream, const gsdh_paged_cache* c, int layer, co
                           const int* positions, int n, int n_heads, const float* angles, int n_angles,
                           int interleaved);
 
+/* Rotary positions from frequencies: pairs of the first rotary_dim dims of a head
+ * are turned by position * freqs[i] radians (formed in 64 bits, so far positions
+ * keep their angles), the dims behind them stay.  interleaved: pairs (2 i, 2 i +
+ * 1), else (i, i + rotary_dim / 2), i < rotary_dim / 2.  scale multiplies cosines and
+ * sines (1; other for models whose attention is stretched with their context). */
+typedef struct gsdh_rope {
+    const double* freqs; /* device [rotary_dim / 2] */
+    int rotary_dim;      /* even, 2 .. head_dim */
+    int interleaved;
+    float scale;
+} gsdh_rope;
+
+/* freqs[i], i < rotary_dim / 2, on the host:
+ *   PLAIN     f_i = theta^(-2 i / rotary_dim)
+ *   LINEAR    f_i / factor
+ *   NTK       with theta * factor^(rotary_dim / (rotary_dim - 2))
+ *   BY_PARTS  f_i where it makes `high` or more turns in `context` positions, f_i /
+ *             factor where it makes `low` or fewer, between them linear in the turns
+ * (arguments that the kind does not name are not looked at). */
+enum { GSDH_ROPE_PLAIN = 0, GSDH_ROPE_LINEAR = 1, GSDH_ROPE_NTK = 2, GSDH_ROPE_BY_PARTS = 3 };
+int gsdh_rope_frequencies(int kind, double theta, int rotary_dim, double factor, double context, double low,
+                          double high, double* freqs);
+
+/* The rotation of gsd_cpu_rope_and_store_kv (gsd_lq_cpu_engine.c:185-262) for n rows
+ * of n_heads x head_dim of `dtype` (GSDH_ROWS_*): out[t * out_stride ..] = x[t *
+ * x_stride ..] turned to position positions[t], evaluated in fp32 and rounded once.
+ * q and K that lie side by side are rows of n_heads + n_kv_heads heads.  out may be x
+ * with the same stride, and must not overlap it otherwise.  A position may be
+ * negative: turning by -p undoes p (up to scale), which is also the gradient.
+ * head_dim: a multiple of 8, up to 1024; rows 16-byte aligned, strides in elements,
+ * of whole 16 bytes, at least n_heads * head_dim for out. */
+int gsdh_rope_rows(void* stream, const gsdh_rope* r, const void* x, int dtype, int64_t x_stride, void* out,
+                   int64_t out_stride, const int* positions, int n, int n_heads, int head_dim);
+
+/* gsdh_paged_rope_store with such a rotation, for rows of `dtype`: q_out gets the
+ * turned q (rounded to dtype), the pages the turned k and v (rounded once to the
+ * cache's type).  No table of angles, so any position below the sequence's length;
+ * what is left out, and when, is as there. */
+int gsdh_paged_rope_append(void* stream, const gsdh_paged_cache* c, int layer, const gsdh_rope* r, int dtype,
+                           const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                           int64_t v_stride, void* q_out, int64_t q_out_stride, const int* seqs,
+                           const int* positions, int n, int n_heads);
+
 /* Pages.  All need c->refs; lists are device int [n], n <= n_seqs.  Free pages
  * are taken lowest index first, in the order of the list, so the same calls
  * give the same tables.  An entry outside the cache is left out
@@ -380,6 +423,41 @@ uint64_t gsdh_token_logprobs_workspace_bytes(int n, int vocab, int top_n);
 int gsdh_token_logprobs(void* stream, const void* logits, int dtype, int64_t row_stride, int n, int vocab,
                         const int* tokens, int top_n, float* logprob, float* entropy, int* top_ids,
                         float* top_logprobs, void* workspace, uint64_t workspace_bytes);
+
+/* What is done to rows of logits before a token is chosen (by gsdh_greedy_argmax,
+ * gsdh_token_logprobs or sample_token, gsd_lq_cpu_runtime.py:422-443).  Each part may
+ * be absent (its pointers NULL); all are device memory, read when the launch runs.
+ *   history [n][history_width]: of row r, the first history_lens[r] entries are the
+ *     tokens so far, the first prompt_lens[r] of them the prompt's (NULL: none).
+ *     repetition[r]: a token that occurs among them has x / r where x > 0, else x * r;
+ *     frequency[r], presence[r]: a token that occurs count > 0 times behind the prompt
+ *     has frequency * count + presence subtracted.  (NULL: that one is left out.)
+ *   bias_ids[e], bias[e], e in bias_starts[r] .. bias_starts[r + 1] - 1 (bias_starts
+ *     [n + 1], within 0 .. n_bias): added to the token; of a token that is listed
+ *     more than once, the last.
+ *   masks [n_masks][mask_words]: bit v % 32 of word v / 32 says whether token v is
+ *     allowed; row r goes by masks[mask_rows[r]], -1: all are.  What is not allowed
+ *     is -inf, whatever it was; a mask may leave nothing.
+ * In this order, in fp32, rounded once.  Tokens outside the vocabulary in the lists
+ * are passed over.  A row becomes NaN whose history_lens lies outside 0 ..
+ * history_width, whose bias_starts fall or leave 0 .. n_bias, or whose mask is none
+ * of -1 .. n_masks - 1. */
+typedef struct gsdh_logit_rules {
+    const int *history, *history_lens, *prompt_lens;
+    const float *repetition, *frequency, *presence; /* [n] */
+    const int *bias_starts, *bias_ids;
+    const float* bias;
+    const uint32_t* masks;
+    const int* mask_rows;
+    int history_width, n_bias, mask_words, n_masks;
+} gsdh_logit_rules;
+
+/* n rows of `vocab` logits at x + r * x_stride (elements of `dtype`, GSDH_LOGITS_*)
+ * to out + r * out_stride; out may be x with the same stride (logits that do not
+ * change are then neither read nor written), and must not overlap it otherwise.
+ * vocab <= 2^24.  No workspace; equal calls give equal bits. */
+int gsdh_logits_adjust(void* stream, const gsdh_logit_rules* r, const void* x, int dtype, int64_t x_stride,
+                       int n, int vocab, void* out, int64_t out_stride);
 
 /* ------------------------------------------------------------------------ */
 /* 2. Model context (replaces GPUMistralV2Model's device side)              */
