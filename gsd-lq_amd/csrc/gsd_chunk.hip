@@ -154,7 +154,7 @@ __device__ __forceinline__ float16v mma(const u32x4v a, const u32x4v b, float16v
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
 }
 
-// eight fp32 values as operands: parts whose sum they are, or (16-bit rows) rounded once
+// eight fp32 values as operands: parts whose sum they are (22 or 24 bits), or (16-bit rows) rounded once
 template <int CT, int NP>
 __device__ __forceinline__ void operands(const float (&x)[8], u32x4v (&w)[NP]) {
     if constexpr (NP == 1 && CT == GSDH_KV_BF16) {
@@ -167,18 +167,23 @@ __device__ __forceinline__ void operands(const float (&x)[8], u32x4v (&w)[NP]) {
 #pragma unroll
         for (int e = 0; e < 8; e++) h[e] = (_Float16)x[e];
         w[0] = __builtin_bit_cast(u32x4v, h);
+    } else if constexpr (NP == 2) {
+        // 11 bits cut off, 11 bits of the rest: two conversions of pairs and a mixed fma per value
+        typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const half2 h = __builtin_bit_cast(half2, __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]));
+            w[0][i] = __builtin_bit_cast(uint32_t, h);
+            w[1][i] = __builtin_bit_cast(uint32_t, half2{(_Float16)__builtin_fmaf((float)h[0], -1.f, x[2 * i]),
+                                                         (_Float16)__builtin_fmaf((float)h[1], -1.f, x[2 * i + 1])});
+        }
     } else {
         const Parts<CT, 8> p = split<CT, 8>(x);
-        static_assert(Parts<CT, 8>::N == NP, "parts of the type");
 #pragma unroll
         for (int i = 0; i < NP; i++) w[i] = p.w[i];
     }
 }
 
-template <typename T>
-__device__ __forceinline__ T rounded(float x) {
-    return (T)x;
-}
 template <typename T>
 __device__ __forceinline__ void store4(T* p, const float (&x)[4]) {
     if constexpr (sizeof(T) == 4) {
@@ -307,13 +312,20 @@ __global__ void __launch_bounds__(kThreads, (blocks_per_cu<HD, Kinds<DT, RT>::NP
         for (int d = 0; d < ND; d++)
 #pragma unroll
             for (int r = 0; r < 16; r++) acc[d][r] = 0.f;
-        float m = -INFINITY, l = 0.f;
+        // The running maximum stays unscaled.  A weight is 2^(x to_log2 + nb), nb the
+        // rounded top_weight - m to_log2: one fma, whose product is exact, so all of a
+        // row's weights are off by the same factor.  Where m to_log2 is beyond 2^20 that
+        // factor would not stay near 1 (or the product overflow): such waves (`steep`)
+        // take 2^((x - m) to_log2 + shift), which weighs the largest 2^top_weight
+        // whatever fp32 rounds off the scaled scores.
+        float m = -INFINITY, l = 0.f, nb = 0.f, shift = 0.f;
+        bool steep = false;
+        constexpr float kSteep = 1048576.f;
 
         // page indices of the tiles from `held` on
-        int held = 0, held_page = 0, held_to = it.t0;
+        int held_page = 0, held_to = it.t0;
         const int batch = max(1, (kPagesHeld - 1) * a.c.page_size / kPos);
         auto hold_pages = [&](int t) {   // all waves have read what was held
-            held = t;
             held_to = t + batch;
             held_page = max(t * kPos, it.first) >> psl;
             const int pg = table[min(held_page + tid, page_last)];
@@ -399,6 +411,67 @@ __global__ void __launch_bounds__(kThreads, (blocks_per_cu<HD, Kinds<DT, RT>::NP
             const unsigned char* const kt = lds + (unsigned)stage * 2 * TILE;
             const unsigned char* const vt = kt + TILE;
             const int p0 = t * kPos;
+            auto v_frag = [&](int s, int d) {
+                typedef short s4 __attribute__((ext_vector_type(4)));
+                typedef __attribute__((address_space(3))) s4 lds_s4;
+                u32x4v f;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const unsigned char* p = vt + v_at + (16 * s + 8 * h) * RB + (v_word ^ (64u * d));
+                    const auto w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(lds_byte*)p);
+                    const uint2 u = __builtin_bit_cast(uint2, w);
+                    f[2 * h] = u.x;
+                    f[2 * h + 1] = u.y;
+                }
+                return f;
+            };
+            // What a row does not see has weight 0, but 0 times an infinity or a NaN is not
+            // 0: where some row does not see all of a tile, such V are looked for, the dims of
+            // the rows that do see them become NaN, and they go into the product as zeros.
+            if (p0 + kPos - 1 > it.pos || (a.window > 0 && p0 <= it.end - 1 - a.window)) {
+                constexpr uint32_t kToTop = CT == GSDH_KV_BF16 ? 0x00800080u : 0x04000400u;   // carries an exponent of ones into the sign
+                auto odd = [&](uint32_t w) { return (((w & 0x7FFF7FFFu) + kToTop) & 0x80008000u) >> 15; };   // 1 per half
+                u32x4v* const mine = reinterpret_cast<u32x4v*>(lds + (unsigned)stage * 2 * TILE + TILE) + tid;
+                constexpr int kWords = TILE / 16 / kThreads;
+                uint32_t any = 0;
+#pragma unroll
+                for (int i = 0; i < kWords; i++) {
+                    const u32x4v w = mine[i * kThreads];
+                    any |= odd(w[0]) | odd(w[1]) | odd(w[2]) | odd(w[3]);
+                }
+                if (__syncthreads_or((int)any)) {
+                    constexpr uint32_t kOne = CT == GSDH_KV_BF16 ? 0x3F80u : 0x3C00u;
+#pragma unroll
+                    for (int d = 0; d < ND; d++) {
+                        float16v count;
+#pragma unroll
+                        for (int r = 0; r < 16; r++) count[r] = 0.f;
+#pragma unroll 1
+                        for (int s = 0; s < 4; s++) {
+                            u32x4v f = v_frag(s, d), see;
+#pragma unroll
+                            for (int w = 0; w < 4; w++) {
+                                f[w] = odd(f[w]) * kOne;
+                                const int p = p0 + 16 * s + 8 * (w / 2) + 4 * hi + 2 * (w % 2);
+                                see[w] = (p <= mypos && p >= mylow ? kOne : 0u) | (p + 1 <= mypos && p + 1 >= mylow ? kOne << 16 : 0u);
+                            }
+                            count = mma<CT>(f, see, count);
+                        }
+#pragma unroll
+                        for (int r = 0; r < 16; r++)
+                            if (count[r] > 0.f) acc[d][r] = __builtin_nanf("");
+                    }
+                    __syncthreads();
+#pragma unroll 1
+                    for (int i = 0; i < kWords; i++) {
+                        u32x4v w = mine[i * kThreads];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) w[e] &= ~(odd(w[e]) * 0xFFFFu);
+                        mine[i * kThreads] = w;
+                    }
+                    __syncthreads();
+                }
+            }
             const bool seen = live && p0 <= phi && (a.window <= 0 || p0 + kPos - 1 >= plo - a.window + 1);
             if (seen) {
                 float16v xs[2];
@@ -414,21 +487,15 @@ __global__ void __launch_bounds__(kThreads, (blocks_per_cu<HD, Kinds<DT, RT>::NP
 #pragma unroll
                         for (int p = NP - 1; p >= 0; p--) xs[n] = mma<CT>(f, q[s][p], xs[n]);
                     }
-                // Scores and their maximum stay unscaled: what the exponential gets is the
-                // difference, so the largest has weight 1 whatever fp32 rounds off the
-                // scaled scores.  What a row does not see is -inf.
+                // what a row does not see is -inf
                 const bool edge = p0 + kPos - 1 > plo || (a.window > 0 && p0 <= phi - a.window);
-                if (edge) {
+                if (edge || lost) {
 #pragma unroll
                     for (int e = 0; e < 32; e++) {
                         const int p = p0 + 32 * (e / 16) + 8 * (e % 16 / 4) + 4 * hi + e % 4;
                         if (p > mypos || p < mylow) xs[e / 16][e % 16] = -INFINITY;
                         else if (lost >> (e / 4) & 1) xs[e / 16][e % 16] = __builtin_nanf("");
                     }
-                } else if (lost) {
-#pragma unroll
-                    for (int e = 0; e < 32; e++)
-                        if (lost >> (e / 4) & 1) xs[e / 16][e % 16] = __builtin_nanf("");
                 }
                 float top = -INFINITY;
 #pragma unroll
@@ -436,93 +503,46 @@ __global__ void __launch_bounds__(kThreads, (blocks_per_cu<HD, Kinds<DT, RT>::NP
                 const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
                 top = fmaxf(m, fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])));
                 if (__any(top > m)) {
-                    const float f = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - top) * to_log2);
+                    const bool was_steep = !(fabsf(m * to_log2) < kSteep), is_steep = !(fabsf(top * to_log2) < kSteep);
+                    const float nb1 = is_steep ? 0.f : fmaf(-top, to_log2, top_weight), shift1 = is_steep ? top_weight : fmaf(top, to_log2, nb1);
+                    // (nothing seen so far: there is nothing to weigh anew)
+                    const float f = m == -INFINITY ? 1.f
+                                  : __builtin_amdgcn_exp2f(was_steep || is_steep ? fmaf(m - top, to_log2, shift1 - shift) : nb1 - nb);
 #pragma unroll
                     for (int d = 0; d < ND; d++) acc[d] *= f;
                     l *= f;
                     m = top;
+                    nb = nb1;
+                    shift = shift1;
+                    steep = __any(is_steep && top != -INFINITY);
                 }
-                const float base = m == -INFINITY ? 0.f : m;
-                u32x4v pw[4][NP];
+                if (steep) {   // weights in place of scores, as exponents
+                    const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-                for (int s = 0; s < 4; s++) {
+                    for (int e = 0; e < 32; e++) xs[e / 16][e % 16] = fmaf(xs[e / 16][e % 16] - base, to_log2, shift);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) xs[e / 16][e % 16] = fmaf(xs[e / 16][e % 16], to_log2, nb);
+                }
+                // of 16 positions
+                auto weights = [&](int s, u32x4v (&pw)[NP]) {
                     float x[8];
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        x[e] = __builtin_amdgcn_exp2f(fmaf(xs[s / 2][8 * (s % 2) + e] - base, to_log2, top_weight));
+                        x[e] = __builtin_amdgcn_exp2f(xs[s / 2][8 * (s % 2) + e]);
                         l += x[e];
                     }
-                    operands<CT, NP>(x, pw[s]);
-                }
-                auto v_frag = [&](int s, int d) {
-                    typedef short s4 __attribute__((ext_vector_type(4)));
-                    typedef __attribute__((address_space(3))) s4 lds_s4;
-                    u32x4v f;
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const unsigned char* p = vt + v_at + (16 * s + 8 * h) * RB + (v_word ^ (64u * d));
-                        const auto w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(lds_byte*)p);
-                        const uint2 u = __builtin_bit_cast(uint2, w);
-                        f[2 * h] = u.x;
-                        f[2 * h + 1] = u.y;
-                    }
-                    return f;
+                    operands<CT, NP>(x, pw);
                 };
-                if (!edge) {
 #pragma unroll
-                    for (int s = 0; s < 4; s++)
+                for (int s = 0; s < 4; s++) {
+                    u32x4v pw[NP];
+                    weights(s, pw);
 #pragma unroll
-                        for (int d = 0; d < ND; d++) {
-                            const u32x4v f = v_frag(s, d);
+                    for (int d = 0; d < ND; d++) {
+                        const u32x4v f = v_frag(s, d);
 #pragma unroll
-                            for (int p = NP - 1; p >= 0; p--) acc[d] = mma<CT>(f, pw[s][p], acc[d]);
-                        }
-                } else {
-                    // What a row does not see has weight 0, but 0 times an infinity or a NaN
-                    // is not 0: such V go in as zeros.
-                    constexpr uint32_t kToTop = CT == GSDH_KV_BF16 ? 0x00800080u : 0x04000400u;   // carries an exponent of ones into the sign
-                    auto odd = [&](uint32_t w) { return (((w & 0x7FFF7FFFu) + kToTop) & 0x80008000u) >> 15; };   // 1 per half
-                    uint32_t any = 0;
-#pragma unroll
-                    for (int s = 0; s < 4; s++)
-#pragma unroll
-                        for (int d = 0; d < ND; d++) {
-                            u32x4v f = v_frag(s, d);
-#pragma unroll
-                            for (int w = 0; w < 4; w++) {
-                                const uint32_t o = odd(f[w]);
-                                any |= o;
-                                f[w] &= ~(o * 0xFFFFu);
-                            }
-#pragma unroll
-                            for (int p = NP - 1; p >= 0; p--) acc[d] = mma<CT>(f, pw[s][p], acc[d]);
-                        }
-                    if (__any(any != 0)) {
-                        // the rows that do see one: the count of them makes the dim NaN
-                        constexpr uint32_t kOne = CT == GSDH_KV_BF16 ? 0x3F80u : 0x3C00u;
-#pragma unroll 1
-                        for (int d = 0; d < ND; d++) {
-                            float16v count;
-#pragma unroll
-                            for (int r = 0; r < 16; r++) count[r] = 0.f;
-#pragma unroll 1
-                            for (int s = 0; s < 4; s++) {
-                                u32x4v f = v_frag(s, d), see;
-#pragma unroll
-                                for (int w = 0; w < 4; w++) {
-                                    f[w] = odd(f[w]) * kOne;
-                                    const int p = p0 + 16 * s + 8 * (w / 2) + 4 * hi + 2 * (w % 2);
-                                    see[w] = (p <= mypos && p >= mylow ? kOne : 0u) | (p + 1 <= mypos && p + 1 >= mylow ? kOne << 16 : 0u);
-                                }
-                                count = mma<CT>(f, see, count);
-                            }
-#pragma unroll
-                            for (int dd = 0; dd < ND; dd++)
-                                if (dd == d)
-#pragma unroll
-                                    for (int r = 0; r < 16; r++)
-                                        if (count[r] > 0.f) acc[dd][r] = __builtin_nanf("");
-                        }
+                        for (int p = NP - 1; p >= 0; p--) acc[d] = mma<CT>(f, pw[p], acc[d]);
                     }
                 }
             }
@@ -531,8 +551,9 @@ __global__ void __launch_bounds__(kThreads, (blocks_per_cu<HD, Kinds<DT, RT>::NP
             lost = lost_next;
         }
 
-        // (scores beyond fp32's range stay finite: a difference of two is a number)
-        if (m != -INFINITY) m = fminf(fmaxf(m * to_log2, -FLT_MAX), FLT_MAX);
+        // what the weights are relative to, as an exponent of 2 (beyond fp32's range it stays
+        // finite: a difference of two is a number)
+        if (m != -INFINITY) m = fabsf(m * to_log2) < kSteep ? -nb : fminf(fmaxf(m * to_log2, -FLT_MAX), FLT_MAX) - top_weight;
         l = swap_add32(l, l, false);
         if (r0 + col < it.rows) {
             if (it.splits == 1) {
