@@ -15,24 +15,33 @@ typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr int kWaves = 4, kThreads = 64 * kWaves;
-constexpr int kRows = 32 * kWaves;   // query rows (token x head of a KV head's group) of a block's step, 32 per wave
+constexpr int kWaveRows = 32;        // query rows (token x head of a KV head's group) of a wave
+constexpr int kMostRows = 256;       // of a block
 constexpr int kPos = 64;             // positions of a tile
 constexpr int kRuns = kPos / 8;      // its runs of eight positions: a page is at least that
-constexpr int kCost = 256;           // what an item's start and end weigh beside its positions
+// What a block does is measured in quarters of the time that a position of up to 32
+// rows takes, whose K and V have to come (a tile of 64 1.2 us); a position of more
+// rows is that often more, by the products of its rows' parts (measured: a tile of
+// 256 rows 2.2 us in 16 bits, 4.2 us in two parts), and an item's start and end, waits
+// under load, are 13 us.
+constexpr int kCost = 2800;
 constexpr int kWhole = 4;            // an item of so few tiles is not cut
-constexpr int kLeastSpan = 256;      // the least a block takes
-static_assert(kCost >= 2 * kPos && kLeastSpan >= kPos, "an item's tiles lie within its cost, and every span inside it has one");
+constexpr int kLeastSpan = 2048;     // the least a block takes
+__device__ __forceinline__ int cost_of_rows(bool few, int rows, int parts) {
+    return few ? (rows <= 32 ? 4 : max(4, 3 * parts)) : rows <= 128 ? 6 * parts : 8 * parts;
+}
+static_assert(kCost >= 2 * kPos * 16 && kLeastSpan >= kPos * 24, "an item's tiles lie within its cost, and every span inside it has one");
 constexpr int kPagesHeld = 256;      // page indices in LDS
-constexpr int kMostGroups = 1024;
-constexpr int kJoinRows = 8;         // rows that a block joins
+constexpr int kMostGroups = 256;     // of blocks, one per KV head
+constexpr int kJoinRows = 8;         // rows that a block joins at a time
+constexpr int kJoinBlocks = 4;       // of an item: four fill the chip once, of 32 most came and went for nothing (8 us)
 
 // ---------------------------------------------------------------------------
 //   x_tp = sm_scale q_t.K_p  (p <= the token's position, and within the window),
 //   out_t = sum_p e^(x_tp - m_t) V_p / sum_p e^(x_tp - m_t)
 //
-// in one pass over K and V with a running maximum m and sum l.  An item is 128
-// query rows of one sequence and KV head (consecutive tokens x the heads of the
+// in one pass over K and V with a running maximum m and sum l.  An item is 128 or
+// 256 query rows of one sequence and KV head (consecutive tokens x the heads of the
 // group); a wave has 32 of them as the columns of S^T = K Q^T and O^T = V^T P^T
 // (32 x 32 x 16 both), over tiles of 64 positions in LDS.  A lane (column l &
 // 31, half j = l >> 5) gets the scores of positions 8 b + 4 j + i (i < 4) of 32
@@ -62,7 +71,9 @@ struct ChunkArgs {
     float* part_ml;
     Joint* joints;   // [group n_kv + head]
     int64_t q_stride, out_stride;
-    int layer, n, n_tokens, group, window, groups, tokens, slot_rows;   // tokens: of an item
+    int layer, n, n_tokens, group, window, groups, slot_rows;
+    int tokens, parts;   // of an item; of a row's 32-bit values
+    bool few;
     float scale;
 };
 
@@ -94,19 +105,25 @@ __device__ __forceinline__ Chunk chunk_of(const ChunkArgs& a, int i) {
     k.base = len - k.m;
     return k;
 }
-// cost of a chunk's items before item u: their positions, and kCost each
+__device__ __forceinline__ int cost_of_position(const ChunkArgs& a, int rows) { return cost_of_rows(a.few, rows, a.parts); }
+// cost of a chunk's items before item u: their positions, by rows, and kCost each
 __device__ __forceinline__ u64 cost_before(const ChunkArgs& a, const Chunk& k, int u) {
     u64 s = (u64)u * kCost;
-    if (k.bad) return s;
-    const u64 n = (u64)u, t = (u64)a.tokens;
-    s += n * (u64)k.base + t * (n * (n + 1) / 2);
-    if (u == k.items) s -= t * n - (u64)k.m;   // (the last item may be shorter)
+    if (k.bad || u == 0) return s;
     const int64_t low = (int64_t)k.base + 1 - a.window;   // first position of the window of token 0
-    if (a.window > 0 && u > 0) {
-        const int64_t from = low > 0 ? 0 : -low / a.tokens + 1;   // the first item whose first position is above 0
-        if (u > from) s -= (u64)((u - from) * low + (int64_t)a.tokens * ((int64_t)u * (u - 1) / 2 - from * (from - 1) / 2));
+    const bool all = u == k.items;
+    if (all) {   // the last item may be shorter
+        const int token = (u - 1) * a.tokens;
+        s += (u64)cost_of_position(a, (k.m - token) * a.group) * (u64)((int64_t)k.base + k.m - (a.window > 0 ? max(low + token, (int64_t)0) : 0));
+        u--;
     }
-    return s;
+    const u64 n = (u64)u, t = (u64)a.tokens;
+    u64 p = n * (u64)k.base + t * (n * (n + 1) / 2);
+    if (a.window > 0) {
+        const int64_t from = low > 0 ? 0 : -low / a.tokens + 1;   // the first item whose first position is above 0
+        if (u > from) p -= (u64)((u - from) * low + (int64_t)a.tokens * ((int64_t)u * (u - 1) / 2 - from * (from - 1) / 2));
+    }
+    return s + p * (u64)cost_of_position(a, a.tokens * a.group);
 }
 
 // sum over the lanes up to this one
@@ -127,6 +144,12 @@ __device__ __forceinline__ u64 readlane64(u64 v, int lane) {
     return (u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)v, lane) |
            (u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(v >> 32), lane) << 32;
 }
+
+// A chunk and where its costs begin, as they wait in LDS (in registers they would stand in the products' way).
+struct Placed {
+    Chunk k;
+    u64 at;
+};
 
 // What a block does of an item.
 struct Item {
@@ -194,6 +217,12 @@ __device__ __forceinline__ void store4(T* p, const float (&x)[4]) {
     }
 }
 
+template <int N>
+__device__ __forceinline__ void loads_but() {   // all but the last N loads (and stores) of the wave are done
+    __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void lds_done() { __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 // DT: the cache's type; RT: the rows' (float, _Float16, __bf16).  The products
 // are in fp16, but bf16 for bf16 caches and rows.
 template <int DT, typename RT>
@@ -202,19 +231,47 @@ struct Kinds {
     static constexpr int CT = DT == GSDH_KV_E4M3 ? (std::is_same<RT, __bf16>::value ? GSDH_KV_BF16 : GSDH_KV_F16) : DT;
     static constexpr int NP = !kWide ? 1 : CT == GSDH_KV_BF16 ? 3 : 2;
 };
-// blocks per CU: registers of a wave that holds the outputs of 32 rows and their q
+// One block per CU.  Two waves per SIMD, one multiplying while the other weighs, as
+// long as the outputs and q of 32 rows fit 256 registers.  (Two blocks of four waves
+// per CU read every tile twice, and the one that came first is served first: it ended
+// a fifth earlier and left the CU half idle.)
 template <int HD, int NP>
-constexpr int blocks_per_cu() {
-    return HD == 256 || (HD == 128 && NP == 3) ? 1 : 2;
+constexpr int waves_of() {
+    return HD == 256 || (HD == 128 && NP == 3) ? 4 : 8;
+}
+// tiles in LDS: one is read, the others are on their way
+template <int HD, int DT>
+constexpr int stages_of() {
+    return DT == GSDH_KV_E4M3 || HD == 256 ? 2 : 4;
 }
 
-template <int HD, int DT, typename RT>
-__global__ void __launch_bounds__(kThreads, (blocks_per_cu<HD, Kinds<DT, RT>::NP>())) chunk_attn_kernel(const ChunkArgs a) {
+template <int HD, int DT, int NW>
+constexpr unsigned tiles_bytes() {
+    const unsigned shared = 2u * stages_of<HD, DT>() * kPos * HD * 2, own = NW * 2u * (kPos / 2) * HD * 2;
+    return shared > own ? shared : own;
+}
+
+// FEW: items of up to 64 rows, whose waves each take positions of their own (32 at a
+// time, of the same rows as the waves `blocks` from it), and whose outputs are
+// joined at the end: as many bytes under way and as much multiplied as with many
+// rows.  Else items of 128 or 256 rows, which all waves read the same tiles for.  A
+// call takes one way for all its chunks, by the mean of their rows: 16 chunks of 20
+// rows over 3400 positions TIME_FEW us and TIME_FEW_WIDE us, a prompt of 4096 tokens (16384 rows) TIME_PROMPT_FEW us and
+// TIME_PROMPT us.  (Both ways in one kernel spilled registers in both loops.)
+template <int HD, int DT, typename RT, bool FEW>
+__global__ void __launch_bounds__((64 * waves_of<HD, Kinds<DT, RT>::NP>()), (waves_of<HD, Kinds<DT, RT>::NP>() / 4))
+chunk_attn_kernel(const ChunkArgs a) {
     constexpr int CT = Kinds<DT, RT>::CT, NP = Kinds<DT, RT>::NP;
     constexpr int ES = DT == GSDH_KV_E4M3 ? 1 : 2, KS = HD / 16, ND = HD / 32;
+    constexpr int NW = waves_of<HD, NP>(), kThreads = 64 * NW, NS = stages_of<HD, DT>(), kAhead = NS - 1;
+    static_assert(kThreads >= kPagesHeld && kRuns % NW == 0, "a thread per page held, whole runs per wave");
     constexpr unsigned RB = HD * 2, TILE = kPos * RB;   // a row and a tile of 16-bit values in LDS
-    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];   // K, V of a tile, twice; then the pages
-    int* const pages = reinterpret_cast<int*>(lds + 4 * TILE);
+    constexpr unsigned BUF = tiles_bytes<HD, DT, NW>();
+    // K, V of NS tiles, or of half a tile for each wave, or the waves' outputs; the pages; the waves' (m, l)
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    int* const pages = reinterpret_cast<int*>(lds + BUF);
+    float2* const wave_ml = reinterpret_cast<float2*>(lds + BUF + kPagesHeld * 4);   // [NW][32]
+    Placed* const placed = reinterpret_cast<Placed*>(lds + BUF + kPagesHeld * 4 + NW * kWaveRows * 8);   // [64]
     const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_byte*)lds;
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, hi = lane >> 5;
     const int G = a.group, nkv = a.c.n_kv_heads, head = (int)(blockIdx.x % (unsigned)nkv), grp = (int)(blockIdx.x / (unsigned)nkv);
@@ -238,51 +295,39 @@ __global__ void __launch_bounds__(kThreads, (blocks_per_cu<HD, Kinds<DT, RT>::NP
     // -- one item's part ----------------------------------------------------
     auto run_item = [&](const Item& it) {
         const int tokens_hi = (it.rows - 1) / G;
-        if (it.bad) {
-            if (tid == 0 && head == 0) page_status(a.c, GSDH_PAGES_BAD_INDEX);
-            for (int i = tid; i < it.rows * (HD / 4); i += kThreads) {
-                const int r = i / (HD / 4), d = i % (HD / 4) * 4;
-                const float nan = __builtin_nanf("");
-                const float x[4] = {nan, nan, nan, nan};
-                store4(static_cast<RT*>(a.out) + (int64_t)(it.token + r / G) * a.out_stride + ((int64_t)head * G + r % G) * HD + d, x);
-            }
-            return;
-        }
         // the wave's rows, and what they see
-        const int r0 = 32 * wid, row = min(r0 + col, it.rows - 1), tok = row / G, qh = head * G + row % G;
+        const int blocks = !FEW ? NW : it.rows <= kWaveRows ? 1 : 2;   // of 32 rows
+        const int r0 = kWaveRows * (FEW ? wid & (blocks - 1) : wid), row = min(r0 + col, it.rows - 1), tok = row / G, qh = head * G + row % G;
         const bool live = r0 < it.rows;
         const int mypos = it.pos + tok, mylow = a.window > 0 ? mypos - a.window + 1 : 0;
-        const int plo = it.pos + min(r0, it.rows - 1) / G, phi = it.pos + min((r0 + 31) / G, tokens_hi);
+        const int plo = it.pos + min(r0, it.rows - 1) / G, phi = it.pos + min((r0 + kWaveRows - 1) / G, tokens_hi);
         const int* const table = a.c.tables + (size_t)(unsigned)it.seq * a.c.table_width;
         const int page_last = (it.end - 1) >> psl;
 
         // q's operand
         u32x4v q[KS][NP];
         float to_log2 = 1.f;
+        typedef RT r8 __attribute__((ext_vector_type(8)));
+        r8 qrow[KS];   // as it comes: asked for before the pages are, used once the first tiles are asked for
         if (live) {
             const RT* src = static_cast<const RT*>(a.q) + (int64_t)(it.token + tok) * a.q_stride + (int64_t)qh * HD + 8 * hi;
+#pragma unroll
+            for (int s = 0; s < KS; s++) qrow[s] = *reinterpret_cast<const r8*>(src + 16 * s);
+        }
+        auto form_q = [&] {
+            if (!live) return;
             const float scale = a.scale * kLog2e * kscale;
             if constexpr (NP == 1 && CT == GSDH_KV_F16) {
                 const uint32_t flip = scale < 0.f || (scale == 0.f && __builtin_signbit(scale)) ? 0x80008000u : 0u;
 #pragma unroll
-                for (int s = 0; s < KS; s++) q[s][0] = *reinterpret_cast<const u32x4v*>(src + 16 * s) ^ flip;
+                for (int s = 0; s < KS; s++) q[s][0] = __builtin_bit_cast(u32x4v, qrow[s]) ^ flip;
                 to_log2 = fabsf(scale);
             } else {
-                float x[KS][8], most = 0.f;
+                float most = 0.f;
 #pragma unroll
-                for (int s = 0; s < KS; s++) {
-                    if constexpr (sizeof(RT) == 4) {
-                        const float4 u = *reinterpret_cast<const float4*>(src + 16 * s), w = *reinterpret_cast<const float4*>(src + 16 * s + 4);
-                        x[s][0] = u.x; x[s][1] = u.y; x[s][2] = u.z; x[s][3] = u.w;
-                        x[s][4] = w.x; x[s][5] = w.y; x[s][6] = w.z; x[s][7] = w.w;
-                    } else {
-                        const bf8 u = *reinterpret_cast<const bf8*>(src + 16 * s);
+                for (int s = 0; s < KS; s++)
 #pragma unroll
-                        for (int e = 0; e < 8; e++) x[s][e] = (float)u[e];
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(x[s][e]));
-                }
+                    for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf((float)qrow[s][e]));
                 const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
                 most = fmaxf(__uint_as_float(other[0]), __uint_as_float(other[1]));
                 // by a power of two: fp16 parts keep their bits below 1024, bf16 ones stay
@@ -294,14 +339,15 @@ __global__ void __launch_bounds__(kThreads, (blocks_per_cu<HD, Kinds<DT, RT>::NP
                 to_log2 = fabsf(scale) * down;
 #pragma unroll
                 for (int s = 0; s < KS; s++) {
+                    float x[8];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) x[s][e] *= up;
-                    operands<CT, NP>(x[s], q[s]);
+                    for (int e = 0; e < 8; e++) x[e] = (float)qrow[s][e] * up;
+                    operands<CT, NP>(x, q[s]);
                 }
             }
             // (a scale of 0 stays above it: a masked -inf times it is -inf)
             to_log2 = fmaxf(to_log2, FLT_TRUE_MIN);
-        }
+        };
         // P as 2^14 times itself: what lies below fp16's normal range stays exact longer;
         // bf16: over a power of two that is above the number of positions, so that no
         // sum of finite V passes fp32's range
@@ -328,237 +374,353 @@ __global__ void __launch_bounds__(kThreads, (blocks_per_cu<HD, Kinds<DT, RT>::NP
         auto hold_pages = [&](int t) {   // all waves have read what was held
             held_to = t + batch;
             held_page = max(t * kPos, it.first) >> psl;
-            const int pg = table[min(held_page + tid, page_last)];
-            pages[tid] = (unsigned)pg < (unsigned)a.c.n_pages ? pg : -1;
+            const int pg = table[min(held_page + min(tid, kPagesHeld - 1), page_last)];
+            if (tid < kPagesHeld) pages[tid] = (unsigned)pg < (unsigned)a.c.n_pages ? pg : -1;
             __syncthreads();
         };
-        // the page of a run of a tile (runs that no row sees: the nearest page), per lane
-        auto page_of = [&](int t, int run) {
-            const int p = min(max((t * kPos + 8 * run) >> psl, held_page), page_last);
-            return pages[p - held_page];
+        // the page of a run of eight positions (one that no row sees: the nearest page), per lane
+        auto page_of = [&](int pos) { return pages[min(max(pos >> psl, held_page), page_last) - held_page]; };
+        // (a lane number that the compiler cannot trace: addresses are formed for each item,
+        // not kept beside the choice of items)
+        int ln = lane;
+        __asm__ volatile("" : "+v"(ln));
+        const int v_row = 4 * (ln >> 5) + (ln & 15) / 4;
+        const unsigned k_at = (unsigned)(ln & 31) * RB, k_word = 16u * (unsigned)((ln >> 5) ^ swz_k(ln & 31)), v_at = (unsigned)v_row * RB;
+        const unsigned v_word = 16u * (unsigned)((2 * (ln >> 4 & 1) + ((ln & 3) >> 1)) ^ swz_v(v_row)) + 8u * (ln & 1);
+        // V's operand: positions 16 s + 8 h + 4 hi + 0 .. 3 of dim 32 d + col
+        auto v_frag = [&](const unsigned char* vt, int s, int d) {
+            typedef short s4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s4 lds_s4;
+            u32x4v f;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const unsigned char* p = vt + v_at + (16 * s + 8 * h) * RB + (v_word ^ (64u * d));
+                const auto w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(lds_byte*)p);
+                const uint2 u = __builtin_bit_cast(uint2, w);
+                f[2 * h] = u.x;
+                f[2 * h + 1] = u.y;
+            }
+            return f;
         };
-        unsigned lost = 0, lost_next = 0;   // runs of a tile whose page lies outside the pool
-        uint4 raw[DT == GSDH_KV_E4M3 ? 2 * HD / 64 : 1];   // e4m3: the next tile's bytes on their way to LDS
-        // K and V of tile t: 16-bit rows straight into LDS, a wave two runs of each
-        auto load_tile = [&](int t, int stage) {
-            const int pg = page_of(t, lane & (kRuns - 1));
-            lost_next = (unsigned)__ballot(pg < 0) & (unsigned)((1 << kRuns) - 1);
-            if constexpr (DT != GSDH_KV_E4M3) {
-                constexpr int RPI = 1024 / RB, IPR = 8 / RPI, WPR = RB / 16;   // rows of a load, loads of a run, words of a row
+        // What a row does not see has weight 0, but 0 times an infinity or a NaN is not 0:
+        // where some row does not see all of N x 32 positions, such V are looked for (thread
+        // `who` of T, which `any_of` and `meet` bring together), the dims of the rows that do
+        // see them become NaN, and they go into the product as zeros.
+        auto odd_values = [&](auto halves, auto threads, int p0, unsigned char* vt, int who, auto any_of, auto meet) {
+            constexpr int N = decltype(halves)::value, T = decltype(threads)::value, kWords = N * 32 * RB / 16 / T;
+            constexpr uint32_t kToTop = CT == GSDH_KV_BF16 ? 0x00800080u : 0x04000400u;   // carries an exponent of ones into the sign
+            auto odd = [&](uint32_t w) { return (((w & 0x7FFF7FFFu) + kToTop) & 0x80008000u) >> 15; };   // 1 per half
+            u32x4v* const mine = reinterpret_cast<u32x4v*>(vt) + who;
+            uint32_t any = 0;
 #pragma unroll
-                for (int rr = 0; rr < 2; rr++) {
-                    const int run = 2 * wid + rr, page = max(__builtin_amdgcn_readlane(pg, run), 0);
-                    const size_t at = (size_t)page * page_b + (unsigned)((t * kPos + 8 * run) & psm) * row_b;
+            for (int i = 0; i < kWords; i++) {
+                const u32x4v w = mine[i * T];
+                any |= odd(w[0]) | odd(w[1]) | odd(w[2]) | odd(w[3]);
+            }
+            if (!any_of(any)) return;
+            constexpr uint32_t kOne = CT == GSDH_KV_BF16 ? 0x3F80u : 0x3C00u;
 #pragma unroll
-                    for (int k = 0; k < IPR; k++) {
-                        const int r = k * RPI + lane / WPR, word = lane % WPR;   // of the run
-                        const uint32_t to = lds_at + (unsigned)stage * 2 * TILE + (unsigned)(run * 8 + k * RPI) * RB;
-                        lds_dma16(kb + at, (unsigned)r * row_b + 16u * (unsigned)(word ^ swz_k(8 * rr + r)), to);
-                        lds_dma16(vb + at, (unsigned)r * row_b + 16u * (unsigned)(word ^ swz_v(8 * rr + r)), to + TILE);
+            for (int d = 0; d < ND; d++) {
+                float16v count;
+#pragma unroll
+                for (int r = 0; r < 16; r++) count[r] = 0.f;
+#pragma unroll 1
+                for (int s = 0; s < 2 * N; s++) {
+                    u32x4v f = v_frag(vt, s, d), see;
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        f[w] = odd(f[w]) * kOne;
+                        const int p = p0 + 16 * s + 8 * (w / 2) + 4 * hi + 2 * (w % 2);
+                        see[w] = (p <= mypos && p >= mylow ? kOne : 0u) | (p + 1 <= mypos && p + 1 >= mylow ? kOne << 16 : 0u);
                     }
+                    count = mma<CT>(f, see, count);
                 }
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (count[r] > 0.f) acc[d][r] = __builtin_nanf("");
+            }
+            meet();
+#pragma unroll 1
+            for (int i = 0; i < kWords; i++) {
+                u32x4v w = mine[i * T];
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] &= ~(odd(w[e]) * 0xFFFFu);
+                mine[i * T] = w;
+            }
+            meet();
+        };
+        // The wave's rows and N x 32 positions from p0 on; gone: runs whose page lies outside the pool.
+        auto step = [&](auto halves, int p0, const unsigned char* kt, const unsigned char* vt, unsigned gone, auto scored, auto weighed) {
+            constexpr int N = decltype(halves)::value;
+            float16v xs[N];
+#pragma unroll
+            for (int n = 0; n < N; n++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) xs[n][r] = 0.f;
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int n = 0; n < N; n++) {
+                    const u32x4v f = *reinterpret_cast<const u32x4v*>(kt + k_at + 32 * n * RB + (k_word ^ (32u * s)));
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; p--) xs[n] = mma<CT>(f, q[s][p], xs[n]);
+                }
+            scored();
+            // what a row does not see is -inf
+            if (gone || p0 + 32 * N - 1 > plo || (a.window > 0 && p0 <= phi - a.window)) {
+#pragma unroll
+                for (int e = 0; e < 16 * N; e++) {
+                    const int p = p0 + 32 * (e / 16) + 8 * (e % 16 / 4) + 4 * hi + e % 4;
+                    if (p > mypos || p < mylow) xs[e / 16][e % 16] = -INFINITY;
+                    else if (gone >> (e / 4) & 1) xs[e / 16][e % 16] = __builtin_nanf("");
+                }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 16 * N; e++) top = fmaxf(top, xs[e / 16][e % 16]);
+            const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            top = fmaxf(m, fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])));
+            if (__any(top > m)) {
+                const bool was_steep = !(fabsf(m * to_log2) < kSteep), is_steep = !(fabsf(top * to_log2) < kSteep);
+                const float nb1 = is_steep ? 0.f : fmaf(-top, to_log2, top_weight), shift1 = is_steep ? top_weight : fmaf(top, to_log2, nb1);
+                // (nothing seen so far: there is nothing to weigh anew)
+                const float f = m == -INFINITY ? 1.f
+                              : __builtin_amdgcn_exp2f(was_steep || is_steep ? fmaf(m - top, to_log2, shift1 - shift) : nb1 - nb);
+#pragma unroll
+                for (int d = 0; d < ND; d++) acc[d] *= f;
+                l *= f;
+                m = top;
+                nb = nb1;
+                shift = shift1;
+                steep = __any(is_steep && top != -INFINITY);
+            }
+            if (steep) {   // the weights' exponents in place of the scores
+                const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                for (int e = 0; e < 16 * N; e++) xs[e / 16][e % 16] = fmaf(xs[e / 16][e % 16] - base, to_log2, shift);
             } else {
-                // a lane: 16 bytes of a row; a load of the wave: 1024 / HD rows, in one run
-                constexpr int RPL = 1024 / HD, LPT = kPos / RPL / kWaves;   // loads of a wave and tile
 #pragma unroll
-                for (int k = 0; k < LPT; k++) {
-                    const int r = (k * kWaves + wid) * RPL + lane / (HD / 16), run = r / 8;
-                    const int page = max(__shfl(pg, run, 64), 0);
-                    const size_t at = (size_t)page * page_b + (unsigned)((t * kPos + r) & psm) * row_b + 16u * (unsigned)(lane % (HD / 16));
-                    raw[2 * k] = *reinterpret_cast<const uint4*>(kb + at);
-                    raw[2 * k + 1] = *reinterpret_cast<const uint4*>(vb + at);
+                for (int e = 0; e < 16 * N; e++) xs[e / 16][e % 16] = fmaf(xs[e / 16][e % 16], to_log2, nb);
+            }
+            weighed();
+#pragma unroll
+            for (int s = 0; s < 2 * N; s++) {
+                float x[8];
+                u32x4v pw[NP];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    x[e] = __builtin_amdgcn_exp2f(xs[s / 2][8 * (s % 2) + e]);
+                    l += x[e];
+                }
+                operands<CT, NP>(x, pw);
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    const u32x4v f = v_frag(vt, s, d);
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; p--) acc[d] = mma<CT>(f, pw[p], acc[d]);
                 }
             }
         };
-        auto convert_tile = [&](int stage) {   // e4m3: the bytes as 16-bit values
-            if constexpr (DT == GSDH_KV_E4M3) {
-                constexpr int RPL = 1024 / HD, LPT = kPos / RPL / kWaves;
+        // some row of the block, or (the wave's own positions) of the wave, does not see all of them
+        auto masked = [&](int p0, int n, int low, int high) { return p0 + n - 1 > low || (a.window > 0 && p0 <= high - a.window); };
+        using One = std::integral_constant<int, 1>;
+        using Two = std::integral_constant<int, 2>;
+
+        // A row of K or V as it comes to LDS: 16-bit ones by loads past the registers, of
+        // RPI rows each; e4m3 through `raw`, RPL rows per load of the wave.
+        constexpr int RPI = 1024 / RB, IPR = 8 / RPI, WPR = RB / 16, RPL = 1024 / HD;
+        auto load_run = [&](const unsigned char* base, int page, int p, uint32_t to, auto swz, int row_in_tile) {
+            const unsigned char* const from = base + ((size_t)max(page, 0) * page_b + (unsigned)(p & psm) * row_b);
 #pragma unroll
-                for (int k = 0; k < LPT; k++) {
-                    const int r = (k * kWaves + wid) * RPL + lane / (HD / 16), word = 2 * (lane % (HD / 16));
-#pragma unroll
-                    for (int w = 0; w < 2; w++) {
-                        const uint4 b = raw[2 * k + w];
-                        unsigned char* to = lds + (unsigned)stage * 2 * TILE + w * TILE + (unsigned)r * RB;
-                        const int sw = w ? swz_v(r) : swz_k(r);
-                        *reinterpret_cast<uint4*>(to + 16 * (word ^ sw)) =
-                            make_uint4(e4m3_pair<CT, false>(b.x), e4m3_pair<CT, true>(b.x), e4m3_pair<CT, false>(b.y), e4m3_pair<CT, true>(b.y));
-                        *reinterpret_cast<uint4*>(to + 16 * ((word + 1) ^ sw)) =
-                            make_uint4(e4m3_pair<CT, false>(b.z), e4m3_pair<CT, true>(b.z), e4m3_pair<CT, false>(b.w), e4m3_pair<CT, true>(b.w));
-                    }
-                }
+            for (int k = 0; k < IPR; k++) {
+                const int r = k * RPI + ln / WPR, word = ln % WPR;   // of the run
+                lds_dma16(from, (unsigned)r * row_b + 16u * (unsigned)(word ^ swz(row_in_tile + r)), to + (unsigned)(row_in_tile + k * RPI) * RB);
             }
+        };
+        auto load_raw = [&](const unsigned char* base, int page, int p) {   // this lane's 16 bytes of position p
+            return *reinterpret_cast<const uint4*>(base + ((size_t)max(page, 0) * page_b + (unsigned)(p & psm) * row_b + 16u * (unsigned)(ln % (HD / 16))));
+        };
+        auto convert = [&](const uint4 b, unsigned char* tile, int r, int sw) {
+            unsigned char* const to = tile + (unsigned)r * RB;
+            const int word = 2 * (ln % (HD / 16));
+            *reinterpret_cast<uint4*>(to + 16 * (word ^ sw)) =
+                make_uint4(e4m3_pair<CT, false>(b.x), e4m3_pair<CT, true>(b.x), e4m3_pair<CT, false>(b.y), e4m3_pair<CT, true>(b.y));
+            *reinterpret_cast<uint4*>(to + 16 * ((word + 1) ^ sw)) =
+                make_uint4(e4m3_pair<CT, false>(b.z), e4m3_pair<CT, true>(b.z), e4m3_pair<CT, false>(b.w), e4m3_pair<CT, true>(b.w));
         };
 
         __syncthreads();   // (the last item's tiles and pages are read)
-        hold_pages(it.t0);
-        load_tile(it.t0, 0);
-        convert_tile(0);
-        lost = lost_next;
-        const unsigned k_at = (unsigned)col * RB, k_word = 16u * (unsigned)(hi ^ swz_k(col));
-        const unsigned v_row = (unsigned)(4 * hi + (lane & 15) / 4);
-        const unsigned v_at = v_row * RB, v_word = (16u * (unsigned)((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ swz_v((int)v_row))) + 8u * (lane & 1);
-        for (int t = it.t0; t < it.t1; t++) {
-            const int stage = (t - it.t0) & 1;
-            // tile t is in LDS, and nobody reads tile t - 1 any more
-            __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            const bool more = t + 1 < it.t1;
-            if (more) {
-                if (t + 1 == held_to) hold_pages(t + 1);
-                load_tile(t + 1, stage ^ 1);
-            }
-            const unsigned char* const kt = lds + (unsigned)stage * 2 * TILE;
-            const unsigned char* const vt = kt + TILE;
-            const int p0 = t * kPos;
-            auto v_frag = [&](int s, int d) {
-                typedef short s4 __attribute__((ext_vector_type(4)));
-                typedef __attribute__((address_space(3))) s4 lds_s4;
-                u32x4v f;
+        if constexpr (!FEW) {
+            u64 lost = 0;   // runs whose page lies outside the pool: a byte for the tile at hand and each ahead
+            constexpr int LPT = 2 * kPos / RPL / NW;   // loads of a wave and tile (e4m3): K's, then V's
+            uint4 raw[DT == GSDH_KV_E4M3 ? LPT : 1];
+            auto load_tile = [&](int t, int stage, int ahead) {
+                const int pg = page_of(t * kPos + 8 * (lane & (kRuns - 1)));
+                lost |= (u64)((unsigned)__ballot(pg < 0) & (unsigned)((1 << kRuns) - 1)) << 8 * ahead;
+                if constexpr (DT != GSDH_KV_E4M3) {
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const unsigned char* p = vt + v_at + (16 * s + 8 * h) * RB + (v_word ^ (64u * d));
-                    const auto w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(lds_byte*)p);
-                    const uint2 u = __builtin_bit_cast(uint2, w);
-                    f[2 * h] = u.x;
-                    f[2 * h + 1] = u.y;
-                }
-                return f;
-            };
-            // What a row does not see has weight 0, but 0 times an infinity or a NaN is not
-            // 0: where some row does not see all of a tile, such V are looked for, the dims of
-            // the rows that do see them become NaN, and they go into the product as zeros.
-            if (p0 + kPos - 1 > it.pos || (a.window > 0 && p0 <= it.end - 1 - a.window)) {
-                constexpr uint32_t kToTop = CT == GSDH_KV_BF16 ? 0x00800080u : 0x04000400u;   // carries an exponent of ones into the sign
-                auto odd = [&](uint32_t w) { return (((w & 0x7FFF7FFFu) + kToTop) & 0x80008000u) >> 15; };   // 1 per half
-                u32x4v* const mine = reinterpret_cast<u32x4v*>(lds + (unsigned)stage * 2 * TILE + TILE) + tid;
-                constexpr int kWords = TILE / 16 / kThreads;
-                uint32_t any = 0;
-#pragma unroll
-                for (int i = 0; i < kWords; i++) {
-                    const u32x4v w = mine[i * kThreads];
-                    any |= odd(w[0]) | odd(w[1]) | odd(w[2]) | odd(w[3]);
-                }
-                if (__syncthreads_or((int)any)) {
-                    constexpr uint32_t kOne = CT == GSDH_KV_BF16 ? 0x3F80u : 0x3C00u;
-#pragma unroll
-                    for (int d = 0; d < ND; d++) {
-                        float16v count;
-#pragma unroll
-                        for (int r = 0; r < 16; r++) count[r] = 0.f;
-#pragma unroll 1
-                        for (int s = 0; s < 4; s++) {
-                            u32x4v f = v_frag(s, d), see;
-#pragma unroll
-                            for (int w = 0; w < 4; w++) {
-                                f[w] = odd(f[w]) * kOne;
-                                const int p = p0 + 16 * s + 8 * (w / 2) + 4 * hi + 2 * (w % 2);
-                                see[w] = (p <= mypos && p >= mylow ? kOne : 0u) | (p + 1 <= mypos && p + 1 >= mylow ? kOne << 16 : 0u);
-                            }
-                            count = mma<CT>(f, see, count);
-                        }
-#pragma unroll
-                        for (int r = 0; r < 16; r++)
-                            if (count[r] > 0.f) acc[d][r] = __builtin_nanf("");
+                    for (int rr = 0; rr < kRuns / NW; rr++) {
+                        const int run = kRuns / NW * wid + rr, page = __builtin_amdgcn_readlane(pg, run);
+                        const uint32_t to = lds_at + (unsigned)stage * 2 * TILE;
+                        load_run(kb, page, t * kPos + 8 * run, to, swz_k, 8 * run);
+                        load_run(vb, page, t * kPos + 8 * run, to + TILE, swz_v, 8 * run);
                     }
-                    __syncthreads();
-#pragma unroll 1
-                    for (int i = 0; i < kWords; i++) {
-                        u32x4v w = mine[i * kThreads];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) w[e] &= ~(odd(w[e]) * 0xFFFFu);
-                        mine[i * kThreads] = w;
-                    }
-                    __syncthreads();
-                }
-            }
-            const bool seen = live && p0 <= phi && (a.window <= 0 || p0 + kPos - 1 >= plo - a.window + 1);
-            if (seen) {
-                float16v xs[2];
-#pragma unroll
-                for (int n = 0; n < 2; n++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) xs[n][r] = 0.f;
-#pragma unroll
-                for (int s = 0; s < KS; s++)
-#pragma unroll
-                    for (int n = 0; n < 2; n++) {
-                        const u32x4v f = *reinterpret_cast<const u32x4v*>(kt + k_at + 32 * n * RB + (k_word ^ (32u * s)));
-#pragma unroll
-                        for (int p = NP - 1; p >= 0; p--) xs[n] = mma<CT>(f, q[s][p], xs[n]);
-                    }
-                // what a row does not see is -inf
-                const bool edge = p0 + kPos - 1 > plo || (a.window > 0 && p0 <= phi - a.window);
-                if (edge || lost) {
-#pragma unroll
-                    for (int e = 0; e < 32; e++) {
-                        const int p = p0 + 32 * (e / 16) + 8 * (e % 16 / 4) + 4 * hi + e % 4;
-                        if (p > mypos || p < mylow) xs[e / 16][e % 16] = -INFINITY;
-                        else if (lost >> (e / 4) & 1) xs[e / 16][e % 16] = __builtin_nanf("");
-                    }
-                }
-                float top = -INFINITY;
-#pragma unroll
-                for (int e = 0; e < 32; e++) top = fmaxf(top, xs[e / 16][e % 16]);
-                const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-                top = fmaxf(m, fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])));
-                if (__any(top > m)) {
-                    const bool was_steep = !(fabsf(m * to_log2) < kSteep), is_steep = !(fabsf(top * to_log2) < kSteep);
-                    const float nb1 = is_steep ? 0.f : fmaf(-top, to_log2, top_weight), shift1 = is_steep ? top_weight : fmaf(top, to_log2, nb1);
-                    // (nothing seen so far: there is nothing to weigh anew)
-                    const float f = m == -INFINITY ? 1.f
-                                  : __builtin_amdgcn_exp2f(was_steep || is_steep ? fmaf(m - top, to_log2, shift1 - shift) : nb1 - nb);
-#pragma unroll
-                    for (int d = 0; d < ND; d++) acc[d] *= f;
-                    l *= f;
-                    m = top;
-                    nb = nb1;
-                    shift = shift1;
-                    steep = __any(is_steep && top != -INFINITY);
-                }
-                if (steep) {   // weights in place of scores, as exponents
-                    const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-                    for (int e = 0; e < 32; e++) xs[e / 16][e % 16] = fmaf(xs[e / 16][e % 16] - base, to_log2, shift);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 32; e++) xs[e / 16][e % 16] = fmaf(xs[e / 16][e % 16], to_log2, nb);
-                }
-                // of 16 positions
-                auto weights = [&](int s, u32x4v (&pw)[NP]) {
-                    float x[8];
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        x[e] = __builtin_amdgcn_exp2f(xs[s / 2][8 * (s % 2) + e]);
-                        l += x[e];
-                    }
-                    operands<CT, NP>(x, pw);
-                };
-#pragma unroll
-                for (int s = 0; s < 4; s++) {
-                    u32x4v pw[NP];
-                    weights(s, pw);
-#pragma unroll
-                    for (int d = 0; d < ND; d++) {
-                        const u32x4v f = v_frag(s, d);
-#pragma unroll
-                        for (int p = NP - 1; p >= 0; p--) acc[d] = mma<CT>(f, pw[p], acc[d]);
+                    for (int k = 0; k < LPT; k++) {
+                        const int load = wid * LPT + k, r = load % (kPos / RPL) * RPL + ln / (HD / 16);
+                        raw[k] = load_raw(load < kPos / RPL ? kb : vb, __shfl(pg, r / 8, 64), t * kPos + r);
                     }
                 }
+            };
+            auto convert_tile = [&](int stage) {
+                if constexpr (DT == GSDH_KV_E4M3) {
+#pragma unroll
+                    for (int k = 0; k < LPT; k++) {
+                        const int load = wid * LPT + k, r = load % (kPos / RPL) * RPL + ln / (HD / 16);
+                        const bool of_v = load >= kPos / RPL;
+                        convert(raw[k], lds + (unsigned)stage * 2 * TILE + (of_v ? TILE : 0u), r, of_v ? swz_v(r) : swz_k(r));
+                    }
+                }
+            };
+            hold_pages(it.t0);
+#pragma unroll
+            for (int i = 0; i < kAhead; i++)
+                if (it.t0 + i < it.t1) load_tile(it.t0 + i, i, i);
+            form_q();   // (while the first tiles are on their way)
+            convert_tile(0);
+            for (int t = it.t0; t < it.t1; t++) {
+                const int stage = (t - it.t0) % NS;
+                // tile t is in LDS, the loads of those behind it may be under way; and nobody
+                // reads tile t - 1 any more, whose place the tile kAhead behind t takes
+                constexpr int kLoads = DT == GSDH_KV_E4M3 ? 0 : 2 * (int)TILE / 1024 / NW;   // of a wave and tile
+                if (kAhead >= 3 && t + 2 < it.t1) loads_but<kAhead >= 3 ? 2 * kLoads : 0>();
+                else if (kAhead >= 2 && t + 1 < it.t1) loads_but<kAhead >= 2 ? kLoads : 0>();
+                else loads_but<0>();
+                lds_barrier();
+                const bool more = t + kAhead < it.t1;
+                if (more) {
+                    if (t + kAhead == held_to) hold_pages(t + kAhead);
+                    load_tile(t + kAhead, (stage + kAhead) % NS, kAhead);
+                }
+                unsigned char* const kt = lds + (unsigned)stage * 2 * TILE;
+                const int p0 = t * kPos;
+                const unsigned gone = (unsigned)lost & 0xFFu;
+                if (masked(p0, kPos, it.pos, it.end - 1))
+                    odd_values(Two{}, std::integral_constant<int, kThreads>{}, p0, kt + TILE, tid, [](uint32_t any) { return __syncthreads_or((int)any); },
+                               [] { __syncthreads(); });
+                if (live && p0 <= phi && (a.window <= 0 || p0 + kPos - 1 >= plo - a.window + 1))
+                    step(Two{}, p0, kt, kt + TILE, gone, [] {}, [] {});
+                if (more) convert_tile((stage + kAhead) % NS);
+                if (gone && tid == 0 && head == 0) page_status(a.c, GSDH_PAGES_BAD_INDEX);
+                lost >>= 8;
             }
-            if (more) convert_tile(stage ^ 1);
-            if (lost && tid == 0 && head == 0) page_status(a.c, GSDH_PAGES_BAD_INDEX);
-            lost = lost_next;
+        } else {
+            constexpr unsigned HALF = TILE / 2;
+            constexpr int kLoads = (int)HALF / 1024, LPH = kPos / 2 / RPL;   // of K or of V
+            unsigned char* const kt = lds + (unsigned)wid * 2 * HALF;
+            const uint32_t to = lds_at + (unsigned)wid * 2 * HALF;
+            const int every = NW / blocks;
+            uint4 raw[DT == GSDH_KV_E4M3 ? 2 * LPH : 1];
+            int pg = 0;   // pages of a half's runs (lane & 3)
+            auto pages_for = [&](int h) { pg = page_of(32 * h + 8 * (ln & 3)); };
+            auto load_half = [&](int h, const unsigned char* base, uint32_t at, auto swz) {
+#pragma unroll
+                for (int run = 0; run < 4; run++) load_run(base, __builtin_amdgcn_readlane(pg, run), 32 * h + 8 * run, at, swz, 8 * run);
+            };
+            auto load_bytes = [&](int h) {
+                if constexpr (DT == GSDH_KV_E4M3) {
+#pragma unroll
+                    for (int k = 0; k < 2 * LPH; k++) {
+                        const int r = k % LPH * RPL + ln / (HD / 16);
+                        raw[k] = load_raw(k < LPH ? kb : vb, __shfl(pg, r / 8, 64), 32 * h + r);
+                    }
+                }
+            };
+            // the halves of tiles that the wave's rows see, of those whose pages are held
+            int u = 0, u1 = 0;
+            auto begin = [&](int tb) {
+                hold_pages(tb);
+                u = max(max(2 * tb, it.first / 32), a.window > 0 ? max(0, plo - a.window + 1) / 32 : 0) + wid / blocks;
+                u1 = live ? min(2 * min(tb + batch, it.t1), phi / 32 + 1) : 0;
+                if (u >= u1) return;
+                pages_for(u);
+                if constexpr (DT == GSDH_KV_E4M3) {
+                    load_bytes(u);
+                } else {
+                    load_half(u, kb, to, swz_k);
+                    load_half(u, vb, to + HALF, swz_v);
+                }
+            };
+            begin(it.t0);
+            form_q();
+            for (int tb = it.t0;;) {
+                for (; u < u1; u += every) {
+                    const int next = u + every, p0 = 32 * u;
+                    const bool more = next < u1;
+                    const unsigned gone = (unsigned)__ballot(pg < 0) & 15u;
+                    if (gone && lane == 0 && head == 0) page_status(a.c, GSDH_PAGES_BAD_INDEX);
+                    if constexpr (DT == GSDH_KV_E4M3) {
+#pragma unroll
+                        for (int k = 0; k < 2 * LPH; k++) {
+                            const int r = k % LPH * RPL + ln / (HD / 16);
+                            convert(raw[k], kt + (k < LPH ? 0u : HALF), r, k < LPH ? swz_k(r) : swz_v(r));
+                        }
+                        if (more) {
+                            pages_for(next);
+                            load_bytes(next);
+                        }
+                    }
+                    const bool edge = masked(p0, 32, plo, phi);
+                    if (DT == GSDH_KV_E4M3) {
+                    } else if (edge) {
+                        loads_but<0>();   // K and V are in LDS
+                    } else {
+                        loads_but<kLoads>();   // K is
+                    }
+                    if (edge)
+                        odd_values(One{}, std::integral_constant<int, 64>{}, p0, kt + HALF, lane, [](uint32_t any) { return __any(any != 0); },
+                                   [] { lds_done(); });
+                    step(One{}, p0, kt, kt + HALF, gone,
+                         [&] {
+                             if constexpr (DT != GSDH_KV_E4M3) {
+                                 if (more) {   // K is read: the next one's may take its place
+                                     pages_for(next);
+                                     lds_done();
+                                     load_half(next, kb, to, swz_k);
+                                 }
+                             }
+                         },
+                         [&] {
+                             if (DT == GSDH_KV_E4M3 || edge) return;
+                             if (more) loads_but<kLoads>();   // V is in LDS
+                             else loads_but<0>();
+                         });
+                    if constexpr (DT != GSDH_KV_E4M3) {
+                        if (more) {
+                            lds_done();
+                            load_half(next, vb, to + HALF, swz_v);
+                        }
+                    }
+                }
+                tb += batch;
+                if (tb >= it.t1) break;
+                __syncthreads();   // (the pages held are read)
+                begin(tb);
+            }
         }
 
         // what the weights are relative to, as an exponent of 2 (beyond fp32's range it stays
         // finite: a difference of two is a number)
         if (m != -INFINITY) m = fabsf(m * to_log2) < kSteep ? -nb : fminf(fmaxf(m * to_log2, -FLT_MAX), FLT_MAX) - top_weight;
         l = swap_add32(l, l, false);
-        if (r0 + col < it.rows) {
+        auto slot_row = [&](int r) { return (2 * ((size_t)grp * nkv + head) + (it.split == 0)) * a.slot_rows + r; };
+        auto out_row = [&](int r) { return static_cast<RT*>(a.out) + (int64_t)(it.token + r / G) * a.out_stride + ((int64_t)head * G + r % G) * HD; };
+        if constexpr (!FEW) {
+            if (r0 + col >= it.rows) return;
             if (it.splits == 1) {
                 const float f = vscale / l;   // (a sum of 0: every score was -inf; NaN)
-                RT* o = static_cast<RT*>(a.out) + (int64_t)(it.token + tok) * a.out_stride + (int64_t)qh * HD + 4 * hi;
+                RT* o = out_row(row) + 4 * hi;
 #pragma unroll
                 for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -567,24 +729,66 @@ __global__ void __launch_bounds__(kThreads, (blocks_per_cu<HD, Kinds<DT, RT>::NP
                         store4(o + 32 * d + 8 * b, x);
                     }
             } else {
-                const size_t slot = 2 * ((size_t)grp * nkv + head) + (it.split == 0);
-                float* o = a.part + (slot * a.slot_rows + row) * HD + 4 * hi;
+                float* o = a.part + slot_row(row) * HD + 4 * hi;
 #pragma unroll
                 for (int d = 0; d < ND; d++)
 #pragma unroll
                     for (int b = 0; b < 4; b++)
                         *reinterpret_cast<float4*>(o + 32 * d + 8 * b) = make_float4(acc[d][4 * b], acc[d][4 * b + 1], acc[d][4 * b + 2], acc[d][4 * b + 3]);
-                if (hi == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * (slot * a.slot_rows + row)) = make_float2(m, l);
+                if (hi == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * slot_row(row)) = make_float2(m, l);
+            }
+            return;
+        }
+        // the waves' outputs, 16-byte words at word ^ row, joined in LDS
+        constexpr int kWords = HD / 4;
+        float4* const red = reinterpret_cast<float4*>(lds);   // [NW][32][kWords]
+        __syncthreads();   // (all halves are read)
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int b = 0; b < 4; b++)
+                red[(wid * kWaveRows + col) * kWords + ((8 * d + 2 * b + hi) ^ (col & (kWords - 1)))] =
+                    make_float4(acc[d][4 * b], acc[d][4 * b + 1], acc[d][4 * b + 2], acc[d][4 * b + 3]);
+        if (hi == 0) wave_ml[wid * kWaveRows + col] = make_float2(m, l);
+        __syncthreads();
+        for (int i = tid; i < it.rows * kWords; i += kThreads) {
+            const int r = i / kWords, word = i % kWords, c = r % kWaveRows;
+            float top = -INFINITY, sum = 0.f;
+            for (int w = r / kWaveRows; w < NW; w += blocks) top = fmaxf(top, wave_ml[w * kWaveRows + c].x);
+            const float base = top == -INFINITY ? 0.f : top;
+            float o[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int w = r / kWaveRows; w < NW; w += blocks) {
+                const float2 ml = wave_ml[w * kWaveRows + c];
+                const float4 y = red[(w * kWaveRows + c) * kWords + (word ^ (c & (kWords - 1)))];
+                const float f = __builtin_amdgcn_exp2f(ml.x - base);
+                sum += f * ml.y;
+                o[0] += f * y.x; o[1] += f * y.y; o[2] += f * y.z; o[3] += f * y.w;
+            }
+            if (it.splits == 1) {
+                const float f = vscale / sum, x[4] = {f * o[0], f * o[1], f * o[2], f * o[3]};
+                store4(out_row(r) + 4 * word, x);
+            } else {
+                *reinterpret_cast<float4*>(a.part + slot_row(r) * HD + 4 * word) = make_float4(o[0], o[1], o[2], o[3]);
+                if (word == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * slot_row(r)) = make_float2(top, sum);
             }
         }
     };
 
+    auto bad_item = [&](const Item& it) {
+        if (tid == 0 && head == 0) page_status(a.c, GSDH_PAGES_BAD_INDEX);
+        for (int i = tid; i < it.rows * (HD / 4); i += kThreads) {
+            const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+            const float nan = __builtin_nanf("");
+            const float x[4] = {nan, nan, nan, nan};
+            store4(static_cast<RT*>(a.out) + (int64_t)(it.token + r / G) * a.out_stride + ((int64_t)head * G + r % G) * HD + d, x);
+        }
+    };
     // -- which items --------------------------------------------------------
     // The chunks' costs lie end to end, and each group of blocks, one per KV
     // head, takes a span of `size` of them: all have as much to do whatever the
     // lengths are.  Every wave finds the block's span by itself.
-    Chunk k{};
     u64 mine = 0;
+    Chunk k{};
     for (int i = lane; i < a.n; i += 64) {
         k = chunk_of(a, i);
         mine += cost_before(a, k, k.items);
@@ -595,17 +799,21 @@ __global__ void __launch_bounds__(kThreads, (blocks_per_cu<HD, Kinds<DT, RT>::NP
     Joint joint{0, 0, 0};
     u64 base = 0;
     for (int c0 = 0; c0 < a.n && base < span_hi; c0 += 64) {
-        if (a.n > 64) k = c0 + lane < a.n ? chunk_of(a, c0 + lane) : Chunk{};
-        else if (lane >= a.n) k = Chunk{};
+        if (a.n > 64) k = c0 + lane < a.n ? chunk_of(a, c0 + lane) : Chunk{};   // (up to 64 are at hand)
         const u64 cost = cost_before(a, k, k.items), incl = wave_scan64(cost), at = base + incl - cost;
         base += readlane64(incl, 63);
         u64 todo = __ballot(cost > 0 && at < span_hi && at + cost > lo);
+        if (!todo) continue;
+        __syncthreads();   // (what lay there is read; all waves write the same)
+        placed[lane] = Placed{k, at};
+        __syncthreads();
         while (todo) {
             const int src = __builtin_ctzll(todo);
             todo &= todo - 1;
-            const auto of = [&](int x) { return __builtin_amdgcn_readlane(x, src); };
-            const Chunk h{of(k.seq), of(k.t0), of(k.m), of(k.base), of(k.items), of((int)k.bad) != 0};
-            const u64 p0 = readlane64(at, src);
+            const auto of = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+            const Placed c = placed[src];
+            const Chunk h{of(c.k.seq), of(c.k.t0), of(c.k.m), of(c.k.base), of(c.k.items), of((int)c.k.bad) != 0};
+            const u64 p0 = readlane64(c.at, 0);
             // the first item that ends behind the span's start
             int u = 0;
             for (int below = h.items - 1; u < below;) {
@@ -633,53 +841,75 @@ __global__ void __launch_bounds__(kThreads, (blocks_per_cu<HD, Kinds<DT, RT>::NP
                 if (h.bad || tiles <= kWhole) {
                     if (p < lo) continue;   // (the group has it in whose span it starts)
                 } else {
-                    const auto cut = [&](u64 x) { return x <= p ? 0 : (int)min((u64)tiles, (x - p) / kPos); };
+                    const u64 tile_cost = (u64)kPos * (u64)cost_of_position(a, it.rows);
+                    const auto cut = [&](u64 x) { return x <= p ? 0 : (int)min((u64)tiles, (x - p) / tile_cost); };
                     const int c_lo = cut(lo), c_hi = cut(span_hi);
                     if (c_lo >= c_hi) continue;
-                    const u64 from = (p + kPos + size - 1) / size - 1, to = (p + (u64)tiles * kPos + size - 1) / size - 1;
+                    const u64 from = (p + tile_cost + size - 1) / size - 1, to = (p + (u64)tiles * tile_cost + size - 1) / size - 1;
                     it.t1 = it.t0 + c_hi;
                     it.t0 += c_lo;
                     it.split = (int)((u64)grp - from);
                     it.splits = (int)(to - from) + 1;
                     if (it.split == 0 && it.splits > 1) joint = Joint{it.splits, it.token, it.rows};
                 }
-                run_item(it);
+                if (it.bad) bad_item(it);
+                else run_item(it);
             }
         }
     }
     if (tid == 0) a.joints[(size_t)grp * nkv + head] = joint;
 }
 
-// The parts of the items that several blocks shared: a block for kJoinRows rows
-// of an item (of most places there is none).
+// The parts of the items that several blocks shared: kJoinBlocks blocks for an
+// item (at most places there is none), kJoinRows rows at a time.  The weights of all
+// parts first, in LDS, then their outputs, eight loads under way at a time.
 template <int HD, typename RT>
 __global__ void __launch_bounds__(256) chunk_join_kernel(const ChunkArgs a) {
-    const int nkv = a.c.n_kv_heads, slices = a.slot_rows / kJoinRows;
-    const int place = (int)(blockIdx.x / (unsigned)slices), r0 = (int)(blockIdx.x % (unsigned)slices) * kJoinRows;
+    __shared__ float weight[kJoinRows][kMostGroups], inv[kJoinRows];
+    const int nkv = a.c.n_kv_heads, place = (int)(blockIdx.x / kJoinBlocks), head = place % nkv, grp = place / nkv, G = a.group;
     const Joint j = a.joints[place];
-    if (r0 >= j.rows || j.parts == 0) return;
-    const int head = place % nkv, grp = place / nkv, G = a.group;
+    if (j.parts == 0) return;
     const float vscale = a.c.dtype == GSDH_KV_E4M3 ? a.c.v_scale[a.layer * nkv + head] : 1.f;
     auto slot_of = [&](int k) { return 2 * ((size_t)(grp + k) * nkv + head) + (k == 0); };
-    for (int i = threadIdx.x; i < min(kJoinRows, j.rows - r0) * (HD / 4); i += 256) {
-        const int row = r0 + i / (HD / 4), d = i % (HD / 4) * 4;
+    for (int r0 = (int)(blockIdx.x % kJoinBlocks) * kJoinRows; r0 < j.rows; r0 += kJoinBlocks * kJoinRows) {
+        const int rows = min(kJoinRows, j.rows - r0);
+        const int r = threadIdx.x / 32, lane = threadIdx.x % 32;   // 32 threads per row
         float top = -INFINITY, sum = 0.f;
-        for (int k = 0; k < j.parts; k++) top = fmaxf(top, a.part_ml[2 * (slot_of(k) * a.slot_rows + row)]);
-        const float base = top == -INFINITY ? 0.f : top;
-        float o[4] = {0.f, 0.f, 0.f, 0.f};
-        // (a part whose weight is 0 is added too: a NaN or an infinity among its V shows)
-#pragma unroll 4
-        for (int k = 0; k < j.parts; k++) {
-            const size_t at = slot_of(k) * a.slot_rows + row;
-            const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
-            const float4 y = *reinterpret_cast<const float4*>(a.part + at * HD + d);
-            const float f = __builtin_amdgcn_exp2f(ml.x - base);
-            sum += f * ml.y;
-            o[0] += f * y.x; o[1] += f * y.y; o[2] += f * y.z; o[3] += f * y.w;
+        if (r < rows) {
+            for (int k = lane; k < j.parts; k += 32) {
+                const float m = a.part_ml[2 * (slot_of(k) * a.slot_rows + r0 + r)];
+                weight[r][k] = m;
+                top = fmaxf(top, m);
+            }
         }
-        const float f = vscale / sum;
-        const float x[4] = {f * o[0], f * o[1], f * o[2], f * o[3]};
-        store4(static_cast<RT*>(a.out) + (int64_t)(j.token + row / G) * a.out_stride + ((int64_t)head * G + row % G) * HD + d, x);
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 32));
+        const float base = top == -INFINITY ? 0.f : top;
+        if (r < rows) {
+            for (int k = lane; k < j.parts; k += 32) {
+                const float f = __builtin_amdgcn_exp2f(weight[r][k] - base);
+                weight[r][k] = f;
+                sum += f * a.part_ml[2 * (slot_of(k) * a.slot_rows + r0 + r) + 1];
+            }
+        }
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 32);
+        if (r < rows && lane == 0) inv[r] = vscale / sum;
+        __syncthreads();
+        for (int i = threadIdx.x; i < rows * (HD / 4); i += 256) {
+            const int c = i / (HD / 4), row = r0 + c, d = i % (HD / 4) * 4;
+            float o[4] = {0.f, 0.f, 0.f, 0.f};
+            // (a part whose weight is 0 is added too: a NaN or an infinity among its V shows)
+#pragma unroll 8
+            for (int k = 0; k < j.parts; k++) {
+                const float4 y = *reinterpret_cast<const float4*>(a.part + (slot_of(k) * a.slot_rows + row) * HD + d);
+                const float f = weight[c][k];
+                o[0] += f * y.x; o[1] += f * y.y; o[2] += f * y.z; o[3] += f * y.w;
+            }
+            const float x[4] = {inv[c] * o[0], inv[c] * o[1], inv[c] * o[2], inv[c] * o[3]};
+            store4(static_cast<RT*>(a.out) + (int64_t)(j.token + row / G) * a.out_stride + ((int64_t)head * G + row % G) * HD + d, x);
+        }
+        __syncthreads();   // (the weights are read)
     }
 }
 
@@ -687,15 +917,13 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const ChunkArgs a) {
 // launches
 // ---------------------------------------------------------------------------
 struct ChunkSpace {
-    int groups, tokens, slot_rows;
+    int groups, slot_rows;
     uint64_t joints, ml, part, bytes;   // where each begins
 };
 ChunkSpace chunk_space(const gsdh_paged_cache& c, int n_tokens, int n_heads, int cus) {
     ChunkSpace s;
-    const int group = n_heads / c.n_kv_heads;
-    s.groups = std::min(std::max(1, (cus > 0 ? cus : 1) * 2 / c.n_kv_heads), kMostGroups);
-    s.tokens = kRows / group;
-    s.slot_rows = (int)std::min<int64_t>(kRows, ((int64_t)n_tokens * group + kJoinRows - 1) / kJoinRows * kJoinRows);
+    s.groups = std::min(std::max(1, (cus > 0 ? cus : 1) / c.n_kv_heads), kMostGroups);
+    s.slot_rows = (int)std::min<int64_t>(kMostRows, ((int64_t)n_tokens * (n_heads / c.n_kv_heads) + kJoinRows - 1) / kJoinRows * kJoinRows);
     const uint64_t places = (uint64_t)s.groups * c.n_kv_heads, rows = 2 * places * s.slot_rows;
     s.joints = 0;
     s.ml = (places * sizeof(Joint) + 255) / 256 * 256;
@@ -708,18 +936,26 @@ bool chunk_shape(const gsdh_paged_cache& c, int n, int n_tokens, int n_heads) {
     return n >= 0 && n_tokens >= 0 && n_heads > 0 && n_heads % c.n_kv_heads == 0 && n_heads / c.n_kv_heads <= 16;
 }
 
-template <int HD, int DT, typename RT>
+template <int HD, int DT, typename RT, bool FEW>
 hipError_t launch_chunk(ChunkArgs a, bool alone, hipStream_t st) {
     static LdsLimit limit;
-    const size_t lds = 4 * (size_t)kPos * HD * 2 + kPagesHeld * 4;
-    constexpr int per_cu = blocks_per_cu<HD, Kinds<DT, RT>::NP>();
-    a.groups = std::max(1, a.groups * per_cu / 2);
-    const hipError_t e = raise_lds_limit(limit, reinterpret_cast<const void*>(chunk_attn_kernel<HD, DT, RT>), lds);
+    constexpr int waves = waves_of<HD, Kinds<DT, RT>::NP>();
+    const size_t lds = (size_t)tiles_bytes<HD, DT, waves>() + kPagesHeld * 4 + waves * kWaveRows * 8 + 64 * sizeof(Placed);
+    a.few = FEW;
+    a.tokens = kWaveRows * (FEW ? 2 : waves) / a.group;
+    a.parts = Kinds<DT, RT>::NP;
+    const hipError_t e = raise_lds_limit(limit, reinterpret_cast<const void*>(chunk_attn_kernel<HD, DT, RT, FEW>), lds);
     if (e != hipSuccess) return e;
     const unsigned places = (unsigned)(a.groups * a.c.n_kv_heads);
-    hipLaunchKernelGGL((chunk_attn_kernel<HD, DT, RT>), dim3(places), dim3(kThreads), lds, st, a);
-    if (!alone) hipLaunchKernelGGL((chunk_join_kernel<HD, RT>), dim3(places * (a.slot_rows / kJoinRows)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((chunk_attn_kernel<HD, DT, RT, FEW>), dim3(places), dim3(64 * waves), lds, st, a);
+    if (!alone) hipLaunchKernelGGL((chunk_join_kernel<HD, RT>), dim3(places * kJoinBlocks), dim3(256), 0, st, a);
     return hipGetLastError();
+}
+template <int HD, int DT, typename RT>
+hipError_t launch_chunk(const ChunkArgs& a, bool alone, hipStream_t st) {
+    // (chunks of at most 64 rows on average)
+    return (int64_t)a.n_tokens * a.group <= (int64_t)2 * kWaveRows * a.n ? launch_chunk<HD, DT, RT, true>(a, alone, st)
+                                                                        : launch_chunk<HD, DT, RT, false>(a, alone, st);
 }
 
 template <int HD>
@@ -775,7 +1011,7 @@ int gsdh_paged_chunk_attention(void* stream, const gsdh_paged_cache* c, int laye
     a.c = *c;
     a.q = q; a.q_stride = q_stride; a.out = out; a.out_stride = out_stride; a.seqs = seqs; a.starts = starts;
     a.layer = layer; a.n = n; a.n_tokens = n_tokens; a.group = n_heads / c->n_kv_heads; a.window = window; a.scale = sm_scale;
-    a.groups = s.groups; a.tokens = s.tokens; a.slot_rows = s.slot_rows;
+    a.groups = s.groups; a.slot_rows = s.slot_rows;
     char* ws = static_cast<char*>(workspace);
     a.joints = reinterpret_cast<Joint*>(ws + s.joints);
     a.part_ml = reinterpret_cast<float*>(ws + s.ml);
