@@ -177,33 +177,29 @@ __device__ __forceinline__ float16v mma(const u32x4v a, const u32x4v b, float16v
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
 }
 
-// eight fp32 values as operands: parts whose sum they are (22 or 24 bits), or (16-bit rows) rounded once
+// two fp32 values as words of operands: parts whose sum they are (22 or 24 bits), or (16-bit rows) rounded once
 template <int CT, int NP>
-__device__ __forceinline__ void operands(const float (&x)[8], u32x4v (&w)[NP]) {
+__device__ __forceinline__ void operand_words(float x, float y, uint32_t (&w)[NP]) {
+    typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
     if constexpr (NP == 1 && CT == GSDH_KV_BF16) {
-        bf8 h;
-#pragma unroll
-        for (int e = 0; e < 8; e++) h[e] = (__bf16)x[e];
-        w[0] = __builtin_bit_cast(u32x4v, h);
+        w[0] = __builtin_bit_cast(uint32_t, bf2{(__bf16)x, (__bf16)y});
     } else if constexpr (NP == 1) {
-        half8 h;
-#pragma unroll
-        for (int e = 0; e < 8; e++) h[e] = (_Float16)x[e];
-        w[0] = __builtin_bit_cast(u32x4v, h);
+        w[0] = __builtin_bit_cast(uint32_t, half2{(_Float16)x, (_Float16)y});
     } else if constexpr (NP == 2) {
         // 11 bits cut off, 11 bits of the rest: two conversions of pairs and a mixed fma per value
-        typedef _Float16 half2 __attribute__((ext_vector_type(2)));
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const half2 h = __builtin_bit_cast(half2, __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]));
-            w[0][i] = __builtin_bit_cast(uint32_t, h);
-            w[1][i] = __builtin_bit_cast(uint32_t, half2{(_Float16)__builtin_fmaf((float)h[0], -1.f, x[2 * i]),
-                                                         (_Float16)__builtin_fmaf((float)h[1], -1.f, x[2 * i + 1])});
-        }
+        const half2 h = __builtin_bit_cast(half2, __builtin_amdgcn_cvt_pkrtz(x, y));
+        w[0] = __builtin_bit_cast(uint32_t, h);
+        w[1] = __builtin_bit_cast(uint32_t, half2{(_Float16)__builtin_fmaf((float)h[0], -1.f, x), (_Float16)__builtin_fmaf((float)h[1], -1.f, y)});
     } else {
-        const Parts<CT, 8> p = split<CT, 8>(x);
+        // 8 + 8 + 8 bits cut off, exact
 #pragma unroll
-        for (int i = 0; i < NP; i++) w[i] = p.w[i];
+        for (int i = 0; i < 3; i++) {
+            const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+            w[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+            x -= __uint_as_float(a & 0xFFFF0000u);
+            y -= __uint_as_float(b & 0xFFFF0000u);
+        }
     }
 }
 
@@ -216,6 +212,10 @@ __device__ __forceinline__ void store4(T* p, const float (&x)[4]) {
         *reinterpret_cast<t4*>(p) = t4{(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
     }
 }
+
+// The compiler moves nothing across: what is asked for ahead of its use stays ahead
+// (left to itself it reads each operand right before its product, and waits).
+__device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0); }
 
 template <int N>
 __device__ __forceinline__ void loads_but() {   // all but the last N loads (and stores) of the wave are done
@@ -339,10 +339,13 @@ chunk_attn_kernel(const ChunkArgs a) {
                 to_log2 = fabsf(scale) * down;
 #pragma unroll
                 for (int s = 0; s < KS; s++) {
-                    float x[8];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = (float)qrow[s][e] * up;
-                    operands<CT, NP>(x, q[s]);
+                    for (int i = 0; i < 4; i++) {
+                        uint32_t w[NP];
+                        operand_words<CT, NP>((float)qrow[s][2 * i] * up, (float)qrow[s][2 * i + 1] * up, w);
+#pragma unroll
+                        for (int p = 0; p < NP; p++) q[s][p][i] = w[p];
+                    }
                 }
             }
             // (a scale of 0 stays above it: a masked -inf times it is -inf)
@@ -367,6 +370,7 @@ chunk_attn_kernel(const ChunkArgs a) {
         float m = -INFINITY, l = 0.f, nb = 0.f, shift = 0.f;
         bool steep = false;
         constexpr float kSteep = 1048576.f;
+        constexpr int kDepth = 2;   // operands that are asked for ahead of their products
 
         // page indices of the tiles from `held` on
         int held_page = 0, held_to = it.t0;
@@ -457,14 +461,20 @@ chunk_attn_kernel(const ChunkArgs a) {
             for (int n = 0; n < N; n++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) xs[n][r] = 0.f;
+            auto k_frag = [&](int i) {   // K's operand: positions 32 (i % N) + col, dims 16 (i / N) + 8 hi ..
+                return *reinterpret_cast<const u32x4v*>(kt + k_at + 32 * (i % N) * RB + (k_word ^ (32u * (i / N))));
+            };
+            u32x4v f[kDepth];
 #pragma unroll
-            for (int s = 0; s < KS; s++)
+            for (int i = 0; i < kDepth; i++) f[i] = k_frag(i);
+            keep_order();
 #pragma unroll
-                for (int n = 0; n < N; n++) {
-                    const u32x4v f = *reinterpret_cast<const u32x4v*>(kt + k_at + 32 * n * RB + (k_word ^ (32u * s)));
+            for (int i = 0; i < KS * N; i++) {
 #pragma unroll
-                    for (int p = NP - 1; p >= 0; p--) xs[n] = mma<CT>(f, q[s][p], xs[n]);
-                }
+                for (int p = NP - 1; p >= 0; p--) xs[i % N] = mma<CT>(f[i % kDepth], q[i / N][p], xs[i % N]);
+                if (i + kDepth < KS * N) f[i % kDepth] = k_frag(i + kDepth);
+                keep_order();
+            }
             scored();
             // what a row does not see is -inf
             if (gone || p0 + 32 * N - 1 > plo || (a.window > 0 && p0 <= phi - a.window)) {
@@ -503,22 +513,33 @@ chunk_attn_kernel(const ChunkArgs a) {
                 for (int e = 0; e < 16 * N; e++) xs[e / 16][e % 16] = fmaf(xs[e / 16][e % 16], to_log2, nb);
             }
             weighed();
+            // weights of a pair of positions, as words of an operand
+            u32x4v pw[2][NP];
+            auto weights = [&](int s, int i) {
+                const float x = __builtin_amdgcn_exp2f(xs[s / 2][8 * (s % 2) + 2 * i]), y = __builtin_amdgcn_exp2f(xs[s / 2][8 * (s % 2) + 2 * i + 1]);
+                l += x + y;
+                uint32_t w[NP];
+                operand_words<CT, NP>(x, y, w);
 #pragma unroll
-            for (int s = 0; s < 2 * N; s++) {
-                float x[8];
-                u32x4v pw[NP];
+                for (int p = 0; p < NP; p++) pw[s % 2][p][i] = w[p];
+            };
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    x[e] = __builtin_amdgcn_exp2f(xs[s / 2][8 * (s % 2) + e]);
-                    l += x[e];
+            for (int i = 0; i < kDepth; i++) f[i] = v_frag(vt, i / ND, i % ND);
+#pragma unroll
+            for (int i = 0; i < 4; i++) weights(0, i);
+            keep_order();
+            // the next eight positions' weights are formed between the products of these
+#pragma unroll
+            for (int i = 0; i < 2 * N * ND; i++) {
+                const int s = i / ND, d = i % ND;
+#pragma unroll
+                for (int p = NP - 1; p >= 0; p--) acc[d] = mma<CT>(f[i % kDepth], pw[s % 2][p], acc[d]);
+                if (i + kDepth < 2 * N * ND) f[i % kDepth] = v_frag(vt, (i + kDepth) / ND, (i + kDepth) % ND);
+                if (s + 1 < 2 * N) {
+#pragma unroll
+                    for (int k = 4 * d / ND; k < 4 * (d + 1) / ND; k++) weights(s + 1, k);
                 }
-                operands<CT, NP>(x, pw);
-#pragma unroll
-                for (int d = 0; d < ND; d++) {
-                    const u32x4v f = v_frag(vt, s, d);
-#pragma unroll
-                    for (int p = NP - 1; p >= 0; p--) acc[d] = mma<CT>(f, pw[p], acc[d]);
-                }
+                keep_order();
             }
         };
         // some row of the block, or (the wave's own positions) of the wave, does not see all of them
