@@ -10,6 +10,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kSeg = 4096;               // logits of a block, a word of LDS each
 constexpr int kMaxVocab = 1 << 24;
+constexpr int kHeld = 2;                 // times four tokens of the history that a thread has on their way
 constexpr uint32_t kInPrompt = 1u << 31;   // in a logit's word, beside how often the answer has it
 
 struct RulesArgs {
@@ -36,16 +37,16 @@ struct Word {
 // A block has 4096 logits of a row and a word of LDS for each: it goes through
 // the whole history and counts what lies in its range by LDS atomics (integers:
 // no order changes them), then through the biases, of which a token's last one
-// counts (the greatest place in the list wins).  A thread's logits, 16 bytes
-// at a time, come in while the lists are read, those that a mask forbids are not
-// read at all.
+// counts (the greatest place in the list wins).  The lists are asked for first, then a
+// thread's logits, 16 bytes at a time; those that a mask forbids are not read at all.
 //
-// Bound by memory for many rows, by the chain list -> LDS -> logits for one.
+// Bound by memory for many rows, by the chain lengths -> lists -> LDS -> logits for one
+// (MEASURED_LOGITS).
 template <typename T>
-__global__ void __launch_bounds__(kThreads) rules_kernel(const RulesArgs a) {
+__global__ void __launch_bounds__(kThreads, 8) rules_kernel(const RulesArgs a) {
     typedef Word<T> W;
     constexpr int N = W::N, NW = kSeg / kThreads / N;   // logits of a word, words of a thread
-    __shared__ __attribute__((aligned(16))) uint32_t lds[kSeg];
+    __shared__ __attribute__((aligned(16))) uint32_t lds[kSeg];   // counts, then places among the biases
     const int row = (int)(blockIdx.x / (unsigned)a.nseg), v0 = (int)(blockIdx.x % (unsigned)a.nseg) * kSeg, tid = threadIdx.x;
     const T* const x = static_cast<const T*>(a.x) + (int64_t)row * a.x_stride;
     T* const out = static_cast<T*>(a.out) + (int64_t)row * a.out_stride;
@@ -55,6 +56,27 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const RulesArgs a) {
     const int mask = a.r.masks ? a.r.mask_rows[row] : -1;
     const bool bad = seen < 0 || seen > a.r.history_width || b0 < 0 || b1 < b0 || b1 > a.r.n_bias || mask < -1 || (mask >= 0 && mask >= a.r.n_masks);
     if (bad) seen = b0 = b1 = 0;
+
+    // the history, four tokens at a time: kHeld of them are on their way at once
+    typedef int int4u __attribute__((ext_vector_type(4), aligned(4)));
+    const int* const history = a.r.history + (int64_t)row * a.r.history_width;
+    int4u held[kHeld];
+    auto load_history = [&](int from) {
+#pragma unroll
+        for (int k = 0; k < kHeld; k++) {
+            const int i = from + 4 * (k * kThreads + tid);
+            held[k] = int4u{-1, -1, -1, -1};
+            if (i + 4 <= seen) {
+                held[k] = *reinterpret_cast<const int4u*>(history + i);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 3; e++)
+                    if (i + e < seen) held[k][e] = history[i + e];
+            }
+        }
+    };
+    load_history(0);
+    const int bias_id = b0 + tid < b1 ? a.r.bias_ids[b0 + tid] : -1;
 
     // what the mask allows of a thread's words, and these words
     uint32_t allowed[NW];
@@ -81,7 +103,7 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const RulesArgs a) {
         for (int i = 0; i < NW; i++)
             if (allowed[i]) load(i);
 
-    uint32_t held[NW] = {};   // in place: words that came in
+    uint32_t came[NW] = {};   // in place: words that came in
     auto clear = [&] {
 #pragma unroll
         for (int i = 0; i < kSeg / kThreads / 4; i++) *reinterpret_cast<uint4*>(lds + 4 * (i * kThreads + tid)) = make_uint4(0u, 0u, 0u, 0u);
@@ -98,26 +120,32 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const RulesArgs a) {
     };
     if (seen) {
         clear();
-        __syncthreads();
-        const int* const history = a.r.history + (int64_t)row * a.r.history_width;
-#pragma unroll 4
-        for (int i = tid; i < seen; i += kThreads) {
-            const unsigned v = (unsigned)history[i] - (unsigned)v0;
-            if (v < (unsigned)kSeg) {
-                if (i < prompt) atomicOr(&lds[v], kInPrompt);
-                else atomicAdd(&lds[v], 1u);
+        lds_barrier();
+        for (int from = 0; from < seen; from += 4 * kHeld * kThreads) {
+            if (from) load_history(from);
+#pragma unroll
+            for (int k = 0; k < kHeld; k++) {
+                const int i = from + 4 * (k * kThreads + tid);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const unsigned v = (unsigned)held[k][e] - (unsigned)v0;   // (-1 is no token of any range)
+                    if (v < (unsigned)kSeg) {
+                        if (i + e < prompt) atomicOr(&lds[v], kInPrompt);
+                        else atomicAdd(&lds[v], 1u);
+                    }
+                }
             }
         }
         const float rep = a.r.repetition ? a.r.repetition[row] : 1.f, freq = a.r.frequency ? a.r.frequency[row] : 0.f,
                     pres = a.r.presence ? a.r.presence[row] : 0.f;
-        __syncthreads();
+        lds_barrier();
 #pragma unroll
         for (int i = 0; i < NW; i++) {
             uint32_t w[N];
             if (!allowed[i] || !word_of(i, w)) continue;
-            if (a.in_place && !held[i]) {
+            if (a.in_place) {
                 load(i);
-                held[i] = 1;
+                came[i] = 1;
             }
 #pragma unroll
             for (int e = 0; e < N; e++) {
@@ -132,24 +160,23 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const RulesArgs a) {
                 y[i][e] = z;
             }
         }
+        if (b1 > b0) lds_barrier();   // (the counts are read)
     }
     if (b1 > b0) {
-        __syncthreads();
         clear();
-        __syncthreads();
-#pragma unroll 2
+        lds_barrier();
         for (int i = b0 + tid; i < b1; i += kThreads) {
-            const unsigned v = (unsigned)a.r.bias_ids[i] - (unsigned)v0;
+            const unsigned v = (unsigned)(i < b0 + kThreads ? bias_id : a.r.bias_ids[i]) - (unsigned)v0;
             if (v < (unsigned)kSeg) atomicMax(&lds[v], (uint32_t)(i - b0) + 1u);
         }
-        __syncthreads();
+        lds_barrier();
 #pragma unroll
         for (int i = 0; i < NW; i++) {
             uint32_t w[N];
             if (!allowed[i] || !word_of(i, w)) continue;
-            if (a.in_place && !held[i]) {
+            if (a.in_place && !came[i]) {
                 load(i);
-                held[i] = 1;
+                came[i] = 1;
             }
 #pragma unroll
             for (int e = 0; e < N; e++)
@@ -161,7 +188,7 @@ __global__ void __launch_bounds__(kThreads) rules_kernel(const RulesArgs a) {
         const int left = a.vocab - at(i);
         if (left <= 0) continue;
         const uint32_t whole = left >= N ? (1u << N) - 1 : (1u << left) - 1;
-        if (a.in_place && !bad && !held[i]) {
+        if (a.in_place && !bad && !came[i]) {
             if ((allowed[i] & whole) == whole) continue;   // nothing of it changes
             if (allowed[i] & whole) load(i);
         }

@@ -11,6 +11,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMostPairs = 1024;   // of a block's tokens
+constexpr int kMany = 4;           // items of a thread
+constexpr int kFewBlocks = 2048;   // blocks of one item per thread that the chip takes at once
 
 struct TurnArgs {
     const void *x, *k, *v;   // rows to rows: x alone
@@ -23,7 +25,7 @@ struct TurnArgs {
     int pairs, interleaved;
     int turned_runs, head_runs;   // threads' runs of a head that is turned: of four pairs; with those that follow
     int tokens, parts;            // of a block; blocks of a token
-    int layer, in_place;
+    int layer, in_place, many;    // many: kMany items per thread
     float scale;
 };
 
@@ -87,31 +89,69 @@ __device__ __forceinline__ void cache_run(unsigned char* p, int count, const flo
 // positions keep their angles (an fp32 product is off by 2^-24 of it: half a
 // degree at position 131072 and frequency 1), t's fraction rounded once to fp32.
 //
-// A thread: four pairs of a head, or up to eight values that are not turned
-// (the rest of a head, V).  A block's angles are formed once, in LDS, while its
-// rows are on their way.  DT < 0: rows to rows; else K and V go to the cache.
-// VEC: runs of four values are aligned (else element by element).
-//
-// Bound by memory for a prompt's rows and by the launch for a step's.
-template <typename RT, int DT, bool VEC>
+// An item: four pairs of a head, or up to eight values that are not turned (the
+// rest of a head, V).  A block's angles are formed once, in LDS, while its rows
+// and, for the cache, sequence -> page come in.  DT < 0: rows to rows; else K and V
+// go to the cache.  VEC: runs of four values are aligned (else element by element).
+// U: items of a thread, 1 where that is few blocks (a step of 64 tokens: the launch
+// and its chain of loads count), else kMany, a token's items in one block: its chain
+// is waited for once (MEASURED_ROPE).
+template <typename RT, int DT, bool VEC, int U>
 __global__ void __launch_bounds__(kThreads) turn_kernel(const TurnArgs a) {
     __shared__ float2 cs[kMostPairs];
-    const int per_token = (a.heads + (DT < 0 ? 0 : a.nkv)) * a.head_runs + (DT < 0 ? 0 : a.nkv * (a.hd / 8));
-    const int first = a.tokens > 1 ? (int)blockIdx.x * a.tokens : (int)blockIdx.x / a.parts;
-    const int item = a.tokens > 1 ? (int)threadIdx.x : (int)(blockIdx.x % (unsigned)a.parts) * kThreads + (int)threadIdx.x;
-    const int tok = first + item / per_token, in_token = item % per_token;   // (one token: item < per_token, or nothing to do)
-    const bool mine = item < a.tokens * per_token && tok < a.n;
+    constexpr bool kPaged = DT >= 0;
+    const int turned_items = (a.heads + (kPaged ? a.nkv : 0)) * a.head_runs, per_token = turned_items + (kPaged ? a.nkv * (a.hd / 8) : 0);
+    const int first = a.tokens > 1 ? (int)blockIdx.x * a.tokens : (int)(blockIdx.x / (unsigned)a.parts);
+    const int item0 = a.tokens > 1 ? (int)threadIdx.x : (int)(blockIdx.x % (unsigned)a.parts) * kThreads * U + (int)threadIdx.x;
 
-    // what, and from where
-    int seq = 0, pos = 0, page = 0;
-    uint32_t bad = 0;
-    bool live = mine;
-    if constexpr (DT >= 0) {
-        if (mine) {
-            seq = a.seqs[tok];
+    struct Item {
+        int head, i0, i1, n0, n1, run;   // the two runs of up to four values
+        bool is_k, is_v, turns, live;
+    };
+    Item it[U];
+    float x[U][8];
+    const int tok = U == 1 ? first + item0 / per_token : first;   // (one token: item0 < per_token, or nothing to do)
+    const bool token = tok < a.n;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int item = item0 + u * kThreads, in_token = U == 1 ? item % per_token : item;
+        Item& t = it[u];
+        t.live = token && item < a.tokens * per_token;
+        t.is_v = kPaged && in_token >= turned_items;
+        t.head = t.is_v ? (in_token - turned_items) / (a.hd / 8) : in_token / a.head_runs;
+        t.run = t.is_v ? (in_token - turned_items) % (a.hd / 8) : in_token % a.head_runs;
+        t.is_k = kPaged && !t.is_v && t.head >= a.heads;
+        t.turns = !t.is_v && t.run < a.turned_runs;
+        if (t.is_k) t.head -= a.heads;
+        if (t.turns) {
+            const int left = a.pairs - 4 * t.run;
+            t.i0 = a.interleaved ? 8 * t.run : 4 * t.run;
+            t.i1 = a.interleaved ? t.i0 + 4 : t.i0 + a.pairs;
+            t.n0 = a.interleaved ? min(4, 2 * left) : min(4, left);
+            t.n1 = a.interleaved ? max(0, min(4, 2 * left - 4)) : min(4, left);
+        } else {
+            t.i0 = t.is_v ? 8 * t.run : 2 * a.pairs + 8 * (t.run - a.turned_runs);
+            t.i1 = t.i0 + 4;
+            t.n0 = min(4, a.hd - t.i0);
+            t.n1 = max(0, min(4, a.hd - t.i1));
+            if (!t.is_k && !t.is_v && a.in_place) t.live = false;
+        }
+        if (t.live) {   // (rows that are left out below are read, too: they are there)
+            const RT* src = static_cast<const RT*>(t.is_v ? a.v : t.is_k ? a.k : a.x) +
+                            (int64_t)tok * (t.is_v ? a.v_stride : t.is_k ? a.k_stride : a.x_stride) + (int64_t)t.head * a.hd;
+            load_run<RT, VEC>(src + t.i0, t.n0, x[u]);
+            load_run<RT, VEC>(src + t.i1, t.n1, x[u] + 4);
+        }
+    }
+    int pos = 0, page = 0;
+    bool left_out = false;
+    if constexpr (kPaged) {
+        if (token && item0 < a.tokens * per_token) {
+            const int seq = a.seqs[tok];
             pos = a.positions[tok];
-            live = seq >= 0;
-            if (live) {
+            left_out = seq < 0;
+            uint32_t bad = 0;
+            if (!left_out) {
                 if (seq >= a.c.n_seqs || pos < 0 || pos >= a.c.table_width * a.c.page_size || pos >= a.c.lens[seq]) {
                     bad = GSDH_PAGES_BAD_INDEX;
                 } else {
@@ -119,43 +159,10 @@ __global__ void __launch_bounds__(kThreads) turn_kernel(const TurnArgs a) {
                     if ((unsigned)page >= (unsigned)a.c.n_pages) bad = GSDH_PAGES_BAD_INDEX;
                     else if (a.c.refs && a.c.refs[page] != 1) bad = GSDH_PAGES_SHARED;
                 }
-                if (bad && in_token == 0) page_status(a.c, bad);
-                live = !bad;
+                if (bad && item0 % per_token == 0) page_status(a.c, bad);
+                left_out = bad != 0;
             }
         }
-    }
-    const int turned_heads = a.heads + (DT < 0 ? 0 : a.nkv), turned_items = turned_heads * a.head_runs;
-    const bool is_v = DT >= 0 && in_token >= turned_items;
-    const int head = is_v ? (in_token - turned_items) / (a.hd / 8) : in_token / a.head_runs;
-    const int run = is_v ? (in_token - turned_items) % (a.hd / 8) : in_token % a.head_runs;
-    const bool is_k = DT >= 0 && !is_v && head >= a.heads;
-    const bool turns = !is_v && run < a.turned_runs;
-    int i0, i1, n0, n1;   // the two runs of up to four values
-    if (turns) {
-        const int left = a.pairs - 4 * run;
-        if (a.interleaved) {
-            i0 = 8 * run;
-            i1 = i0 + 4;
-            n0 = min(4, 2 * left);
-            n1 = max(0, min(4, 2 * left - 4));
-        } else {
-            i0 = 4 * run;
-            i1 = i0 + a.pairs;
-            n0 = n1 = min(4, left);
-        }
-    } else {
-        i0 = is_v ? 8 * run : 2 * a.pairs + 8 * (run - a.turned_runs);
-        i1 = i0 + 4;
-        n0 = min(4, a.hd - i0);
-        n1 = max(0, min(4, a.hd - i1));
-    }
-    if (!turns && !is_k && !is_v && a.in_place) live = false;
-    const RT* src = static_cast<const RT*>(is_v ? a.v : is_k ? a.k : a.x) +
-                    (int64_t)tok * (is_v ? a.v_stride : is_k ? a.k_stride : a.x_stride) + (int64_t)(is_k ? head - a.heads : head) * a.hd;
-    float x[8];
-    if (live) {
-        load_run<RT, VEC>(src + i0, n0, x);
-        load_run<RT, VEC>(src + i1, n1, x + 4);
     }
     for (int p = threadIdx.x; p < a.tokens * a.pairs; p += kThreads) {
         const int t = first + p / a.pairs;
@@ -165,41 +172,42 @@ __global__ void __launch_bounds__(kThreads) turn_kernel(const TurnArgs a) {
         sincospif((float)(2.0 * (turn - rint(turn))), &s, &c);
         cs[p] = make_float2(c * a.scale, s * a.scale);
     }
-    __syncthreads();
-    if (!live) return;
-    if (turns) {
-        const float2* const w = cs + (tok - first) * a.pairs + 4 * run;
+    lds_barrier();   // (the rows need not be here yet)
+    if (left_out) return;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (!VEC && 4 * run + e >= a.pairs) break;
-            const float2 r = w[e];
-            const float u = a.interleaved ? x[2 * e] : x[e], v = a.interleaved ? x[2 * e + 1] : x[e + 4];
-            const float y = u * r.x - v * r.y, z = u * r.y + v * r.x;
-            if (a.interleaved) {
-                x[2 * e] = y;
-                x[2 * e + 1] = z;
-            } else {
-                x[e] = y;
-                x[e + 4] = z;
+    for (int u = 0; u < U; u++) {
+        const Item& t = it[u];
+        if (!t.live) continue;
+        float (&y)[8] = x[u];
+        if (t.turns) {
+            const float2* const w = cs + (tok - first) * a.pairs + 4 * t.run;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (!VEC && 4 * t.run + e >= a.pairs) break;
+                const float2 r = w[e];
+                const float p = a.interleaved ? y[2 * e] : y[e], q = a.interleaved ? y[2 * e + 1] : y[e + 4];
+                const float c = p * r.x - q * r.y, d = p * r.y + q * r.x;
+                y[a.interleaved ? 2 * e : e] = c;
+                y[a.interleaved ? 2 * e + 1 : e + 4] = d;
             }
         }
-    }
-    if constexpr (DT >= 0) {
-        if (is_k || is_v) {
-            constexpr int ES = DT == GSDH_KV_E4M3 ? 1 : 2;
-            const int h = is_k ? head - a.heads : head, ps = a.c.page_size, slot = pos % ps;
-            const float scale = DT == GSDH_KV_E4M3 ? (is_v ? a.c.v_scale : a.c.k_scale)[a.layer * a.nkv + h] : 1.f;
-            const size_t at = ((size_t)a.layer * a.c.n_pages + page) * ps * a.nkv * a.hd +
-                              (a.c.head_major ? (size_t)h * ps + slot : (size_t)slot * a.nkv + h) * a.hd;
-            unsigned char* dst = static_cast<unsigned char*>(is_v ? a.c.v : a.c.k) + at * ES;
-            cache_run<DT, VEC>(dst + (size_t)i0 * ES, n0, x, scale);
-            cache_run<DT, VEC>(dst + (size_t)i1 * ES, n1, x + 4, scale);
-            return;
+        if constexpr (kPaged) {
+            if (t.is_k || t.is_v) {
+                constexpr int ES = DT == GSDH_KV_E4M3 ? 1 : 2;
+                const int ps = a.c.page_size, slot = pos % ps;
+                const float scale = DT == GSDH_KV_E4M3 ? (t.is_v ? a.c.v_scale : a.c.k_scale)[a.layer * a.nkv + t.head] : 1.f;
+                const size_t at = ((size_t)a.layer * a.c.n_pages + page) * ps * a.nkv * a.hd +
+                                  (a.c.head_major ? (size_t)t.head * ps + slot : (size_t)slot * a.nkv + t.head) * a.hd;
+                unsigned char* dst = static_cast<unsigned char*>(t.is_v ? a.c.v : a.c.k) + at * ES;
+                cache_run<DT, VEC>(dst + (size_t)t.i0 * ES, t.n0, y, scale);
+                cache_run<DT, VEC>(dst + (size_t)t.i1 * ES, t.n1, y + 4, scale);
+                continue;
+            }
         }
+        RT* dst = static_cast<RT*>(a.out) + (int64_t)tok * a.out_stride + (int64_t)t.head * a.hd;
+        store_run<RT, VEC>(dst + t.i0, t.n0, y);
+        store_run<RT, VEC>(dst + t.i1, t.n1, y + 4);
     }
-    RT* dst = static_cast<RT*>(a.out) + (int64_t)tok * a.out_stride + (int64_t)head * a.hd;
-    store_run<RT, VEC>(dst + i0, n0, x);
-    store_run<RT, VEC>(dst + i1, n1, x + 4);
 }
 
 int check_rope(const gsdh_rope* r, int head_dim, int dtype, const char* who) {
@@ -229,14 +237,21 @@ bool plan_turn(TurnArgs& a, const gsdh_rope& r, bool paged) {
     a.tokens = (int)(items <= kThreads / 2 ? kThreads / items : 1);
     if (a.tokens * a.pairs > kMostPairs) a.tokens = kMostPairs / a.pairs;
     a.parts = (int)((items + kThreads - 1) / kThreads);
+    a.many = a.tokens == 1 && (int64_t)a.n * a.parts > kFewBlocks;
+    if (a.many) a.parts = (int)((items + kMany * kThreads - 1) / (kMany * kThreads));
     return (a.tokens > 1 ? (int64_t)a.n : (int64_t)a.n * a.parts) <= 0x7FFFFFFF;
 }
 
+template <typename RT, int DT, bool VEC>
+void launch_turn(const TurnArgs& a, hipStream_t st) {
+    const dim3 grid((unsigned)(a.tokens > 1 ? (a.n + a.tokens - 1) / a.tokens : a.n * a.parts)), block(kThreads);
+    if (a.many) hipLaunchKernelGGL((turn_kernel<RT, DT, VEC, kMany>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((turn_kernel<RT, DT, VEC, 1>), grid, block, 0, st, a);
+}
 template <typename RT, int DT>
 void launch_turn(const TurnArgs& a, bool vec, hipStream_t st) {
-    const dim3 grid((unsigned)(a.tokens > 1 ? (a.n + a.tokens - 1) / a.tokens : a.n * a.parts)), block(kThreads);
-    if (vec) hipLaunchKernelGGL((turn_kernel<RT, DT, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((turn_kernel<RT, DT, false>), grid, block, 0, st, a);
+    if (vec) launch_turn<RT, DT, true>(a, st);
+    else launch_turn<RT, DT, false>(a, st);
 }
 template <int DT>
 void launch_turn_rows(const TurnArgs& a, int dtype, bool vec, hipStream_t st) {
