@@ -22,9 +22,9 @@ constexpr int kRuns = kPos / 8;      // its runs of eight positions: a page is a
 // What a block does is measured in quarters of the time that a position of up to 32
 // rows takes, whose K and V have to come (a tile of 64 1.2 us); a position of more
 // rows is that often more, by the products of its rows' parts (measured: a tile of
-// 256 rows 2.2 us in 16 bits, 4.2 us in two parts), and an item's start and end, waits
-// under load, are 13 us.
-constexpr int kCost = 2800;
+// 256 rows 2.1 us in 16 bits, 4.2 us in two parts), and an item's start and end, waits
+// under load, are 20 us (a prompt of 4096 tokens took 307 us with 13 us in its place).
+constexpr int kCost = 4400;
 constexpr int kWhole = 4;            // an item of so few tiles is not cut
 constexpr int kLeastSpan = 2048;     // the least a block takes
 __device__ __forceinline__ int cost_of_rows(bool few, int rows, int parts) {
@@ -60,15 +60,21 @@ struct Joint {   // of an item that several blocks share, at its first one's pla
     int rows;    // token x head rows
 };
 
+// A row's weights so far: the largest score, unscaled, their sum, and what they are
+// relative to: 2^(x to_log2 + nb), or (m to_log2 beyond 2^20) the largest's.
+struct __attribute__((aligned(16))) Sum {
+    float m, l, nb, to_log2;
+};
+
 struct ChunkArgs {
     gsdh_paged_cache c;
     const void* q;
     void* out;
     const int *seqs, *starts;
-    // of shared items: outputs [slot][slot_rows][HD], (m, l) [slot][slot_rows][2], slot =
+    // of shared items: outputs [slot][slot_rows][HD], sums [slot][slot_rows], slot =
     // 2 (group n_kv + head) + 1 for an item's first part, + 0 for a later one
     float* part;
-    float* part_ml;
+    Sum* part_sum;
     Joint* joints;   // [group n_kv + head]
     int64_t q_stride, out_stride;
     int layer, n, n_tokens, group, window, groups, slot_rows;
@@ -150,6 +156,16 @@ struct Placed {
     Chunk k;
     u64 at;
 };
+
+constexpr float kSteep = 1048576.f;   // exponents of 2 beyond which a rounded product would not do
+__device__ __forceinline__ bool is_steep(float m, float to_log2) { return !(fabsf(m * to_log2) < kSteep); }
+// What a part of a row counts beside the part with the row's largest score, top (of
+// these the least nb): a difference of scores, however large they are, or of the
+// rounded exponents that the weights were formed with.
+__device__ __forceinline__ float part_weight(const Sum& s, float top, float nb) {
+    if (s.m == -INFINITY) return 0.f;
+    return __builtin_amdgcn_exp2f(is_steep(top, s.to_log2) || is_steep(s.m, s.to_log2) ? (s.m - top) * s.to_log2 : nb - s.nb);
+}
 
 // What a block does of an item.
 struct Item {
@@ -254,10 +270,16 @@ constexpr unsigned tiles_bytes() {
 // FEW: items of up to 64 rows, whose waves each take positions of their own (32 at a
 // time, of the same rows as the waves `blocks` from it), and whose outputs are
 // joined at the end: as many bytes under way and as much multiplied as with many
-// rows.  Else items of 128 or 256 rows, which all waves read the same tiles for.  A
-// call takes one way for all its chunks, by the mean of their rows: 16 chunks of 20
-// rows over 3400 positions TIME_FEW us and TIME_FEW_WIDE us, a prompt of 4096 tokens (16384 rows) TIME_PROMPT_FEW us and
-// TIME_PROMPT us.  (Both ways in one kernel spilled registers in both loops.)
+// rows, for a longer start and end.  Else items of 128 or 256 rows, which all waves
+// read the same tiles for.  A call takes one way for all its chunks (is_few, with
+// both ways' times); in one kernel both had registers spilled in their loops.
+//
+// Bound by the matrix cores for prompts: 2048 tokens of 32 heads over 8 of 128 dims at the
+// end of 32768 positions, bf16, 1064 us, 1.0 PFLOP/s of products (a library's product of
+// 8192^3 gets 1.2 on the same card, whose clock falls under both: 1.8 GHz in this
+// kernel); 4096 tokens of fp32 rows over fp16 293 us, 0.94 PFLOP/s of products, two for
+// each.  By memory for few rows: 16 chunks of 5 tokens over up to 8191 positions (199 MB)
+// 68 us, of which the stream is 36.
 template <int HD, int DT, typename RT, bool FEW>
 __global__ void __launch_bounds__((64 * waves_of<HD, Kinds<DT, RT>::NP>()), (waves_of<HD, Kinds<DT, RT>::NP>() / 4))
 chunk_attn_kernel(const ChunkArgs a) {
@@ -267,11 +289,11 @@ chunk_attn_kernel(const ChunkArgs a) {
     static_assert(kThreads >= kPagesHeld && kRuns % NW == 0, "a thread per page held, whole runs per wave");
     constexpr unsigned RB = HD * 2, TILE = kPos * RB;   // a row and a tile of 16-bit values in LDS
     constexpr unsigned BUF = tiles_bytes<HD, DT, NW>();
-    // K, V of NS tiles, or of half a tile for each wave, or the waves' outputs; the pages; the waves' (m, l)
+    // K, V of NS tiles, or of half a tile for each wave, or the waves' outputs; the pages; the waves' sums
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     int* const pages = reinterpret_cast<int*>(lds + BUF);
-    float2* const wave_ml = reinterpret_cast<float2*>(lds + BUF + kPagesHeld * 4);   // [NW][32]
-    Placed* const placed = reinterpret_cast<Placed*>(lds + BUF + kPagesHeld * 4 + NW * kWaveRows * 8);   // [64]
+    Sum* const wave_sum = reinterpret_cast<Sum*>(lds + BUF + kPagesHeld * 4);   // [NW][32]
+    Placed* const placed = reinterpret_cast<Placed*>(lds + BUF + kPagesHeld * 4 + NW * kWaveRows * sizeof(Sum));   // [64]
     const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_byte*)lds;
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, hi = lane >> 5;
     const int G = a.group, nkv = a.c.n_kv_heads, head = (int)(blockIdx.x % (unsigned)nkv), grp = (int)(blockIdx.x / (unsigned)nkv);
@@ -369,7 +391,6 @@ chunk_attn_kernel(const ChunkArgs a) {
         // whatever fp32 rounds off the scaled scores.
         float m = -INFINITY, l = 0.f, nb = 0.f, shift = 0.f;
         bool steep = false;
-        constexpr float kSteep = 1048576.f;
         constexpr int kDepth = 2;   // operands that are asked for ahead of their products
 
         // page indices of the tiles from `held` on
@@ -491,18 +512,18 @@ chunk_attn_kernel(const ChunkArgs a) {
             const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
             top = fmaxf(m, fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])));
             if (__any(top > m)) {
-                const bool was_steep = !(fabsf(m * to_log2) < kSteep), is_steep = !(fabsf(top * to_log2) < kSteep);
-                const float nb1 = is_steep ? 0.f : fmaf(-top, to_log2, top_weight), shift1 = is_steep ? top_weight : fmaf(top, to_log2, nb1);
+                const bool was = is_steep(m, to_log2), is = is_steep(top, to_log2);
+                const float nb1 = is ? 0.f : fmaf(-top, to_log2, top_weight), shift1 = is ? top_weight : fmaf(top, to_log2, nb1);
                 // (nothing seen so far: there is nothing to weigh anew)
                 const float f = m == -INFINITY ? 1.f
-                              : __builtin_amdgcn_exp2f(was_steep || is_steep ? fmaf(m - top, to_log2, shift1 - shift) : nb1 - nb);
+                              : __builtin_amdgcn_exp2f(was || is ? fmaf(m - top, to_log2, shift1 - shift) : nb1 - nb);
 #pragma unroll
                 for (int d = 0; d < ND; d++) acc[d] *= f;
                 l *= f;
                 m = top;
                 nb = nb1;
                 shift = shift1;
-                steep = __any(is_steep && top != -INFINITY);
+                steep = __any(is && top != -INFINITY);
             }
             if (steep) {   // the weights' exponents in place of the scores
                 const float base = m == -INFINITY ? 0.f : m;
@@ -731,9 +752,6 @@ chunk_attn_kernel(const ChunkArgs a) {
             }
         }
 
-        // what the weights are relative to, as an exponent of 2 (beyond fp32's range it stays
-        // finite: a difference of two is a number)
-        if (m != -INFINITY) m = fabsf(m * to_log2) < kSteep ? -nb : fminf(fmaxf(m * to_log2, -FLT_MAX), FLT_MAX) - top_weight;
         l = swap_add32(l, l, false);
         auto slot_row = [&](int r) { return (2 * ((size_t)grp * nkv + head) + (it.split == 0)) * a.slot_rows + r; };
         auto out_row = [&](int r) { return static_cast<RT*>(a.out) + (int64_t)(it.token + r / G) * a.out_stride + ((int64_t)head * G + r % G) * HD; };
@@ -756,7 +774,7 @@ chunk_attn_kernel(const ChunkArgs a) {
 #pragma unroll
                     for (int b = 0; b < 4; b++)
                         *reinterpret_cast<float4*>(o + 32 * d + 8 * b) = make_float4(acc[d][4 * b], acc[d][4 * b + 1], acc[d][4 * b + 2], acc[d][4 * b + 3]);
-                if (hi == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * slot_row(row)) = make_float2(m, l);
+                if (hi == 0) a.part_sum[slot_row(row)] = Sum{m, l, nb, to_log2};
             }
             return;
         }
@@ -770,27 +788,45 @@ chunk_attn_kernel(const ChunkArgs a) {
             for (int b = 0; b < 4; b++)
                 red[(wid * kWaveRows + col) * kWords + ((8 * d + 2 * b + hi) ^ (col & (kWords - 1)))] =
                     make_float4(acc[d][4 * b], acc[d][4 * b + 1], acc[d][4 * b + 2], acc[d][4 * b + 3]);
-        if (hi == 0) wave_ml[wid * kWaveRows + col] = make_float2(m, l);
+        if (hi == 0) wave_sum[wid * kWaveRows + col] = Sum{m, l, nb, to_log2};
+        __syncthreads();
+        if (tid < it.rows) {   // a thread per row: what each wave's outputs count
+            float top = -INFINITY, low = INFINITY, sum = 0.f;
+            const int w0 = tid / kWaveRows, c = tid % kWaveRows;
+            const float to = wave_sum[tid].to_log2;
+#pragma unroll
+            for (int w = 0; w < NW; w++)
+                if ((w & (blocks - 1)) == w0) top = fmaxf(top, wave_sum[w * kWaveRows + c].m);
+#pragma unroll
+            for (int w = 0; w < NW; w++) {
+                const Sum p = wave_sum[w * kWaveRows + c];
+                if ((w & (blocks - 1)) == w0 && p.m == top) low = fminf(low, p.nb);
+            }
+#pragma unroll
+            for (int w = 0; w < NW; w++) {
+                if ((w & (blocks - 1)) != w0) continue;
+                const Sum p = wave_sum[w * kWaveRows + c];
+                const float f = part_weight(p, top, low);
+                sum += f * p.l;
+                wave_sum[w * kWaveRows + c].m = f;
+            }
+            if (it.splits == 1) wave_sum[tid].l = vscale / sum;   // (a sum of 0: every score was -inf; NaN)
+            else a.part_sum[slot_row(tid)] = Sum{top, sum, low, to};
+        }
         __syncthreads();
         for (int i = tid; i < it.rows * kWords; i += kThreads) {
             const int r = i / kWords, word = i % kWords, c = r % kWaveRows;
-            float top = -INFINITY, sum = 0.f;
-            for (int w = r / kWaveRows; w < NW; w += blocks) top = fmaxf(top, wave_ml[w * kWaveRows + c].x);
-            const float base = top == -INFINITY ? 0.f : top;
             float o[4] = {0.f, 0.f, 0.f, 0.f};
             for (int w = r / kWaveRows; w < NW; w += blocks) {
-                const float2 ml = wave_ml[w * kWaveRows + c];
                 const float4 y = red[(w * kWaveRows + c) * kWords + (word ^ (c & (kWords - 1)))];
-                const float f = __builtin_amdgcn_exp2f(ml.x - base);
-                sum += f * ml.y;
+                const float f = wave_sum[w * kWaveRows + c].m;
                 o[0] += f * y.x; o[1] += f * y.y; o[2] += f * y.z; o[3] += f * y.w;
             }
             if (it.splits == 1) {
-                const float f = vscale / sum, x[4] = {f * o[0], f * o[1], f * o[2], f * o[3]};
+                const float f = wave_sum[r].l, x[4] = {f * o[0], f * o[1], f * o[2], f * o[3]};
                 store4(out_row(r) + 4 * word, x);
             } else {
                 *reinterpret_cast<float4*>(a.part + slot_row(r) * HD + 4 * word) = make_float4(o[0], o[1], o[2], o[3]);
-                if (word == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * slot_row(r)) = make_float2(top, sum);
             }
         }
     };
@@ -895,23 +931,28 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const ChunkArgs a) {
     for (int r0 = (int)(blockIdx.x % kJoinBlocks) * kJoinRows; r0 < j.rows; r0 += kJoinBlocks * kJoinRows) {
         const int rows = min(kJoinRows, j.rows - r0);
         const int r = threadIdx.x / 32, lane = threadIdx.x % 32;   // 32 threads per row
-        float top = -INFINITY, sum = 0.f;
-        if (r < rows) {
-            for (int k = lane; k < j.parts; k += 32) {
-                const float m = a.part_ml[2 * (slot_of(k) * a.slot_rows + r0 + r)];
-                weight[r][k] = m;
-                top = fmaxf(top, m);
-            }
-        }
+        // (the first 32 parts' sums are loaded once)
+        const Sum* const sums = a.part_sum + r0 + r;
+        const int parts = r < rows ? j.parts : 0;
+        auto sum_of = [&](int k) { return sums[slot_of(k) * a.slot_rows]; };
+        Sum p0{-INFINITY, 0.f, INFINITY, 1.f};
+        if (lane < parts) p0 = sum_of(lane);
+        float top = p0.m, sum = 0.f;
+        for (int k = lane + 32; k < parts; k += 32) top = fmaxf(top, sum_of(k).m);
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 32));
-        const float base = top == -INFINITY ? 0.f : top;
-        if (r < rows) {
-            for (int k = lane; k < j.parts; k += 32) {
-                const float f = __builtin_amdgcn_exp2f(weight[r][k] - base);
-                weight[r][k] = f;
-                sum += f * a.part_ml[2 * (slot_of(k) * a.slot_rows + r0 + r) + 1];
-            }
+        float low = p0.m == top ? p0.nb : INFINITY;
+        for (int k = lane + 32; k < parts; k += 32) {
+            const Sum p = sum_of(k);
+            if (p.m == top) low = fminf(low, p.nb);
+        }
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) low = fminf(low, __shfl_xor(low, o, 32));
+        for (int k = lane; k < parts; k += 32) {
+            const Sum p = k == lane ? p0 : sum_of(k);
+            const float f = part_weight(p, top, low);
+            weight[r][k] = f;
+            sum += f * p.l;
         }
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 32);
@@ -939,7 +980,7 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const ChunkArgs a) {
 // ---------------------------------------------------------------------------
 struct ChunkSpace {
     int groups, slot_rows;
-    uint64_t joints, ml, part, bytes;   // where each begins
+    uint64_t joints, sums, part, bytes;   // where each begins
 };
 ChunkSpace chunk_space(const gsdh_paged_cache& c, int n_tokens, int n_heads, int cus) {
     ChunkSpace s;
@@ -947,8 +988,8 @@ ChunkSpace chunk_space(const gsdh_paged_cache& c, int n_tokens, int n_heads, int
     s.slot_rows = (int)std::min<int64_t>(kMostRows, ((int64_t)n_tokens * (n_heads / c.n_kv_heads) + kJoinRows - 1) / kJoinRows * kJoinRows);
     const uint64_t places = (uint64_t)s.groups * c.n_kv_heads, rows = 2 * places * s.slot_rows;
     s.joints = 0;
-    s.ml = (places * sizeof(Joint) + 255) / 256 * 256;
-    s.part = (s.ml + rows * 8 + 255) / 256 * 256;
+    s.sums = (places * sizeof(Joint) + 255) / 256 * 256;
+    s.part = (s.sums + rows * sizeof(Sum) + 255) / 256 * 256;
     s.bytes = s.part + rows * c.head_dim * 4;
     return s;
 }
@@ -957,11 +998,20 @@ bool chunk_shape(const gsdh_paged_cache& c, int n, int n_tokens, int n_heads) {
     return n >= 0 && n_tokens >= 0 && n_heads > 0 && n_heads % c.n_kv_heads == 0 && n_heads / c.n_kv_heads <= 16;
 }
 
+// Chunks of at most 64 rows on average, over tables that hold 1024 positions or more
+// (the lengths themselves are on the device).  Both ways' times, few and many rows'
+// (us, 32 heads over 8 of 128 dims, fp32 rows over fp16): 16 chunks over 3400 positions
+// of 20 rows 61 and 73, of 64 rows 72 and 78, of 96 rows 94 and 83; of 20 rows over 256
+// positions 26 and 21, over 1024 35 and 37, over 4096 69 and 84.
+bool is_few(const ChunkArgs& a) {
+    return (int64_t)a.n_tokens * a.group <= (int64_t)2 * kWaveRows * a.n && (int64_t)a.c.table_width * a.c.page_size >= 1024;
+}
+
 template <int HD, int DT, typename RT, bool FEW>
 hipError_t launch_chunk(ChunkArgs a, bool alone, hipStream_t st) {
     static LdsLimit limit;
     constexpr int waves = waves_of<HD, Kinds<DT, RT>::NP>();
-    const size_t lds = (size_t)tiles_bytes<HD, DT, waves>() + kPagesHeld * 4 + waves * kWaveRows * 8 + 64 * sizeof(Placed);
+    const size_t lds = (size_t)tiles_bytes<HD, DT, waves>() + kPagesHeld * 4 + waves * kWaveRows * sizeof(Sum) + 64 * sizeof(Placed);
     a.few = FEW;
     a.tokens = kWaveRows * (FEW ? 2 : waves) / a.group;
     a.parts = Kinds<DT, RT>::NP;
@@ -974,9 +1024,7 @@ hipError_t launch_chunk(ChunkArgs a, bool alone, hipStream_t st) {
 }
 template <int HD, int DT, typename RT>
 hipError_t launch_chunk(const ChunkArgs& a, bool alone, hipStream_t st) {
-    // (chunks of at most 64 rows on average)
-    return (int64_t)a.n_tokens * a.group <= (int64_t)2 * kWaveRows * a.n ? launch_chunk<HD, DT, RT, true>(a, alone, st)
-                                                                        : launch_chunk<HD, DT, RT, false>(a, alone, st);
+    return is_few(a) ? launch_chunk<HD, DT, RT, true>(a, alone, st) : launch_chunk<HD, DT, RT, false>(a, alone, st);
 }
 
 template <int HD>
@@ -1035,7 +1083,7 @@ int gsdh_paged_chunk_attention(void* stream, const gsdh_paged_cache* c, int laye
     a.groups = s.groups; a.slot_rows = s.slot_rows;
     char* ws = static_cast<char*>(workspace);
     a.joints = reinterpret_cast<Joint*>(ws + s.joints);
-    a.part_ml = reinterpret_cast<float*>(ws + s.ml);
+    a.part_sum = reinterpret_cast<Sum*>(ws + s.sums);
     a.part = reinterpret_cast<float*>(ws + s.part);
     // where no table holds more than an item that is not cut, nothing is joined
     const bool alone = (int64_t)c->table_width * c->page_size <= kWhole * kPos;

@@ -27,9 +27,23 @@ def space(c, n, tokens, heads):
     return D(np.full(c.lib.gsdh_paged_chunk_attention_workspace_bytes(c.at, n, tokens, heads), 0xA5, np.uint8))   # (may hold anything)
 
 
+FEW_ROWS, FEW_ROOM = 64, 1024   # mean rows of a chunk up to which, positions of a table from which on a call goes by few rows
+
+
+def few(c, q, seqs, starts):
+    """The same chunks, with padding behind them, as a call that goes by few rows."""
+    assert c.width * c.page >= FEW_ROOM
+    n = len(starts) - 1
+    seqs, starts = list(range(n) if seqs is None else seqs), list(starts)
+    more = -(-q.shape[0] * q.shape[1] // c.kv // FEW_ROWS) - n
+    return seqs + [-1] * max(more, 0), starts + [starts[-1]] * max(more, 0)
+
+
 def run_chunks(c, layer, q, rows, seqs, starts, scale, window=0, ws=None, stream=None, q_pad=0, out_pad=0, fill=7.0, repeat=1):
     """The call's rows [tokens, heads, hd] as float64; q holds values of the type."""
     from gsdlq import hip
+    if c.few_rows:
+        seqs, starts = few(c, q, seqs, starts)
     n, (tokens, heads, hd) = len(starts) - 1, q.shape
     w = heads * hd
     qs = np.zeros((tokens, w + q_pad), np.float32)
@@ -91,6 +105,9 @@ def check(got, want, rows, exact_dots=False):
     assert off.size == 0 or off.max() <= 1, (off.max(), np.argwhere((np.abs(got - want) > bound) & named[..., None])[:3].tolist())
 
 
-def chunk_cache(kind, lens, page, kv, hd, head_major, rng, values, layers=1, spare=5):
-    need = sum(-(-n // page) for n in lens)
-    return Cache(kind, layers, need + spare, page, kv, hd, head_major, len(lens), max(lens) // page + 2).fill(lens, rng, values)
+def chunk_cache(kind, lens, page, kv, hd, head_major, rng, values, layers=1, spare=5, few_rows=False):
+    """few_rows: its calls go by few rows, else by many where the tables hold less than 1024 positions."""
+    need, width = sum(-(-n // page) for n in lens), max(lens) // page + 2
+    c = Cache(kind, layers, need + spare, page, kv, hd, head_major, len(lens), max(width, -(-FEW_ROOM // page)) if few_rows else width)
+    c.few_rows = few_rows
+    return c.fill(lens, rng, values)

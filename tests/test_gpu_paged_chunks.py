@@ -43,14 +43,15 @@ def ragged(order=(10, 4, 8, 0, 9, 7, 6, 5, 3, 2, 1)):
     return seqs, starts
 
 
+@pytest.mark.parametrize("few_rows", [False, True])
 @pytest.mark.parametrize("kind,rows", TYPES)
 @pytest.mark.parametrize("heads,kv,hd,page,head_major", [(4, 2, 64, 8, False), (8, 2, 128, 16, True), (4, 4, 128, 128, False), (6, 2, 64, 32, True),
                                                          (16, 2, 256, 8, True), (16, 1, 128, 16, False), (1, 1, 64, 256, False), (7, 1, 128, 8, False)])
-def test_ragged_batch(lib, kind, rows, heads, kv, hd, page, head_major):
+def test_ragged_batch(lib, kind, rows, heads, kv, hd, page, head_major, few_rows):
     """Every length and chunk, padding, NaN wherever nobody wrote, padded strides."""
     banner(f"chunks {kind} {rows} {heads}/{kv}x{hd} page {page} {'head' if head_major else 'slot'}")
     rng = np.random.default_rng(heads * hd + page)
-    c = chunk_cache(kind, LENS, page, kv, hd, head_major, rng, grid, layers=2)
+    c = chunk_cache(kind, LENS, page, kv, hd, head_major, rng, grid, layers=2, few_rows=few_rows)
     seqs, starts = ragged()
     q, scale = grid(rng, (starts[-1] + 1, heads, hd)), 1.0 / float(np.sqrt(hd))
     got = run_chunks(c, 1, q, rows, seqs, starts, scale, q_pad=8, out_pad=16)
@@ -58,12 +59,13 @@ def test_ragged_batch(lib, kind, rows, heads, kv, hd, page, head_major):
     assert c.status() == 0
 
 
+@pytest.mark.parametrize("few_rows", [False, True])
 @pytest.mark.parametrize("kind,rows", TYPES)
 @pytest.mark.parametrize("window", [1, 7, 64, 65, 150, 100000])
-def test_window(lib, kind, rows, window):
+def test_window(lib, kind, rows, window, few_rows):
     banner(f"chunks {kind} {rows} window {window}")
     rng = np.random.default_rng(window)
-    c = chunk_cache(kind, LENS, 16, 2, 64, False, rng, grid)
+    c = chunk_cache(kind, LENS, 16, 2, 64, False, rng, grid, few_rows=few_rows)
     for s, n in enumerate(LENS):   # what the window leaves behind may hold anything
         gone = np.arange(max(0, n - NEW[s] + 1 - window))
         if len(gone):
@@ -94,14 +96,15 @@ def test_long_split_and_joined(lib, kind, rows, heads, kv, hd, lens, new):
         assert np.array_equal(got, run_chunks(c, 0, q, rows, None, starts, scale, ws=ws, repeat=2))
 
 
+@pytest.mark.parametrize("few_rows", [False, True])
 @pytest.mark.parametrize("kind,rows", TYPES)
 @pytest.mark.parametrize("hd", [64, 128, 256])
-def test_prompt(lib, kind, rows, hd):
+def test_prompt(lib, kind, rows, hd, few_rows):
     """A prompt from its first token on, and the same in two pieces."""
     banner(f"prompt {kind} {rows} hd {hd}")
     rng = np.random.default_rng(hd)
     m, heads, kv = 401, 4, 2
-    c = chunk_cache(kind, [m], 16, kv, hd, False, rng, normal)
+    c = chunk_cache(kind, [m], 16, kv, hd, False, rng, normal, few_rows=few_rows)
     q, scale = rounded(normal(rng, (m, heads, hd)), rows).astype(np.float32), 1.0 / float(np.sqrt(hd))
     want = attend_chunks(c, 0, q, [0], [0, m], np.float32(scale))
     got = run_chunks(c, 0, q, rows, [0], [0, m], scale)
@@ -115,14 +118,15 @@ def test_prompt(lib, kind, rows, hd):
     check(np.concatenate([first, rest]), want, rows)
 
 
+@pytest.mark.parametrize("few_rows", [False, True])
 @pytest.mark.parametrize("kind", ["f16", "bf16", "e4m3"])
 @pytest.mark.parametrize("hd", [64, 128])
-def test_one_token_is_decode(lib, kind, hd):
+def test_one_token_is_decode(lib, kind, hd, few_rows):
     """Chunks of one token against the decode attention, over the same cache and rows."""
     banner(f"one token {kind} hd {hd}")
     rng = np.random.default_rng(5)
     lens = [1, 63, 64, 65, 700]
-    c = chunk_cache(kind, lens, 16, 2, hd, False, rng, normal)
+    c = chunk_cache(kind, lens, 16, 2, hd, False, rng, normal, few_rows=few_rows)
     q, starts, seqs = normal(rng, (5, 8, hd)), list(range(6)), [4, 2, 0, 1, 3]
     got = run_chunks(c, 0, q, "f32", seqs, starts, 0.125)
     want = attend_chunks(c, 0, q, seqs, starts, 0.125)
@@ -130,14 +134,15 @@ def test_one_token_is_decode(lib, kind, hd):
     check(c.run_attend(0, q, seqs, 0.125).astype(np.float64), want, "f32")
 
 
+@pytest.mark.parametrize("few_rows", [False, True])
 @pytest.mark.parametrize("kind,rows", TYPES)
-def test_every_position_counts(lib, kind, rows):
+def test_every_position_counts(lib, kind, rows, few_rows):
     """One position that outweighs all others: the rows from it on give its V row, those before it none of it."""
     rng = np.random.default_rng(3)
     n, m, hd = 1000, 200, 64
     places = [0, 1, 31, 32, 63, 64, 127, 500, 799, 800, 801, 831, 832, 863, 895, 896, 998, 999]
     banner(f"chunks {kind} {rows}: {len(places)} places of {n}")
-    c = chunk_cache(kind, [n], 8, 1, hd, False, rng, lambda r, s: grid(r, s) * 0)
+    c = chunk_cache(kind, [n], 8, 1, hd, False, rng, lambda r, s: grid(r, s) * 0, few_rows=few_rows)
     c.set_values(1, 0, 0, np.arange(n), grid(rng, (n, 1, hd)))
     q = np.zeros((m, 2, hd), np.float32)
     q[:, :, 5] = 20.0
@@ -150,10 +155,11 @@ def test_every_position_counts(lib, kind, rows):
         check(got, attend_chunks(c, 0, q, [0], [0, m], 1.0), rows, exact_dots=True)
 
 
+@pytest.mark.parametrize("few_rows", [False, True])
 @pytest.mark.parametrize("kind,rows", TYPES)
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("window", [0, 70])
-def test_what_a_row_does_not_see(lib, kind, rows, bad, window):
+def test_what_a_row_does_not_see(lib, kind, rows, bad, window, few_rows):
     """A NaN or an infinity in V or K: rows that do not see it are as without it, those that do are not finite in
     that dim (V) or of that KV head (K)."""
     if kind == "e4m3" and not np.isnan(bad):
@@ -161,7 +167,7 @@ def test_what_a_row_does_not_see(lib, kind, rows, bad, window):
     banner(f"unseen {kind} {rows} {bad} window {window}")
     rng = np.random.default_rng(11)
     n, m, kv, heads, hd, at, dim = 300, 150, 2, 4, 64, 230, 37
-    c = chunk_cache(kind, [n], 16, kv, hd, False, rng, grid)
+    c = chunk_cache(kind, [n], 16, kv, hd, False, rng, grid, few_rows=few_rows)
     q = grid(rng, (m, heads, hd))
     want = attend_chunks(c, 0, q, [0], [0, m], 0.1, window)
     clean = run_chunks(c, 0, q, rows, [0], [0, m], 0.1, window)
@@ -188,14 +194,15 @@ def test_what_a_row_does_not_see(lib, kind, rows, bad, window):
     c.upload()
 
 
+@pytest.mark.parametrize("few_rows", [False, True])
 @pytest.mark.parametrize("kind,rows", TYPES)
-def test_no_weight_at_all(lib, kind, rows):
+def test_no_weight_at_all(lib, kind, rows, few_rows):
     """Scores that are all -inf are NaN, one that is not takes all; NaN in q stays with its row and head."""
     if kind == "e4m3":
         pytest.skip("e4m3 has no infinities")
     rng = np.random.default_rng(2)
     n, m, hd = 100, 100, 64
-    c = chunk_cache(kind, [n], 16, 1, hd, False, rng, grid)
+    c = chunk_cache(kind, [n], 16, 1, hd, False, rng, grid, few_rows=few_rows)
     k = np.zeros((n, 1, hd), np.float32)
     k[:50, 0, 3] = -np.inf
     c.set_values(0, 0, 0, np.arange(n), k)
@@ -212,14 +219,15 @@ def test_no_weight_at_all(lib, kind, rows):
     assert np.abs(got[ok] - want[:, None]).max() <= tol
 
 
+@pytest.mark.parametrize("few_rows", [False, True])
+@pytest.mark.parametrize("n,m", [(200, 70), (6000, 3)])
 @pytest.mark.parametrize("rows", ["f32", "bf16"])
-def test_the_ends_of_bf16(lib, rows):
+def test_the_ends_of_bf16(lib, rows, n, m, few_rows):
     """Finite rows over all of the type's range give finite results; scores far beyond fp32 after scaling keep the
-    largest weight at 1; a scale of 0 weighs all alike."""
-    rng = np.random.default_rng(4)
-    n, m, hd = 200, 70, 64
+    largest weight at 1, within a block and over many; a scale of 0 weighs all alike."""
+    rng, hd = np.random.default_rng(4), 64
     huge = 2.0 ** 127
-    c = chunk_cache("bf16", [n], 16, 1, hd, False, rng, grid)
+    c = chunk_cache("bf16", [n], 16, 1, hd, False, rng, grid, few_rows=few_rows)
     v = np.sign(grid(rng, (n, 1, hd)) + 0.1) * huge
     c.set_values(1, 0, 0, np.arange(n), v)
     k = grid(rng, (n, 1, hd)) * np.float32(2.0 ** 120)
@@ -231,7 +239,7 @@ def test_the_ends_of_bf16(lib, rows):
         assert np.isfinite(got).all()
         pos = n - m + np.arange(m)
         kk, vv = c.values(0, 0, 0, np.arange(n))[:, 0] / 2.0 ** 120, c.values(1, 0, 0, np.arange(n))[:, 0]
-        for t in (0, 1, 33, m - 1):
+        for t in sorted({0, 1, min(33, m - 1), m - 1}):
             x = kk[:pos[t] + 1] @ (q[t, 0].astype(np.float64) / 2.0 ** 120)
             if scale == 0:
                 want = vv[:pos[t] + 1].mean(0)
@@ -242,10 +250,11 @@ def test_the_ends_of_bf16(lib, rows):
             assert np.abs(got[t, 0] - want).max() <= tol, (scale, t)
 
 
-def test_scales(lib):
+@pytest.mark.parametrize("few_rows", [False, True])
+def test_scales(lib, few_rows):
     """Negative, zero and large scales over fp16, fp32 and fp16 rows."""
     rng = np.random.default_rng(8)
-    c = chunk_cache("f16", [150], 16, 2, 64, False, rng, grid)
+    c = chunk_cache("f16", [150], 16, 2, 64, False, rng, grid, few_rows=few_rows)
     q = grid(rng, (60, 4, 64))
     for rows in ("f32", "f16"):
         for scale in (-0.3, 0.0, -0.0, 40.0, 1e-30):
@@ -253,12 +262,13 @@ def test_scales(lib):
             check(got, attend_chunks(c, 0, q, [0], [0, 60], float(np.float32(scale))), rows, exact_dots=True)
 
 
-def test_bad_indices(lib):
+@pytest.mark.parametrize("few_rows", [False, True])
+def test_bad_indices(lib, few_rows):
     """Left out or NaN, reported, and nothing else touched."""
     from gsdlq import hip
     rng = np.random.default_rng(1)
     lens = [100, 50, 40, 30, 200, 64]
-    c = chunk_cache("f16", lens, 16, 2, 64, False, rng, grid)
+    c = chunk_cache("f16", lens, 16, 2, 64, False, rng, grid, few_rows=few_rows)
     q = grid(rng, (60, 4, 64))
 
     def run(seqs, starts, **kw):
@@ -315,12 +325,13 @@ def test_one_row_of_q_for_all(lib):
     check(H(out, np.float32, 30 * 128).reshape(30, 2, 64).astype(np.float64), attend_chunks(c, 0, q, [0], [0, 30], np.float32(0.2)), "f32", True)
 
 
-def test_replayed_while_sequences_grow(lib):
+@pytest.mark.parametrize("few_rows", [False, True])
+def test_replayed_while_sequences_grow(lib, few_rows):
     """A captured call reads lengths, starts and lists when it runs; every replay against the definition, eager work between."""
     import ctypes
     rng = np.random.default_rng(9)
     lens = [500, 40, 300]
-    c = chunk_cache("f16", lens, 16, 2, 64, False, rng, grid)
+    c = chunk_cache("f16", lens, 16, 2, 64, False, rng, grid, few_rows=few_rows)
     tokens, heads = 50, 4
     q = grid(rng, (tokens, heads, 64))
     dq, out, ws = D(q), D(np.zeros((tokens, heads * 64), np.float32)), space(c, 3, tokens, heads)
@@ -377,12 +388,13 @@ def test_two_streams(lib):
         lib.gsdh_stream_destroy(st)
 
 
-def test_many_chunks(lib):
+@pytest.mark.parametrize("few_rows", [False, True])
+def test_many_chunks(lib, few_rows):
     """More chunks than a wave has lanes, most of them of one token."""
     banner("200 chunks")
     rng = np.random.default_rng(12)
     lens = [1 + (37 * i) % 90 for i in range(200)]
-    c = chunk_cache("f16", lens, 8, 1, 64, False, rng, grid)
+    c = chunk_cache("f16", lens, 8, 1, 64, False, rng, grid, few_rows=few_rows)
     new = [1 if i % 9 else min(n, 30) for i, n in enumerate(lens)]
     starts = np.cumsum([0] + new).tolist()
     q = grid(rng, (starts[-1], 2, 64))
