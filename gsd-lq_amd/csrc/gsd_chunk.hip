@@ -167,6 +167,14 @@ __device__ __forceinline__ float part_weight(const Sum& s, float top, float nb) 
     return __builtin_amdgcn_exp2f(is_steep(top, s.to_log2) || is_steep(s.m, s.to_log2) ? (s.m - top) * s.to_log2 : nb - s.nb);
 }
 
+// What the first wave has found for the block.
+struct Plan {
+    u64 size, lo, hi;   // of spans; the block's
+    u64 base;           // cost before the next 64 chunks
+    u64 todo;           // which of the 64 placed chunks have something in it
+    int last;           // no more after these
+};
+
 // What a block does of an item.
 struct Item {
     int seq;
@@ -293,6 +301,7 @@ chunk_attn_kernel(const ChunkArgs a) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     int* const pages = reinterpret_cast<int*>(lds + BUF);
     Sum* const wave_sum = reinterpret_cast<Sum*>(lds + BUF + kPagesHeld * 4);   // [NW][32]
+    Plan* const plan = reinterpret_cast<Plan*>(lds + BUF + kPagesHeld * 4 + NW * kWaveRows * sizeof(Sum) + 64 * sizeof(Placed));
     Placed* const placed = reinterpret_cast<Placed*>(lds + BUF + kPagesHeld * 4 + NW * kWaveRows * sizeof(Sum));   // [64]
     const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_byte*)lds;
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, hi = lane >> 5;
@@ -329,7 +338,7 @@ chunk_attn_kernel(const ChunkArgs a) {
         // q's operand
         u32x4v q[KS][NP];
         float to_log2 = 1.f;
-        typedef RT r8 __attribute__((ext_vector_type(8)));
+        typedef RT r8 __attribute__((ext_vector_type(8), aligned(16)));
         r8 qrow[KS];   // as it comes: asked for before the pages are, used once the first tiles are asked for
         if (live) {
             const RT* src = static_cast<const RT*>(a.q) + (int64_t)(it.token + tok) * a.q_stride + (int64_t)qh * HD + 8 * hi;
@@ -370,8 +379,8 @@ chunk_attn_kernel(const ChunkArgs a) {
                     }
                 }
             }
-            // (a scale of 0 stays above it: a masked -inf times it is -inf)
-            to_log2 = fmaxf(to_log2, FLT_TRUE_MIN);
+            // (a scale of 0 stays above it: a masked -inf times it is -inf; one of NaN makes NaN)
+            if (to_log2 < FLT_TRUE_MIN) to_log2 = FLT_TRUE_MIN;
         };
         // P as 2^14 times itself: what lies below fp16's normal range stays exact longer;
         // bf16: over a power of two that is above the number of positions, so that no
@@ -843,27 +852,42 @@ chunk_attn_kernel(const ChunkArgs a) {
     // -- which items --------------------------------------------------------
     // The chunks' costs lie end to end, and each group of blocks, one per KV
     // head, takes a span of `size` of them: all have as much to do whatever the
-    // lengths are.  Every wave finds the block's span by itself.
-    u64 mine = 0;
-    Chunk k{};
-    for (int i = lane; i < a.n; i += 64) {
-        k = chunk_of(a, i);
-        mine += cost_before(a, k, k.items);
-    }
-    const u64 total = readlane64(wave_scan64(mine), 63);
-    const u64 size = max((total + a.groups - 1) / a.groups, (u64)kLeastSpan);
-    const u64 lo = min((u64)grp * size, total), span_hi = min(lo + size, total);
+    // lengths are.  The first wave finds the block's chunks, 64 at a time; the others
+    // take them from LDS (what each read for itself could differ, and so the barriers
+    // that they meet at, if somebody changed the lengths meanwhile).
     Joint joint{0, 0, 0};
-    u64 base = 0;
-    for (int c0 = 0; c0 < a.n && base < span_hi; c0 += 64) {
-        if (a.n > 64) k = c0 + lane < a.n ? chunk_of(a, c0 + lane) : Chunk{};   // (up to 64 are at hand)
-        const u64 cost = cost_before(a, k, k.items), incl = wave_scan64(cost), at = base + incl - cost;
-        base += readlane64(incl, 63);
-        u64 todo = __ballot(cost > 0 && at < span_hi && at + cost > lo);
-        if (!todo) continue;
-        __syncthreads();   // (what lay there is read; all waves write the same)
-        placed[lane] = Placed{k, at};
+    for (int c0 = 0;; c0 += 64) {
+        if (wid == 0) {
+            Chunk k{};
+            if (c0 == 0) {
+                u64 mine = 0;
+                for (int i = lane; i < a.n; i += 64) {
+                    k = chunk_of(a, i);
+                    mine += cost_before(a, k, k.items);
+                }
+                const u64 total = readlane64(wave_scan64(mine), 63);
+                const u64 size = max((total + a.groups - 1) / a.groups, (u64)kLeastSpan);
+                const u64 lo = min((u64)grp * size, total);
+                plan->size = size;
+                plan->lo = lo;
+                plan->hi = min(lo + size, total);
+                plan->base = 0;
+            }
+            if (a.n > 64) k = c0 + lane < a.n ? chunk_of(a, c0 + lane) : Chunk{};   // (up to 64 are at hand)
+            const u64 lo = plan->lo, end = plan->hi;
+            u64 base = plan->base;
+            const u64 cost = cost_before(a, k, k.items), incl = wave_scan64(cost), at = base + incl - cost;
+            base += readlane64(incl, 63);
+            const u64 mine = __ballot(cost > 0 && at < end && at + cost > lo);
+            placed[lane] = Placed{k, at};
+            plan->todo = mine;
+            plan->base = base;
+            plan->last = c0 + 64 >= a.n || base >= end;
+        }
         __syncthreads();
+        const u64 size = readlane64(plan->size, 0), lo = readlane64(plan->lo, 0), span_hi = readlane64(plan->hi, 0);
+        u64 todo = readlane64(plan->todo, 0);
+        const bool last = __builtin_amdgcn_readfirstlane(plan->last) != 0;
         while (todo) {
             const int src = __builtin_ctzll(todo);
             todo &= todo - 1;
@@ -906,13 +930,15 @@ chunk_attn_kernel(const ChunkArgs a) {
                     it.t1 = it.t0 + c_hi;
                     it.t0 += c_lo;
                     it.split = (int)((u64)grp - from);
-                    it.splits = (int)(to - from) + 1;
+                    it.splits = (int)(min(to, (u64)a.groups - 1) - from) + 1;
                     if (it.split == 0 && it.splits > 1) joint = Joint{it.splits, it.token, it.rows};
                 }
                 if (it.bad) bad_item(it);
                 else run_item(it);
             }
         }
+        if (last) break;
+        __syncthreads();   // (the plan is read)
     }
     if (tid == 0) a.joints[(size_t)grp * nkv + head] = joint;
 }
@@ -995,7 +1021,7 @@ ChunkSpace chunk_space(const gsdh_paged_cache& c, int n_tokens, int n_heads, int
 }
 
 bool chunk_shape(const gsdh_paged_cache& c, int n, int n_tokens, int n_heads) {
-    return n >= 0 && n_tokens >= 0 && n_heads > 0 && n_heads % c.n_kv_heads == 0 && n_heads / c.n_kv_heads <= 16;
+    return n >= 0 && n <= 1 << 20 && n_tokens >= 0 && n_tokens <= 1 << 30 && n_heads > 0 && n_heads % c.n_kv_heads == 0 && n_heads / c.n_kv_heads <= 16;
 }
 
 // Chunks of at most 64 rows on average, over tables that hold 1024 positions or more
@@ -1011,7 +1037,7 @@ template <int HD, int DT, typename RT, bool FEW>
 hipError_t launch_chunk(ChunkArgs a, bool alone, hipStream_t st) {
     static LdsLimit limit;
     constexpr int waves = waves_of<HD, Kinds<DT, RT>::NP>();
-    const size_t lds = (size_t)tiles_bytes<HD, DT, waves>() + kPagesHeld * 4 + waves * kWaveRows * sizeof(Sum) + 64 * sizeof(Placed);
+    const size_t lds = (size_t)tiles_bytes<HD, DT, waves>() + kPagesHeld * 4 + waves * kWaveRows * sizeof(Sum) + 64 * sizeof(Placed) + sizeof(Plan);
     a.few = FEW;
     a.tokens = kWaveRows * (FEW ? 2 : waves) / a.group;
     a.parts = Kinds<DT, RT>::NP;
@@ -1061,7 +1087,7 @@ int gsdh_paged_chunk_attention(void* stream, const gsdh_paged_cache* c, int laye
     if ((dtype == GSDH_ROWS_F16 && c->dtype == GSDH_KV_BF16) || (dtype == GSDH_ROWS_BF16 && c->dtype == GSDH_KV_F16))
         return fail(-1, "%s: rows of 16 bits are of the cache's type (or over an e4m3 cache)", who);
     if (!chunk_shape(*c, n, n_tokens, n_heads))
-        return fail(-1, "%s: %d chunks, %d tokens, %d heads over %d KV heads (1..16 query heads per KV head)", who, n, n_tokens, n_heads,
+        return fail(-1, "%s: %d chunks (at most 2^20), %d tokens (2^30), %d heads over %d KV heads (1..16 query heads per KV head)", who, n, n_tokens, n_heads,
                     c->n_kv_heads);
     if (n > c->n_seqs && !seqs) return fail(-1, "%s: %d chunks, %d sequences", who, n, c->n_seqs);
     if (window < 0) return fail(-1, "%s: window %d", who, window);

@@ -295,7 +295,7 @@ int gsdh_rope_rows(void* stream, const gsdh_rope* r, const void* x, int dtype, i
     if (head_dim < 8 || head_dim > 1024 || head_dim % 8) return fail(-1, "%s: head_dim %d is not a multiple of 8 in 8..1024", who, head_dim);
     const int rc = check_rope(r, head_dim, dtype, who);
     if (rc) return rc;
-    if (n < 0 || n_heads <= 0 || n_heads > 16384) return fail(-1, "%s: %d tokens of %d heads", who, n, n_heads);
+    if (n < 0 || n > 1 << 30 || n_heads <= 0 || n_heads > 16384) return fail(-1, "%s: %d tokens of %d heads", who, n, n_heads);
     if (n == 0) return 0;
     if (!x || !out || !positions) return fail(-1, "%s: null buffer", who);
     const int64_t width = (int64_t)n_heads * head_dim;
@@ -320,7 +320,7 @@ int gsdh_paged_rope_append(void* stream, const gsdh_paged_cache* c, int layer, c
     rc = check_rope(r, c->head_dim, dtype, who);
     if (rc) return rc;
     if (layer < 0 || layer >= c->n_layers) return fail(-1, "%s: layer %d outside 0..%d", who, layer, c->n_layers - 1);
-    if (n < 0 || n_heads <= 0 || n_heads > 16384) return fail(-1, "%s: %d tokens of %d heads", who, n, n_heads);
+    if (n < 0 || n > 1 << 30 || n_heads <= 0 || n_heads > 16384) return fail(-1, "%s: %d tokens of %d heads", who, n, n_heads);
     if (n == 0) return 0;
     if (!q || !k || !v || !q_out || !seqs || !positions) return fail(-1, "%s: null buffer", who);
     const int64_t width = (int64_t)n_heads * c->head_dim;

@@ -292,7 +292,7 @@ enum { GSDH_ROWS_F32 = 0, GSDH_ROWS_F16 = 1, GSDH_ROWS_BF16 = 2 };
  * so.  What a row does not see never reaches it, NaN and infinities included; what it
  * sees acts as in gsdh_paged_attention, an infinity in V as a NaN where a tile has a
  * mask.  Rows that two chunks name hold either's.
- * n_heads / n_kv_heads 1 .. 16; rows 16-byte aligned, strides in elements, of whole
+ * n <= 2^20, n_tokens <= 2^30; n_heads / n_kv_heads 1 .. 16; rows 16-byte aligned, strides in elements, of whole
  * 16 bytes, at least n_heads * head_dim for out.  workspace:
  * gsdh_paged_chunk_attention_workspace_bytes(c, n, n_tokens, n_heads) bytes (0 for an
  * invalid shape), 16-byte aligned; what it holds before a call does not matter, and

@@ -252,7 +252,7 @@ def test_the_ends_of_bf16(lib, rows, n, m, few_rows):
 
 @pytest.mark.parametrize("few_rows", [False, True])
 def test_scales(lib, few_rows):
-    """Negative, zero and large scales over fp16, fp32 and fp16 rows."""
+    """Negative, zero and large scales over fp16, fp32 and fp16 rows; one of NaN makes NaN."""
     rng = np.random.default_rng(8)
     c = chunk_cache("f16", [150], 16, 2, 64, False, rng, grid, few_rows=few_rows)
     q = grid(rng, (60, 4, 64))
@@ -260,6 +260,7 @@ def test_scales(lib, few_rows):
         for scale in (-0.3, 0.0, -0.0, 40.0, 1e-30):
             got = run_chunks(c, 0, q, rows, [0], [0, 60], scale)
             check(got, attend_chunks(c, 0, q, [0], [0, 60], float(np.float32(scale))), rows, exact_dots=True)
+        assert np.isnan(run_chunks(c, 0, q, rows, [0], [0, 60], np.nan)).all()
 
 
 @pytest.mark.parametrize("few_rows", [False, True])

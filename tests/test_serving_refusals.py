@@ -57,7 +57,7 @@ def test_caches(lib, other, text):
 @pytest.mark.parametrize("other,text", [
     (dict(layer=2), "layer 2"), (dict(layer=-1), "layer -1"), (dict(dtype=3), "type 3"), (dict(dtype=-1), "type -1"), (dict(dtype=2), "cache's type"),
     (dict(heads=3), "3 heads"), (dict(heads=34, q_stride=4096, out_stride=4096), "34 heads"), (dict(heads=0), "0 heads"), (dict(n=-1), "-1 chunks"),
-    (dict(tokens=-1), "-1 tokens"), (dict(seqs=None, n=5), "5 chunks, 4 sequences"), (dict(window=-1), "window -1"), (dict(q=None), "rows of q"),
+    (dict(tokens=-1), "-1 tokens"), (dict(tokens=(1 << 30) + 1), "1073741825 tokens"), (dict(n=(1 << 20) + 1), "1048577 chunks"), (dict(seqs=None, n=5), "5 chunks, 4 sequences"), (dict(window=-1), "window -1"), (dict(q=None), "rows of q"),
     (dict(q=BUF + 4), "rows of q"), (dict(q_stride=258), "rows of q"), (dict(q_stride=-256), "rows of q"), (dict(out=BUF + 8), "rows of q"),
     (dict(out_stride=252), "at least 256"), (dict(dtype=1, q_stride=260), "rows of q"), (dict(starts=None), "null starts"),
     (dict(ws=None), "0 bytes of workspace"), (dict(ws_bytes=100), "100 bytes of workspace"), (dict(ws=BUF + 8), "not 16-byte aligned")])
@@ -90,7 +90,7 @@ def test_chunk_workspace(lib):
 @pytest.mark.parametrize("other,text", [
     (dict(r=rope(rotary_dim=0)), "rotary_dim 0"), (dict(r=rope(rotary_dim=7)), "rotary_dim 7"), (dict(r=rope(rotary_dim=66)), "rotary_dim 66"),
     (dict(r=rope(freqs=None)), "frequencies"), (dict(r=rope(freqs=BUF + 4)), "frequencies"), (dict(dtype=3), "type 3"), (dict(n=-1), "-1 tokens"),
-    (dict(heads=0), "0 heads"), (dict(heads=16385), "16385 heads")])
+    (dict(n=(1 << 30) + 1), "1073741825 tokens"), (dict(heads=0), "0 heads"), (dict(heads=16385), "16385 heads")])
 def test_rotations(lib, other, text):
     for call in (rows, append):
         with pytest.raises(hip.HipError, match=text):
