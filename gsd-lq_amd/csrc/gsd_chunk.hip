@@ -34,7 +34,9 @@ static_assert(kCost >= 2 * kPos * 16 && kLeastSpan >= kPos * 24, "an item's tile
 constexpr int kPagesHeld = 256;      // page indices in LDS
 constexpr int kMostGroups = 256;     // of blocks, one per KV head
 constexpr int kJoinRows = 8;         // rows that a block joins at a time
-constexpr int kJoinBlocks = 4;       // of an item: four fill the chip once, of 32 most came and went for nothing (8 us)
+// blocks that join an item: four of few rows fill the chip once (of 32 most came and went for nothing: 8 us,
+// 5 with four), 256 rows are read by more (22 us with four)
+constexpr int kJoinFew = 4, kJoinMany = 16;
 
 // ---------------------------------------------------------------------------
 //   x_tp = sm_scale q_t.K_p  (p <= the token's position, and within the window),
@@ -79,6 +81,7 @@ struct ChunkArgs {
     int64_t q_stride, out_stride;
     int layer, n, n_tokens, group, window, groups, slot_rows;
     int tokens, parts;   // of an item; of a row's 32-bit values
+    int join_blocks;
     bool few;
     float scale;
 };
@@ -283,9 +286,9 @@ constexpr unsigned tiles_bytes() {
 // both ways' times); in one kernel both had registers spilled in their loops.
 //
 // Bound by the matrix cores for prompts: 2048 tokens of 32 heads over 8 of 128 dims at the
-// end of 32768 positions, bf16, 1064 us, 1.0 PFLOP/s of products (a library's product of
+// end of 32768 positions, bf16, 1079 us, 1.0 PFLOP/s of products (a library's product of
 // 8192^3 gets 1.2 on the same card, whose clock falls under both: 1.8 GHz in this
-// kernel); 4096 tokens of fp32 rows over fp16 293 us, 0.94 PFLOP/s of products, two for
+// kernel); 4096 tokens of fp32 rows over fp16 284 us, 0.97 PFLOP/s of products, two for
 // each.  By memory for few rows: 16 chunks of 5 tokens over up to 8191 positions (199 MB)
 // 68 us, of which the stream is 36.
 template <int HD, int DT, typename RT, bool FEW>
@@ -943,18 +946,18 @@ chunk_attn_kernel(const ChunkArgs a) {
     if (tid == 0) a.joints[(size_t)grp * nkv + head] = joint;
 }
 
-// The parts of the items that several blocks shared: kJoinBlocks blocks for an
+// The parts of the items that several blocks shared: join_blocks blocks for an
 // item (at most places there is none), kJoinRows rows at a time.  The weights of all
 // parts first, in LDS, then their outputs, eight loads under way at a time.
 template <int HD, typename RT>
 __global__ void __launch_bounds__(256) chunk_join_kernel(const ChunkArgs a) {
     __shared__ float weight[kJoinRows][kMostGroups], inv[kJoinRows];
-    const int nkv = a.c.n_kv_heads, place = (int)(blockIdx.x / kJoinBlocks), head = place % nkv, grp = place / nkv, G = a.group;
+    const int nkv = a.c.n_kv_heads, place = (int)(blockIdx.x / (unsigned)a.join_blocks), head = place % nkv, grp = place / nkv, G = a.group;
     const Joint j = a.joints[place];
     if (j.parts == 0) return;
     const float vscale = a.c.dtype == GSDH_KV_E4M3 ? a.c.v_scale[a.layer * nkv + head] : 1.f;
     auto slot_of = [&](int k) { return 2 * ((size_t)(grp + k) * nkv + head) + (k == 0); };
-    for (int r0 = (int)(blockIdx.x % kJoinBlocks) * kJoinRows; r0 < j.rows; r0 += kJoinBlocks * kJoinRows) {
+    for (int r0 = (int)(blockIdx.x % (unsigned)a.join_blocks) * kJoinRows; r0 < j.rows; r0 += a.join_blocks * kJoinRows) {
         const int rows = min(kJoinRows, j.rows - r0);
         const int r = threadIdx.x / 32, lane = threadIdx.x % 32;   // 32 threads per row
         // (the first 32 parts' sums are loaded once)
@@ -1039,13 +1042,14 @@ hipError_t launch_chunk(ChunkArgs a, bool alone, hipStream_t st) {
     constexpr int waves = waves_of<HD, Kinds<DT, RT>::NP>();
     const size_t lds = (size_t)tiles_bytes<HD, DT, waves>() + kPagesHeld * 4 + waves * kWaveRows * sizeof(Sum) + 64 * sizeof(Placed) + sizeof(Plan);
     a.few = FEW;
+    a.join_blocks = FEW ? kJoinFew : kJoinMany;
     a.tokens = kWaveRows * (FEW ? 2 : waves) / a.group;
     a.parts = Kinds<DT, RT>::NP;
     const hipError_t e = raise_lds_limit(limit, reinterpret_cast<const void*>(chunk_attn_kernel<HD, DT, RT, FEW>), lds);
     if (e != hipSuccess) return e;
     const unsigned places = (unsigned)(a.groups * a.c.n_kv_heads);
     hipLaunchKernelGGL((chunk_attn_kernel<HD, DT, RT, FEW>), dim3(places), dim3(64 * waves), lds, st, a);
-    if (!alone) hipLaunchKernelGGL((chunk_join_kernel<HD, RT>), dim3(places * kJoinBlocks), dim3(256), 0, st, a);
+    if (!alone) hipLaunchKernelGGL((chunk_join_kernel<HD, RT>), dim3(places * (unsigned)a.join_blocks), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 template <int HD, int DT, typename RT>
