@@ -30,7 +30,7 @@ constexpr int kLeastSpan = 2048;     // the least a block takes
 __device__ __forceinline__ int cost_of_rows(bool few, int rows, int parts) {
     return few ? (rows <= 32 ? 4 : max(4, 3 * parts)) : rows <= 128 ? 6 * parts : 8 * parts;
 }
-static_assert(kCost >= 2 * kPos * 16 && kLeastSpan >= kPos * 24, "an item's tiles lie within its cost, and every span inside it has one");
+static_assert(kCost >= 2 * kPos * 24 && kLeastSpan >= kPos * 24, "an item's tiles lie within its cost, and every span inside it has one");
 constexpr int kPagesHeld = 256;      // page indices in LDS
 constexpr int kMostGroups = 256;     // of blocks, one per KV head
 constexpr int kJoinRows = 8;         // rows that a block joins at a time

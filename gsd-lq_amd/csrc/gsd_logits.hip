@@ -10,6 +10,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kSeg = 4096;               // logits of a block, a word of LDS each
 constexpr int kMaxVocab = 1 << 24;
+constexpr int kMaxList = 1 << 30;         // tokens of a row's history; biases
 constexpr int kHeld = 2;                 // times four tokens of the history that a thread has on their way
 constexpr uint32_t kInPrompt = 1u << 31;   // in a logit's word, beside how often the answer has it
 
@@ -45,7 +46,8 @@ struct Word {
 // (23 MB) 13.5 us; then by memory: 256 rows of 32768 fp32 logits (48 MB) 16.0 us, 3.0
 // TB/s.  (A token of the history per load, after the logits: 19.0 and 17.0 us; counts and
 // places in LDS of their own leave room for 5 blocks per CU in place of 8: 16.3 and 21.4;
-// 16 tokens of a thread on their way in place of 8: 13.8 and 18.7.)
+// 16 tokens of a thread on their way in place of 8: 13.8 and 18.7; blocks of 1024 threads
+// and 16384 logits, which read a history less often: 12.5, but 16.4 and 7.3 for one row.)
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 8) rules_kernel(const RulesArgs a) {
     typedef Word<T> W;
@@ -228,6 +230,8 @@ int gsdh_logits_adjust(void* stream, const gsdh_logit_rules* r, const void* x, i
     if (r->history && (!r->history_lens || r->history_width < 0))
         return fail(-1, "%s: a history needs lengths and a width, has %d", who, r->history_width);
     if (!r->history && (r->repetition || r->frequency || r->presence)) return fail(-1, "%s: penalties need a history", who);
+    if (r->history && r->history_width > kMaxList) return fail(-1, "%s: a history of %d tokens (at most 2^30)", who, r->history_width);
+    if (r->bias_starts && r->n_bias > kMaxList) return fail(-1, "%s: %d biases (at most 2^30)", who, r->n_bias);
     if (r->bias_starts ? !r->bias_ids || !r->bias || r->n_bias < 0 : r->bias_ids || r->bias)
         return fail(-1, "%s: bias_starts, bias_ids and bias go together", who);
     if (r->masks ? !r->mask_rows || r->n_masks < 0 || (int64_t)r->mask_words * 32 < vocab : r->mask_rows != nullptr)

@@ -455,7 +455,8 @@ typedef struct gsdh_logit_rules {
 /* n rows of `vocab` logits at x + r * x_stride (elements of `dtype`, GSDH_LOGITS_*)
  * to out + r * out_stride; out may be x with the same stride (logits that do not
  * change are then neither read nor written), and must not overlap it otherwise.
- * vocab <= 2^24.  No workspace; equal calls give equal bits. */
+ * vocab <= 2^24, history_width and n_bias <= 2^30.  No workspace; equal calls give
+ * equal bits. */
 int gsdh_logits_adjust(void* stream, const gsdh_logit_rules* r, const void* x, int dtype, int64_t x_stride,
                        int n, int vocab, void* out, int64_t out_stride);
 

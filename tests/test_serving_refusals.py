@@ -120,6 +120,7 @@ B = BUF
     (dict(dtype=3), "type 3"), (dict(n=-1), "-1 rows"), (dict(vocab=0), "0 logits"), (dict(vocab=(1 << 24) + 1, xs=1 << 25, os_=1 << 25), "at most"),
     (dict(os_=99), "99 apart"), (dict(xs=-1), "apart"), (dict(out=BUF, xs=104, os_=108), "apart"), (dict(x=None), "null"), (dict(x=BUF + 2), "not aligned"),
     (dict(dtype=1, out=BUF + 65537), "not aligned"), (dict(history=B, history_width=4), "lengths"), (dict(history=B, history_lens=B, history_width=-1), "width"),
+    (dict(history=B, history_lens=B, history_width=(1 << 30) + 1), "1073741825 tokens"), (dict(bias_starts=B, bias_ids=B, bias=B, n_bias=(1 << 30) + 1), "1073741825 biases"),
     (dict(repetition=B), "need a history"), (dict(presence=B), "need a history"), (dict(bias_starts=B, bias_ids=B), "go together"),
     (dict(bias_starts=B, bias=B), "go together"), (dict(bias=B), "go together"), (dict(bias_ids=B), "go together"),
     (dict(bias_starts=B, bias_ids=B, bias=B, n_bias=-1), "go together"), (dict(masks=B, mask_words=4, n_masks=1), "mask_rows"),
