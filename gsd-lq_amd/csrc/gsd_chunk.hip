@@ -64,7 +64,8 @@ struct Joint {   // of an item that several blocks share, at its first one's pla
 };
 
 // A row's weights so far: the largest score, unscaled, their sum, and what they are
-// relative to: 2^(x to_log2 + nb), or (m to_log2 beyond 2^20) the largest's.
+// relative to: 2^(x to_log2 + nb), or (m to_log2 beyond 2^20) the largest's.  A negative
+// to_log2: the factor is -2^127 times it, which fp32 does not hold.
 struct __attribute__((aligned(16))) Sum {
     float m, l, nb, to_log2;
 };
@@ -162,13 +163,16 @@ struct Placed {
 };
 
 constexpr float kSteep = 1048576.f;   // exponents of 2 beyond which a rounded product would not do
-__device__ __forceinline__ bool is_steep(float m, float to_log2) { return !(fabsf(m * to_log2) < kSteep); }
+__device__ __forceinline__ bool is_steep(float m, float to_log2) { return to_log2 < 0.f || !(fabsf(m * to_log2) < kSteep); }
+// A difference of scores as an exponent of 2 is reach(to_log2) times it, then |to_log2| times
+// that (beyond fp32's range: of scores so far apart that the lower one has no weight).
+__device__ __forceinline__ float reach(float to_log2) { return to_log2 < 0.f ? 0x1p127f : 1.f; }
 // What a part of a row counts beside the part with the row's largest score, top (of
 // these the least nb): a difference of scores, however large they are, or of the
 // rounded exponents that the weights were formed with.
 __device__ __forceinline__ float part_weight(const Sum& s, float top, float nb) {
     if (s.m == -INFINITY) return 0.f;
-    return __builtin_amdgcn_exp2f(is_steep(top, s.to_log2) || is_steep(s.m, s.to_log2) ? (s.m - top) * s.to_log2 : nb - s.nb);
+    return __builtin_amdgcn_exp2f(is_steep(top, s.to_log2) || is_steep(s.m, s.to_log2) ? (s.m - top) * reach(s.to_log2) * fabsf(s.to_log2) : nb - s.nb);
 }
 
 // What the first wave has found for the block.
@@ -342,6 +346,7 @@ chunk_attn_kernel(const ChunkArgs a) {
         // q's operand
         u32x4v q[KS][NP];
         float to_log2 = 1.f;
+        bool steep = false;
         typedef RT r8 __attribute__((ext_vector_type(8), aligned(16)));
         r8 qrow[KS];   // as it comes: asked for before the pages are, used once the first tiles are asked for
         if (live) {
@@ -351,12 +356,16 @@ chunk_attn_kernel(const ChunkArgs a) {
         }
         auto form_q = [&] {
             if (!live) return;
-            const float scale = a.scale * kLog2e * kscale;
+            float scale = a.scale * kLog2e * kscale;
+            int back = 127;   // to_log2 is |scale| 2^(back - 127)
+            if (fabsf(scale) == INFINITY) {   // (a quarter of it need not be)
+                scale = a.scale * (0.25f * kLog2e) * kscale;
+                back = 129;
+            }
             if constexpr (NP == 1 && CT == GSDH_KV_F16) {
-                const uint32_t flip = scale < 0.f || (scale == 0.f && __builtin_signbit(scale)) ? 0x80008000u : 0u;
+                const uint32_t flip = __builtin_signbit(scale) ? 0x80008000u : 0u;
 #pragma unroll
                 for (int s = 0; s < KS; s++) q[s][0] = __builtin_bit_cast(u32x4v, qrow[s]) ^ flip;
-                to_log2 = fabsf(scale);
             } else {
                 float most = 0.f;
 #pragma unroll
@@ -366,12 +375,12 @@ chunk_attn_kernel(const ChunkArgs a) {
                 const auto other = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
                 most = fmaxf(__uint_as_float(other[0]), __uint_as_float(other[1]));
                 // by a power of two: fp16 parts keep their bits below 1024, bf16 ones stay
-                // below 2^-9, so that 256 products with finite K stay below 2^127
+                // below 2^-9, so that 256 products with finite K stay below 2^127 (that power
+                // may be subnormal, and its inverse beyond fp32's range)
                 constexpr int kTop = CT == GSDH_KV_BF16 ? -10 : 9;
-                unsigned ex = __float_as_uint(most) >> 23;
-                ex = min(max(ex, 16u), 253u + (unsigned)min(kTop, 1));
-                const float up = copysignf(__uint_as_float((254u + kTop - ex) << 23), scale), down = __uint_as_float((ex - kTop) << 23);
-                to_log2 = fabsf(scale) * down;
+                const int ex = min(max((int)(__float_as_uint(most) >> 23), 16), 254), to = 254 + kTop - ex;
+                back += ex - kTop - 127;
+                const float up = copysignf(__uint_as_float(to > 0 ? (unsigned)to << 23 : 1u << (22 + to)), scale);
 #pragma unroll
                 for (int s = 0; s < KS; s++) {
 #pragma unroll
@@ -383,8 +392,12 @@ chunk_attn_kernel(const ChunkArgs a) {
                     }
                 }
             }
+            to_log2 = fabsf(scale) * __uint_as_float((unsigned)min(back, 254) << 23);
+            if (back > 254) to_log2 *= __uint_as_float((unsigned)(back - 127) << 23);
             // (a scale of 0 stays above it: a masked -inf times it is -inf; one of NaN makes NaN)
             if (to_log2 < FLT_TRUE_MIN) to_log2 = FLT_TRUE_MIN;
+            if (to_log2 == INFINITY && fabsf(scale) != INFINITY) to_log2 = -fminf(fabsf(scale) * __uint_as_float((unsigned)(back - 127) << 23), FLT_MAX);
+            steep = __any(to_log2 < 0.f);
         };
         // P as 2^14 times itself: what lies below fp16's normal range stays exact longer;
         // bf16: over a power of two that is above the number of positions, so that no
@@ -399,11 +412,10 @@ chunk_attn_kernel(const ChunkArgs a) {
         // The running maximum stays unscaled.  A weight is 2^(x to_log2 + nb), nb the
         // rounded top_weight - m to_log2: one fma, whose product is exact, so all of a
         // row's weights are off by the same factor.  Where m to_log2 is beyond 2^20 that
-        // factor would not stay near 1 (or the product overflow): such waves (`steep`)
-        // take 2^((x - m) to_log2 + shift), which weighs the largest 2^top_weight
+        // factor would not stay near 1 (or the product overflow), or to_log2 itself
+        // beyond fp32's range: such waves (`steep`) take 2^((x - m) to_log2 + shift), which weighs the largest 2^top_weight
         // whatever fp32 rounds off the scaled scores.
         float m = -INFINITY, l = 0.f, nb = 0.f, shift = 0.f;
-        bool steep = false;
         constexpr int kDepth = 2;   // operands that are asked for ahead of their products
 
         // page indices of the tiles from `held` on
@@ -529,19 +541,19 @@ chunk_attn_kernel(const ChunkArgs a) {
                 const float nb1 = is ? 0.f : fmaf(-top, to_log2, top_weight), shift1 = is ? top_weight : fmaf(top, to_log2, nb1);
                 // (nothing seen so far: there is nothing to weigh anew)
                 const float f = m == -INFINITY ? 1.f
-                              : __builtin_amdgcn_exp2f(was || is ? fmaf(m - top, to_log2, shift1 - shift) : nb1 - nb);
+                              : __builtin_amdgcn_exp2f(was || is ? fmaf((m - top) * reach(to_log2), fabsf(to_log2), shift1 - shift) : nb1 - nb);
 #pragma unroll
                 for (int d = 0; d < ND; d++) acc[d] *= f;
                 l *= f;
                 m = top;
                 nb = nb1;
                 shift = shift1;
-                steep = __any(is && top != -INFINITY);
+                steep = __any(is && (top != -INFINITY || to_log2 < 0.f));
             }
             if (steep) {   // the weights' exponents in place of the scores
-                const float base = m == -INFINITY ? 0.f : m;
+                const float base = m == -INFINITY ? 0.f : m, far = reach(to_log2), per = fabsf(to_log2);
 #pragma unroll
-                for (int e = 0; e < 16 * N; e++) xs[e / 16][e % 16] = fmaf(xs[e / 16][e % 16] - base, to_log2, shift);
+                for (int e = 0; e < 16 * N; e++) xs[e / 16][e % 16] = fmaf((xs[e / 16][e % 16] - base) * far, per, shift);
             } else {
 #pragma unroll
                 for (int e = 0; e < 16 * N; e++) xs[e / 16][e % 16] = fmaf(xs[e / 16][e % 16], to_log2, nb);
