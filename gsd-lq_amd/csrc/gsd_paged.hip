@@ -501,7 +501,9 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) paged_attn_ker
         }
 
         float4v acc[NT];
-        float m = -INFINITY, l = 0.f, to_log2 = 1.f;   // m: the largest unscaled score; times to_log2: as an exponent of 2
+        // m: the largest unscaled score; times reach and to_log2: as an exponent of 2 (reach
+        // 1, but 2^127 where the factor is beyond fp32's range)
+        float m = -INFINITY, l = 0.f, to_log2 = 1.f, reach = 1.f;
 #pragma unroll
         for (int t = 0; t < NT; t++) acc[t] = float4v{0.f, 0.f, 0.f, 0.f};
         if (have && s.mine < s.t1) {
@@ -521,16 +523,26 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) paged_attn_ker
                         most = fmaxf(most, fabsf(x[i][e]));
                     }
                 }
-                // 2^(kTop - exponent of the largest), kept within the range of normal floats
+                // 2^(kTop - exponent of the largest): it may be subnormal, and its inverse
+                // times the scale beyond fp32's range
                 constexpr int kTop = DT == GSDH_KV_BF16 ? -10 : 9;
-                unsigned ex = __float_as_uint(max_over_groups(most)) >> 23;
-                ex = min(max(ex, 16u), 253u + (unsigned)min(kTop, 1));
+                const int ex = min(max((int)(__float_as_uint(max_over_groups(most)) >> 23), 16), 254), to = 254 + kTop - ex;
                 // (a negative scale is in q's sign; one of 0 stays above it, so that a
                 // masked -inf times it stays -inf, and no farther than 2^-149: a bf16
                 // row's unscaled scores reach 2^127)
-                const float scale = a.scale * kLog2e * kscale;
-                const float up = copysignf(__uint_as_float((254u + kTop - ex) << 23), scale), down = __uint_as_float((ex - kTop) << 23);
-                to_log2 = fabsf(scale) * down;
+                float scale = a.scale * kLog2e * kscale;
+                int back = ex - kTop;   // to_log2 is |scale| 2^(back - 127)
+                if (fabsf(scale) == INFINITY) {   // (a quarter of it need not be)
+                    scale = a.scale * (0.25f * kLog2e) * kscale;
+                    back += 2;
+                }
+                const float up = copysignf(__uint_as_float(to > 0 ? (unsigned)to << 23 : 1u << (22 + to)), scale);
+                to_log2 = fabsf(scale) * __uint_as_float((unsigned)min(back, 254) << 23);
+                if (back > 254) to_log2 *= __uint_as_float((unsigned)(back - 127) << 23);
+                if (to_log2 == INFINITY && fabsf(scale) != INFINITY) {
+                    to_log2 = fminf(fabsf(scale) * __uint_as_float((unsigned)(back - 127) << 23), FLT_MAX);
+                    reach = 0x1p127f;
+                }
                 if (to_log2 < FLT_TRUE_MIN) to_log2 = FLT_TRUE_MIN;
 #pragma unroll
                 for (int i = 0; i < T::KS; i++) {
@@ -547,6 +559,7 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) paged_attn_ker
             // P as 2^14 times itself: the parts below fp16's normal range stay exact; bf16:
             // as P over a power of two that is above the row's number of positions
             const float weight_of_top = DT == GSDH_KV_BF16 ? (float)(__builtin_clz((unsigned)(s.end - s.first)) - 32) : 14.f;
+            const bool far = __any(reach != 1.f);
             int ahead = pages_from(s, s.mine + kAhead * kWaves), place = 0;   // the next kAhead tiles' pages; the next tile among the held
             for (int t = s.mine; t < s.t1; t += kWaves) {
                 float4v xs[H];
@@ -587,7 +600,7 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) paged_attn_ker
                 for (int e = 0; e < 4 * H; e++) top = fmaxf(top, x[e]);
                 top = fmaxf(m, max_over_groups(top));
                 if (__any(top > m)) {
-                    const float f = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - top) * to_log2);
+                    const float f = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - top) * reach * to_log2);
 #pragma unroll
                     for (int n = 0; n < NT; n++) acc[n] *= f;
                     l *= f;
@@ -595,8 +608,14 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) paged_attn_ker
                 }
                 const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
+                for (int e = 0; e < 4 * H; e++) x[e] -= base;
+                if (far) {
+#pragma unroll
+                    for (int e = 0; e < 4 * H; e++) x[e] *= reach;
+                }
+#pragma unroll
                 for (int e = 0; e < 4 * H; e++) {
-                    x[e] = __builtin_amdgcn_exp2f(fmaf(x[e] - base, to_log2, weight_of_top));
+                    x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], to_log2, weight_of_top));
                     l += x[e];
                 }
                 const Parts<DT, 4 * H> p = split<DT, 4 * H>(x);
@@ -631,8 +650,9 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) paged_attn_ker
         }
 
         if (have) {
-            // (scores beyond fp32's range stay finite: a difference of two is a number)
-            if (m != -INFINITY) m = fminf(fmaxf(m * to_log2, -FLT_MAX), FLT_MAX);
+            // (scores beyond fp32's range stay finite: a difference of two is a number, and
+            // parts of a row whose largest are both beyond it count alike)
+            if (m != -INFINITY) m = fminf(fmaxf(m * reach * to_log2, -FLT_MAX), FLT_MAX);
             l = sum_over_groups(l);
             if (__any(lost)) {
                 l = __builtin_nanf("");
