@@ -400,9 +400,9 @@ chunk_attn_kernel(const ChunkArgs a) {
             steep = __any(to_log2 < 0.f);
         };
         // P as 2^14 times itself: what lies below fp16's normal range stays exact longer;
-        // bf16: over a power of two that is above the number of positions, so that no
-        // sum of finite V passes fp32's range
-        const float top_weight = CT == GSDH_KV_BF16 ? (float)(__builtin_clz((unsigned)(it.end - it.first)) - 32) : 14.f;
+        // bf16: over a power of two that is more than twice the number of positions, so that
+        // no sum of finite V passes fp32's range (nb's rounding makes weights up to 2^(1/16) larger)
+        const float top_weight = CT == GSDH_KV_BF16 ? (float)(__builtin_clz((unsigned)(it.end - it.first)) - 33) : 14.f;
 
         float16v acc[ND];
 #pragma unroll

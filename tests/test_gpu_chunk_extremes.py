@@ -1,5 +1,5 @@
 """gsdh_paged_chunk_attention where single numbers are extreme: rows near the
-largest finite bf16, scores and scales beyond fp32's range."""
+largest finite bf16, V there too, scores and scales beyond fp32's range."""
 import numpy as np
 import pytest
 
@@ -68,3 +68,21 @@ def test_scores_beyond_fp32(lib, kind, q, scale, few_rows):
     want, mag, _, _, seen, _ = attend_chunks(c, 0, qs, [0], [0, m], scale)
     assert np.isfinite(got).all()
     assert (np.abs(got - want) <= STEP * (seen * 5 / 8 + 160)[..., None] * mag + 1e-30).all()
+
+
+@pytest.mark.parametrize("few_rows", [False, True])
+@pytest.mark.parametrize("rows", ["f32", "bf16"])
+def test_sums_of_the_largest_v(lib, rows, few_rows):
+    """Rows whose scores are all alike, and far from 0, average V rows of the largest finite bf16: that value, although
+    the weights of a row, all off by one factor, add up to nearly all that their place leaves them."""
+    banner(f"chunks bf16 {rows}: the largest V")
+    rng, hd, n, m = np.random.default_rng(1), 64, 1023, 60
+    most = (2 - 2.0 ** -7) * 2.0 ** 127
+    c = chunk_cache("bf16", [n], 16, 1, hd, False, rng, lambda r, s: np.ones(s, np.float32), few_rows=few_rows)
+    c.set_values(1, 0, 0, np.arange(n), np.full((n, 1, hd), most, np.float32))
+    c.upload()
+    q = np.zeros((m, 16, hd), np.float32)
+    q[:, :, 0] = (128 + rng.integers(0, 50, (m, 16))) * 4096.0   # (scores of 5.2e5 to 7.2e5: up to 2^19.99 as exponents of 2)
+    got = run_chunks(c, 0, q, rows, [0], [0, m], 1.0)
+    assert np.isfinite(got).all()
+    assert np.abs(got / most - 1).max() <= STEP * (n * 5 / 8 + 160) + (2.02 * HALF[rows] if rows == "bf16" else 0)
