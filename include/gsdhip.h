@@ -283,7 +283,7 @@ enum { GSDH_ROWS_F32 = 0, GSDH_ROWS_F16 = 1, GSDH_ROWS_BF16 = 2 };
  * fp32 over any cache, the cache's own 16-bit type, or either over an e4m3 cache;
  * row t at q + t * q_stride, n_heads x head_dim.  With fp32 rows the result is
  * exact to fp32's rounding; with 16-bit rows the weights are rounded once to the
- * type, sums and statistics stay fp32.
+ * type, and so is what their sum, in fp32, adds up; statistics stay fp32.
  * A negative seqs[i] is padding, and rows that no chunk names stay as they were, as
  * do those of a chunk whose starts fall or lie outside 0 .. n_tokens
  * (GSDH_PAGES_BAD_INDEX).  A chunk of 0 rows is one without work.  A chunk of a

@@ -3,7 +3,7 @@ largest finite bf16, V there too, scores and scales beyond fp32's range."""
 import numpy as np
 import pytest
 
-from chunk_util import HALF, STEP, attend_chunks, chunk_cache, run_chunks
+from chunk_util import HALF, STEP, attend_chunks, chunk_cache, rounded, run_chunks
 from gpu_util import banner
 from paged_util import grid, normal
 
@@ -86,3 +86,16 @@ def test_sums_of_the_largest_v(lib, rows, few_rows):
     got = run_chunks(c, 0, q, rows, [0], [0, m], 1.0)
     assert np.isfinite(got).all()
     assert np.abs(got / most - 1).max() <= STEP * (n * 5 / 8 + 160) + (2.02 * HALF[rows] if rows == "bf16" else 0)
+
+
+@pytest.mark.parametrize("few_rows", [False, True])
+@pytest.mark.parametrize("kind,rows", [("f16", "f16"), ("bf16", "bf16"), ("e4m3", "f16"), ("e4m3", "bf16")])
+def test_one_position_is_its_v(lib, kind, rows, few_rows):
+    """16-bit rows that see one position, whose rounded weight is any of 16 bits, give its V row: weight and sum are the
+    same number, and what the quotient and two products round in fp32 is far below half a step of the row."""
+    banner(f"chunks {kind} {rows}: one position")
+    rng, hd, n = np.random.default_rng(3), 64, 1000
+    c = chunk_cache(kind, [n], 16, 1, hd, False, rng, normal, few_rows=few_rows)
+    q = rounded(normal(rng, (n, 4, hd)) * np.float32(2.0 ** 12), rows).astype(np.float32)
+    got = run_chunks(c, 0, q, rows, [0], [0, n], 1.0, window=1)
+    assert np.array_equal(got, np.repeat(c.values(1, 0, 0, np.arange(n)), 4, 1))
