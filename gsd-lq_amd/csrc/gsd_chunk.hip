@@ -209,7 +209,7 @@ __device__ __forceinline__ float16v mma(const u32x4v a, const u32x4v b, float16v
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
 }
 
-// two fp32 values as words of operands: parts whose sum they are (22 or 24 bits), or (16-bit rows) rounded once
+// two fp32 values as words of operands: parts whose sum they are (23 or 24 bits), or (16-bit rows) rounded once
 template <int CT, int NP>
 __device__ __forceinline__ void operand_words(float x, float y, uint32_t (&w)[NP]) {
     typedef _Float16 half2 __attribute__((ext_vector_type(2)));
@@ -219,9 +219,11 @@ __device__ __forceinline__ void operand_words(float x, float y, uint32_t (&w)[NP
     } else if constexpr (NP == 1) {
         w[0] = __builtin_bit_cast(uint32_t, half2{(_Float16)x, (_Float16)y});
     } else if constexpr (NP == 2) {
-        // 11 bits cut off, 11 bits of the rest: two conversions of pairs and a mixed fma per value
-        const half2 h = __builtin_bit_cast(half2, __builtin_amdgcn_cvt_pkrtz(x, y));
-        w[0] = __builtin_bit_cast(uint32_t, h);
+        // 11 bits, rounded, and 11 of the rest: two conversions of pairs and a mixed fma per value
+        // (of words that the compiler cannot trace: it would convert each value once more)
+        w[0] = __builtin_bit_cast(uint32_t, half2{(_Float16)x, (_Float16)y});
+        __asm__("" : "+v"(w[0]));
+        const half2 h = __builtin_bit_cast(half2, w[0]);
         w[1] = __builtin_bit_cast(uint32_t, half2{(_Float16)__builtin_fmaf((float)h[0], -1.f, x), (_Float16)__builtin_fmaf((float)h[1], -1.f, y)});
     } else {
         // 8 + 8 + 8 bits cut off, exact

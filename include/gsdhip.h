@@ -281,8 +281,8 @@ enum { GSDH_ROWS_F32 = 0, GSDH_ROWS_F16 = 1, GSDH_ROWS_BF16 = 2 };
  * max(0, p + 1 - window) .. p (window 0: all of them).  starts: int [n + 1],
  * rising, within 0 .. n_tokens.  Rows of q and out are of `dtype`, RoPE applied:
  * fp32 over any cache, the cache's own 16-bit type, or either over an e4m3 cache;
- * row t at q + t * q_stride, n_heads x head_dim.  With fp32 rows the result is
- * exact to fp32's rounding; with 16-bit rows the weights are rounded once to the
+ * row t at q + t * q_stride, n_heads x head_dim.  With fp32 rows q and the weights
+ * keep 23 bits (24 over bf16), sums are in fp32; with 16-bit rows the weights are rounded once to the
  * type, and so is what their sum, in fp32, adds up; statistics stay fp32.
  * A negative seqs[i] is padding, and rows that no chunk names stay as they were, as
  * do those of a chunk whose starts fall or lie outside 0 .. n_tokens

@@ -1,5 +1,6 @@
 """gsdh_paged_chunk_attention where single numbers are extreme: rows near the
-largest finite bf16, V there too, scores and scales beyond fp32's range."""
+largest finite bf16, V there too, scores and scales beyond fp32's range, and the bits
+that weights keep."""
 import numpy as np
 import pytest
 
@@ -99,3 +100,20 @@ def test_one_position_is_its_v(lib, kind, rows, few_rows):
     q = rounded(normal(rng, (n, 4, hd)) * np.float32(2.0 ** 12), rows).astype(np.float32)
     got = run_chunks(c, 0, q, rows, [0], [0, n], 1.0, window=1)
     assert np.array_equal(got, np.repeat(c.values(1, 0, 0, np.arange(n)), 4, 1))
+
+
+@pytest.mark.parametrize("few_rows", [False, True])
+@pytest.mark.parametrize("kind", ["f16", "bf16", "e4m3"])
+def test_bits_of_a_weight(lib, kind, few_rows):
+    """Rows that see one position give its V row: (a + b) V / l, a + b the 16-bit parts of the weight l, whose bits are any
+    (the exponent's rounding is not that of the product).  Off by what the parts leave of l, 2^-23 (a rounded to 11 bits
+    leaves 2^-11 of its power of two, b half of its own last bit, 2^-12 of that; three bf16 parts leave nothing), by one
+    rounding of the sum (two of three parts), of 1 / l and of the product: five half steps."""
+    banner(f"chunks {kind}: bits of a weight")
+    rng, hd, n = np.random.default_rng(2), 64, 1000
+    c = chunk_cache(kind, [n], 16, 1, hd, False, rng, normal, few_rows=few_rows)
+    q = normal(rng, (n, 4, hd)) * np.float32(2.0 ** 14)
+    got = run_chunks(c, 0, q, "f32", [0], [0, n], 1.0, window=1)
+    want = np.repeat(c.values(1, 0, 0, np.arange(n)), 4, 1)
+    off = np.abs(got - want) / np.where(want == 0, 1, np.abs(want)) / STEP
+    assert off.max() <= 5.001, off.max()
