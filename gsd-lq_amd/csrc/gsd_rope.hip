@@ -277,17 +277,19 @@ int gsdh_rope_frequencies(int kind, double theta, int rotary_dim, double factor,
         return fail(-1, "%s: a context of %g positions, turns from %g to %g", who, context, low, high);
     if (!freqs) return fail(-1, "%s: null buffer", who);
     if (kind == GSDH_ROPE_NTK) theta *= std::pow(factor, (double)rotary_dim / (rotary_dim - 2));
-    for (int i = 0; i < rotary_dim / 2; i++) {
-        double f = std::pow(theta, -2.0 * i / rotary_dim);
-        if (kind == GSDH_ROPE_LINEAR) f /= factor;
-        if (kind == GSDH_ROPE_BY_PARTS) {
-            const double turns = context * f * 0.15915494309189533577;   // 1 / 2 pi
-            double keep = (turns - low) / (high - low);
-            keep = keep < 0 ? 0 : keep > 1 ? 1 : keep;
-            f = keep * f + (1 - keep) * (f / factor);
-        }
-        freqs[i] = f;
-    }
+    if (std::isinf(theta)) return fail(-1, "%s: frequencies of an infinite theta", who);
+    auto frequency = [&](int i) {
+        const double f = std::pow(theta, -2.0 * i / rotary_dim);
+        if (kind == GSDH_ROPE_LINEAR) return f / factor;
+        if (kind != GSDH_ROPE_BY_PARTS) return f;
+        const double turns = context * f * 0.15915494309189533577;   // 1 / 2 pi
+        double keep = (turns - low) / (high - low);
+        keep = keep < 0 ? 0 : keep > 1 ? 1 : keep;
+        return keep * f + (1 - keep) * (f / factor);
+    };
+    for (int i = 0; i < rotary_dim / 2; i++)
+        if (!std::isfinite(frequency(i))) return fail(-1, "%s: frequency %d is not a finite number", who, i);
+    for (int i = 0; i < rotary_dim / 2; i++) freqs[i] = frequency(i);
     return 0;
 }
 

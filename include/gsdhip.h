@@ -340,7 +340,8 @@ typedef struct gsdh_rope {
  *   NTK       with theta * factor^(rotary_dim / (rotary_dim - 2))
  *   BY_PARTS  f_i where it makes `high` or more turns in `context` positions, f_i /
  *             factor where it makes `low` or fewer, between them linear in the turns
- * (arguments that the kind does not name are not looked at). */
+ * (arguments that the kind does not name are not looked at; arguments that make a
+ * frequency infinite or no number are refused, freqs stays as it was). */
 enum { GSDH_ROPE_PLAIN = 0, GSDH_ROPE_LINEAR = 1, GSDH_ROPE_NTK = 2, GSDH_ROPE_BY_PARTS = 3 };
 int gsdh_rope_frequencies(int kind, double theta, int rotary_dim, double factor, double context, double low,
                           double high, double* freqs);
