@@ -1,13 +1,13 @@
 """gsdh_rope_rows and gsdh_paged_rope_append over the rows of prompts: calls of more
 blocks than the chip takes at once, whose threads have four items each, against the
 rotation in 64 bits (tolerances as in test_gpu_rope) and, bit for bit, the same rows
-in calls of a few tokens."""
+in calls of a few tokens; and the append beside the store with a table."""
 import numpy as np
 import pytest
 
 from chunk_util import HALF, rounded
-from gpu_util import banner
-from paged_util import Cache, decode, grid, normal
+from gpu_util import D, H, banner, p
+from paged_util import Cache, decode, grid, ints, normal
 from test_gpu_rope import KV_HALF, LEAST, append, frequencies, run_rows, turn, within
 
 pytestmark = pytest.mark.gpu
@@ -104,3 +104,32 @@ def test_prompts_into_the_cache(lib, kind, rows, heads, kv, hd, rd, interleaved,
         part = slice(t, t + 100)
         assert np.array_equal(got[part], append(c, 1, rows, q[part], k[part], v[part], seqs[part], pos[part], f, interleaved, 1.1))
     assert all(np.array_equal(a, b) for a, b in zip(pools, (c.download("k"), c.download("v"))))
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16", "e4m3"])
+@pytest.mark.parametrize("interleaved", [0, 1])
+def test_append_is_the_store_on_quarter_turns(lib, kind, interleaved):
+    """Frequencies of whole quarter turns per position, another for each pair.  The table's cosines and sines are 0, 1 and
+    -1; an angle that fp64 forms is off by less than 2^-44 of a turn, which nothing shows in fp32 beside 1/4 and 1/2, nor
+    2 pi 2^-44 of a row's element beside another within twice of it.  So K, V and q are the store's, bit for bit."""
+    rng = np.random.default_rng(7)
+    n, heads, kv, hd = 60, 4, 2, 64
+    c = Cache(kind, 1, 8, 16, kv, hd, False, 1).fill([n], rng, grid)
+    pos, quarters = np.arange(n), 1 + np.arange(hd // 2) % 7
+    q, k, v = ((rng.uniform(1, 2, (n, h, hd)) * rng.choice([-1, 1], (n, h, hd))).astype(np.float32) for h in (heads, kv, kv))
+    got = append(c, 0, "f32", q, k, v, [0] * n, pos, quarters * (np.pi / 2), interleaved)
+    one = c.download("k"), c.download("v")
+    turns = pos[:, None] * quarters % 4
+    table = D(np.stack([np.array([1, 0, -1, 0])[turns], np.array([0, 1, 0, -1])[turns]], -1).astype(np.float32))
+    c.upload()
+    dq, dk, dv, do, ds, dp = D(q), D(k), D(v), D(q), ints([0] * n), ints(pos)
+    w, kw = heads * hd, kv * hd
+    lib.gsdh_paged_rope_store(None, c.at, 0, p(dq), w, p(dk), kw, p(dv), kw, p(do), w, p(ds), p(dp), n, heads, p(table), n, interleaved)
+    assert np.array_equal(one[0], c.download("k")) and np.array_equal(one[1], c.download("v"))
+    assert np.array_equal(got, H(do, np.float32, n * w).reshape(n, heads, hd).astype(np.float64))
+    # (it turned: the second half of a turn is the negative of what came)
+    half = (turns == 2)[:, None, :]
+    i, j = (np.arange(0, hd, 2), np.arange(1, hd, 2)) if interleaved else (np.arange(hd // 2), np.arange(hd // 2, hd))
+    for d in (i, j):
+        at = np.broadcast_to(half, got[..., d].shape)
+        assert at.any() and np.array_equal(got[..., d][at], -q[..., d][at])
