@@ -30,7 +30,7 @@ struct Word {
 };
 
 // A logit x of token v becomes
-//   x / r or x r (whichever is less)   if v occurs in the history (r: repetition)
+//   x / r where x > 0, else x r        if v occurs in the history (r: repetition)
 //   - frequency * count - presence     if it occurs in the answer, count times
 //   + bias
 //   -inf                               if the mask forbids it
