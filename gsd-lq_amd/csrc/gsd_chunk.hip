@@ -24,7 +24,9 @@ constexpr int kRuns = kPos / 8;      // its runs of eight positions: a page is a
 // rows is that often more, by the products of its rows' parts (measured: a tile of
 // 256 rows 2.1 us in 16 bits, 4.2 us in two parts), and an item's start and end, waits
 // under load, are 20 us (a prompt of 4096 tokens took 307 us with 13 us in its place; 16
-// chunks of 5 tokens take 68 us, with 10 us in its place 76, with 32 us 70).
+// chunks of 5 tokens take 68 us, with 10 us in its place 76, with 32 us 70).  All of it
+// at 128 dims, 32 heads over 8, fp32 rows over fp16; other head dims and types go by the
+// same costs, which only deal the work out.
 constexpr int kCost = 4400;
 constexpr int kWhole = 4;            // an item of so few tiles is not cut
 constexpr int kLeastSpan = 2048;     // the least a block takes
@@ -55,7 +57,9 @@ constexpr int kJoinFew = 4, kJoinMany = 16;
 // fp32 rows meet the cache's 16-bit rows as sums of 16-bit parts, as in the
 // decode attention (two fp16 or three bf16 parts of q and P); rows of 16 bits
 // are exact as they are, and their P is rounded once to their type: half a step
-// of each weight, as much as the rounding of the output.
+// of each weight, as much as the rounding of the output (bf16, 32768 positions: off by
+// 2.2e-3 of the result, where the output's rounding alone is 1.7e-3; a second part of P
+// would be half as many products again).
 // ---------------------------------------------------------------------------
 struct Joint {   // of an item that several blocks share, at its first one's place
     int parts;   // 0: none
@@ -310,12 +314,20 @@ constexpr unsigned tiles_bytes() {
 // read the same tiles for.  A call takes one way for all its chunks (is_few, with
 // both ways' times); in one kernel both had registers spilled in their loops.
 //
-// Bound by the matrix cores for prompts: 2048 tokens of 32 heads over 8 of 128 dims at the
-// end of 32768 positions, bf16, 1079 us, 1.0 PFLOP/s of products (a library's product of
-// 8192^3 gets 1.2 on the same card, whose clock falls under both: 1.8 GHz in this
-// kernel); 4096 tokens of fp32 rows over fp16 284 us, 0.97 PFLOP/s of products, two for
-// each.  By memory for few rows: 16 chunks of 5 tokens over up to 8191 positions (199 MB)
-// 68 us, of which the stream is 36.
+// Bound by the products and the weights between them, which take turns more than they
+// overlap, for prompts: 2048 tokens of 32 heads over 8 of 128 dims at the end of 32768
+// positions, bf16, 1056 us, 1.0 PFLOP/s of products (a library's product of 8192^3 gets
+// 1.2 on the same card, whose clock falls under both: 1.8 GHz in this kernel), the matrix
+// cores busy for 46 % of the cycles and the VALU for 44 %; 4096 tokens of fp32 rows over
+// fp16 285 us, 0.97 PFLOP/s of products, two for each.  By memory for few rows: 16 chunks
+// of 5 tokens over up to 8191 positions (199 MB) 68 us, of which the stream is 36.
+//
+// Nothing is spilled in the loops at 64 dims, at 128 over fp16 and bf16 and for many 16-bit
+// rows over e4m3, and with 16-bit rows of 256 over fp16 and bf16.  Elsewhere some is: at 256
+// with fp32 rows 10 to 32 reloads stand beside a pass of score products, with 16-bit rows
+// over e4m3 7 to 16; at 128 over e4m3 1 to 6 with fp32 rows, and up to 10 beside the loads of
+// few rows.  4096 tokens of 16 heads over 2 of 256 dims take 278 us in fp16, 420 of fp32
+// rows over fp16, 642 over bf16, 607 over e4m3 (products alone: 115, 229, 344, 229).
 template <int HD, int DT, typename RT, bool FEW>
 __global__ void __launch_bounds__((64 * waves_of<HD, Kinds<DT, RT>::NP>()), (waves_of<HD, Kinds<DT, RT>::NP>() / 4))
 chunk_attn_kernel(const ChunkArgs a) {
@@ -1064,7 +1076,8 @@ bool chunk_shape(const gsdh_paged_cache& c, int n, int n_tokens, int n_heads) {
 // (the lengths themselves are on the device).  Both ways' times, few and many rows'
 // (us, 32 heads over 8 of 128 dims, fp32 rows over fp16): 16 chunks over 3400 positions
 // of 20 rows 61 and 73, of 64 rows 72 and 78, of 96 rows 94 and 83; of 20 rows over 256
-// positions 26 and 21, over 1024 35 and 37, over 4096 69 and 84.
+// positions 26 and 21, over 1024 35 and 37, over 4096 69 and 84.  Other head dims and
+// types go by the same rule.
 bool is_few(const ChunkArgs& a) {
     return (int64_t)a.n_tokens * a.group <= (int64_t)2 * kWaveRows * a.n && (int64_t)a.c.table_width * a.c.page_size >= 1024;
 }
