@@ -222,6 +222,7 @@ __device__ __forceinline__ void operand_words(float x, float y, uint32_t (&w)[NP
         w[0] = __builtin_bit_cast(uint32_t, bf2{(__bf16)x, (__bf16)y});
     } else if constexpr (NP == 1) {
         w[0] = __builtin_bit_cast(uint32_t, half2{(_Float16)x, (_Float16)y});
+        __asm__("" : "+v"(w[0]));   // (the compiler would convert each value once more where its rounded one is summed)
     } else if constexpr (NP == 2) {
         // 11 bits, rounded, and 11 of the rest: two conversions of pairs and a mixed fma per value
         // (of words that the compiler cannot trace: it would convert each value once more)
@@ -241,21 +242,20 @@ __device__ __forceinline__ void operand_words(float x, float y, uint32_t (&w)[NP
     }
 }
 
-// l + x + y of two weights.  Those that are rounded to 16 bits (w) add up as they are
-// multiplied, so an average of V lies among them, and one of equal V is that V.  (The
-// bf16 dot product with ones: off by 1.5 units in the last place at most, measured; 2048
-// tokens at the end of 32768 positions 1089 us, 1138 with two unpacked sums.)
-template <int CT, int NP>
-__device__ __forceinline__ float add_weights(float l, float x, float y, uint32_t w) {
-    if constexpr (NP > 1) {
-        return l + (x + y);
-    } else if constexpr (CT == GSDH_KV_BF16) {
+// l and two weights that are rounded to 16 bits (w): they add up as they are multiplied,
+// so an average of V lies among them, and one of equal V is that V.  bf16: by a dot product
+// with ones, off by 1.5 units in the last place at most, measured (2048 tokens at the end of
+// 32768 positions 1089 us, 1138 with two unpacked sums); fp16's own is off downwards, 0.2 units
+// on average, so a mixed fma in its place.
+template <int CT>
+__device__ __forceinline__ float add_rounded(float l, uint32_t w, float one) {
+    if constexpr (CT == GSDH_KV_BF16) {
         typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
         return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf2, w), __builtin_bit_cast(bf2, 0x3F803F80u), l, false);
     } else {
         typedef _Float16 half2 __attribute__((ext_vector_type(2)));
         const half2 h = __builtin_bit_cast(half2, w);
-        return l + ((float)h[0] + (float)h[1]);
+        return l + __builtin_fmaf((float)h[0], one, (float)h[1]);
     }
 }
 
@@ -379,6 +379,8 @@ chunk_attn_kernel(const ChunkArgs a) {
         u32x4v q[KS][NP];
         float to_log2 = 1.f;
         bool steep = false;
+        float one = 1.f;   // (that the compiler cannot trace: a mixed fma by 1 would become conversions and a sum)
+        __asm__ volatile("" : "+s"(one));
         typedef RT r8 __attribute__((ext_vector_type(8), aligned(16)));
         r8 qrow[KS];   // as it comes: asked for before the pages are, used once the first tiles are asked for
         if (live) {
@@ -568,7 +570,14 @@ chunk_attn_kernel(const ChunkArgs a) {
             for (int e = 0; e < 16 * N; e++) top = fmaxf(top, xs[e / 16][e % 16]);
             const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
             top = fmaxf(m, fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])));
+            // (its reach is formed where it is needed, not kept beside the products)
+            auto factor = [&] {
+                float c = to_log2;
+                __asm__ volatile("" : "+v"(c));
+                return c;
+            };
             if (__any(top > m)) {
+                const float to_log2 = factor();
                 const bool was = is_steep(m, to_log2), is = is_steep(top, to_log2);
                 const float nb1 = is ? 0.f : fmaf(-top, to_log2, top_weight), shift1 = is ? top_weight : fmaf(top, to_log2, nb1);
                 // (nothing seen so far: there is nothing to weigh anew)
@@ -583,7 +592,7 @@ chunk_attn_kernel(const ChunkArgs a) {
                 steep = __any(is && (top != -INFINITY || to_log2 < 0.f));
             }
             if (steep) {   // the weights' exponents in place of the scores
-                const float base = m == -INFINITY ? 0.f : m, far = reach(to_log2), per = fabsf(to_log2);
+                const float base = m == -INFINITY ? 0.f : m, c = factor(), far = reach(c), per = fabsf(c);
 #pragma unroll
                 for (int e = 0; e < 16 * N; e++) xs[e / 16][e % 16] = fmaf((xs[e / 16][e % 16] - base) * far, per, shift);
             } else {
@@ -596,8 +605,9 @@ chunk_attn_kernel(const ChunkArgs a) {
             auto weights = [&](int s, int i) {
                 const float x = __builtin_amdgcn_exp2f(xs[s / 2][8 * (s % 2) + 2 * i]), y = __builtin_amdgcn_exp2f(xs[s / 2][8 * (s % 2) + 2 * i + 1]);
                 uint32_t w[NP];
+                if constexpr (NP > 1) l += x + y;
                 operand_words<CT, NP>(x, y, w);
-                l = add_weights<CT, NP>(l, x, y, w[0]);
+                if constexpr (NP == 1) l = add_rounded<CT>(l, w[0], one);
 #pragma unroll
                 for (int p = 0; p < NP; p++) pw[s % 2][p][i] = w[p];
             };
