@@ -316,18 +316,19 @@ constexpr unsigned tiles_bytes() {
 //
 // Bound by the products and the weights between them, which take turns more than they
 // overlap, for prompts: 2048 tokens of 32 heads over 8 of 128 dims at the end of 32768
-// positions, bf16, 1056 us, 1.0 PFLOP/s of products (a library's product of 8192^3 gets
-// 1.2 on the same card, whose clock falls under both: 1.8 GHz in this kernel), the matrix
-// cores busy for 46 % of the cycles and the VALU for 44 %; 4096 tokens of fp32 rows over
-// fp16 285 us, 0.97 PFLOP/s of products, two for each.  By memory for few rows: 16 chunks
-// of 5 tokens over up to 8191 positions (199 MB) 68 us, of which the stream is 36.
+// positions, bf16, 1056 to 1095 us on several cards, 1.0 PFLOP/s of products (a library's
+// product of 8192^3 gets 1.2, and the clock falls under both: 1.8 GHz in this kernel), the
+// matrix cores busy for 46 % of the cycles and the VALU for 44 %; 4096 tokens of fp32 rows
+// over fp16 285 to 297 us, 0.94 to 0.97 PFLOP/s, two products for each.  By memory for few
+// rows: 16 chunks of 5 tokens over up to 8191 positions (199 MB) 68 us, of which the stream
+// is 36.
 //
 // Nothing is spilled in the loops at 64 dims, at 128 over fp16 and bf16 and for many 16-bit
 // rows over e4m3, and with 16-bit rows of 256 over fp16 and bf16.  Elsewhere some is: at 256
 // with fp32 rows 10 to 32 reloads stand beside a pass of score products, with 16-bit rows
-// over e4m3 7 to 16; at 128 over e4m3 1 to 6 with fp32 rows, and up to 10 beside the loads of
-// few rows.  4096 tokens of 16 heads over 2 of 256 dims take 278 us in fp16, 420 of fp32
-// rows over fp16, 642 over bf16, 607 over e4m3 (products alone: 115, 229, 344, 229).
+// over e4m3 7 to 16, at 128 over e4m3 1 to 5 with fp32 rows; and beside the loads of few rows
+// over e4m3 up to 26.  4096 tokens of 16 heads over 2 of 256 dims take 279 us in fp16, 425 of fp32
+// rows over fp16, 647 over bf16, 609 over e4m3 (products alone: 115, 229, 344, 229).
 template <int HD, int DT, typename RT, bool FEW>
 __global__ void __launch_bounds__((64 * waves_of<HD, Kinds<DT, RT>::NP>()), (waves_of<HD, Kinds<DT, RT>::NP>() / 4))
 chunk_attn_kernel(const ChunkArgs a) {
