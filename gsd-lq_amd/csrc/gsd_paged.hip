@@ -650,9 +650,19 @@ __global__ void __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) paged_attn_ker
         }
 
         if (have) {
-            // (scores beyond fp32's range stay finite: a difference of two is a number, and
-            // parts of a row whose largest are both beyond it count alike)
-            if (m != -INFINITY) m = fminf(fmaxf(m * reach * to_log2, -FLT_MAX), FLT_MAX);
+            // Parts of a row meet by their largest scores as exponents of 2.  Those beyond 2^100
+            // go by the unscaled score's bits, which rise with it, from 2^100 on: finite, and 2^77
+            // apart or more but where they agree to 2^-15 of themselves (below 2^108 a step is 2^84,
+            // of 2^7 bits; all of fp32's positive numbers have 2^31).
+            if (m != -INFINITY) {
+                const float y = m * reach * to_log2;
+                if (fabsf(y) > 0x1p100f) {
+                    const int first = (int)__float_as_uint(0x1p100f / reach / to_log2), at = (int)__float_as_uint(fabsf(m));
+                    m = copysignf(0x1p100f + (float)max(at - first, 0) * 0x1p77f, y);
+                } else {
+                    m = y;
+                }
+            }
             l = sum_over_groups(l);
             if (__any(lost)) {
                 l = __builtin_nanf("");
